@@ -24,7 +24,7 @@ INCLUDE = HERE.parent / "include"
 
 FMT_NF4, FMT_MXFP4 = 0, 1
 OP_FWD, OP_DGRAD = 0, 1
-X_BF16, X_FP16 = 0, 1
+X_BF16, X_FP16, X_FP32 = 0, 1, 2
 S_F32, S_BF16, S_E8M0 = 0, 1, 2
 PATH_AUTO, PATH_STREAM, PATH_TENSOR = 0, 1, 2
 SPLITK_SHIFT = 8
@@ -46,11 +46,11 @@ _lib = None
 _lock = threading.Lock()
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-              "-shared", "-Xcompiler", "-fPIC"]
+              "-shared", "-Xcompiler", "-fPIC", "-t", "0"]
 
 
 def sources():
-    return sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h"))
+    return sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + sorted(INCLUDE.glob("*.h"))
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
@@ -149,6 +149,14 @@ def _declare(lib):
     lib.gnf4b_gather_rows_by_id.argtypes = [vp, i64, i32, vp, i32, vp, vp, vp, vp]
     lib.gnf4b_gather_rows_addr.restype = C.c_int
     lib.gnf4b_gather_rows_addr.argtypes = [vp, i64, i32, vp, vp, vp, i32, i64, vp]
+    lib.gnf4b_quantize_mxfp4.restype = C.c_int
+    lib.gnf4b_quantize_mxfp4.argtypes = [vp, C.c_int, i64, i64, i64, vp, vp, vp]
+    lib.gnf4b_dequantize_mxfp4.restype = C.c_int
+    lib.gnf4b_dequantize_mxfp4.argtypes = [vp, vp, i64, C.c_int, vp, vp]
+    lib.gnf4b_glu_quantize_mxfp4.restype = C.c_int
+    lib.gnf4b_glu_quantize_mxfp4.argtypes = [vp, i64, i64, C.c_int, vp, vp, i32, vp, vp, vp, vp]
+    lib.gnf4b_gemm_grouped_w4a4.restype = C.c_int
+    lib.gnf4b_gemm_grouped_w4a4.argtypes = [vp, vp, i64, vp, i64, i64, vp, i64, i64, vp, vp, i32, i32, i64, i64, i32, vp, vp, vp]
     lib.gnf4b_device_info.restype = C.c_int
     lib.gnf4b_device_info.argtypes = [vp, vp]
     return lib
@@ -172,6 +180,7 @@ EXPORTS = ("gnf4b_abi_version", "gnf4b_strerror", "gnf4b_last_cuda_error", "gnf4
            "gnf4b_ep_peer_layout", "gnf4b_ep_peer_dispatch", "gnf4b_ep_peer_combine",
            "gnf4b_gather_rows_by_id", "gnf4b_gather_rows_addr", "gnf4b_ep_plan_large", "gnf4b_ep_plan_large_scratch_bytes",
            "gnf4b_ep_push_blocks", "gnf4b_ep_wait_flags",
+           "gnf4b_quantize_mxfp4", "gnf4b_dequantize_mxfp4", "gnf4b_glu_quantize_mxfp4", "gnf4b_gemm_grouped_w4a4",
            "gnf4b_device_info")
 
 

@@ -11,6 +11,7 @@
 #include <mutex>
 #include <vector>
 
+#include "api_internal.h"
 #include "common.cuh"
 #include "stream_kernel.cuh"
 #include "decode_kernel.cuh"
@@ -30,18 +31,12 @@ static __device__ __align__(256) unsigned char g_noalloc_scratch[GNF4B_NOALLOC_S
 
 static thread_local char g_cuda_err[256] = "";
 
-static int cuda_fail(cudaError_t e, const char* what) {
+int cuda_fail(cudaError_t e, const char* what) {
     snprintf(g_cuda_err, sizeof g_cuda_err, "%s: %s", what, cudaGetErrorString(e));
     return GNF4B_ECUDA;
 }
 
-struct DevInfo {
-    int sm_count = 0;
-    int smem_optin = 0;
-    bool ok = false;
-};
-
-static int device_info(DevInfo* out) {
+int device_info(DevInfo* out) {
     static std::mutex mu;
     static DevInfo cache[64];
     int dev = 0;
@@ -78,9 +73,6 @@ static int noalloc_scratch(void** out) {
     *out = cache[dev];
     return GNF4B_OK;
 }
-
-static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-static inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 
 // ------------------------------------------------------------------ planning
 struct Plan {
@@ -193,22 +185,6 @@ static int make_plan(int fmt, int op, int x_dtype, int64_t T, int32_t G, int64_t
     return GNF4B_OK;
 }
 
-// cudaFuncSetAttribute is per device and not free; raise a kernel's dynamic shared-memory
-// limit only when a launch needs more than was already granted on this device.
-template <typename F>
-static cudaError_t ensure_smem(F kfn, size_t smem, int* granted /*[64], zero-initialised*/) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    dev &= 63;
-    if ((int)smem > granted[dev]) {
-        e = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
-        granted[dev] = (int)smem;
-    }
-    return cudaSuccess;
-}
-
 // ------------------------------------------------------------------ launches
 template <int FMT, int SDT>
 static cudaError_t launch_stream_au(const StreamArgs& sa, int au, int grid, size_t smem, cudaStream_t st) {
@@ -225,23 +201,6 @@ static cudaError_t launch_stream_au(const StreamArgs& sa, int au, int grid, size
     if (au == 3) GNF4B_LAUNCH_AU(3);
     GNF4B_LAUNCH_AU(0);
 #undef GNF4B_LAUNCH_AU
-}
-
-// Launch with programmatic stream serialization: the kernel may start while its predecessor in the stream is
-// still running and must call pdl_wait() before it touches anything (reads or writes) the predecessor may use.
-template <typename... KArgs, typename... Args>
-static cudaError_t launch_pdl(void (*kfn)(KArgs...), unsigned grid, unsigned block, cudaStream_t st, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(block);
-    cfg.dynamicSmemBytes = 0;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kfn, static_cast<KArgs>(args)...);
 }
 
 template <int FMT, int SDT, int AUV, int RMV, int RW, int XF, int XA = 0, int CH = 0>

@@ -1,0 +1,483 @@
+// Grouped product of two MXFP4 operands on the block-scaled tensor cores.
+//
+//   out^T[n, t] = sum_b 2^(ws[n,b] + xs[t,b] - 254) sum_{i<32} w[n, 32b+i] * x[t, 32b+i]
+//
+// (accumulator lane = weight row n, column = token t.)  Nothing is decoded: the packed e2m1 bytes of both operands go
+// from global memory into shared memory by TMA and from there into tcgen05.mma.kind::mxf4.block_scale, which multiplies
+// 64 contraction elements per instruction, applies both e8m0 exponents per 32 elements and accumulates in fp32.  A
+// zero element times any finite scale is zero, so ragged ends need no mask: TMA fills what lies outside the tensors
+// with zero bytes.  An exponent byte of 255 is NaN, as the OCP format has it.
+//
+// Roles (448 threads, one CTA per SM, persistent):
+//   warp 0      TMA producer: per stage of 256 contraction elements (128 bytes a row, 128-byte swizzle) the weight tile
+//               [rows_w x 128 B] and the item's activation rows in boxes of xbox rows
+//   warp 1      MMA issuer (one lane): tcgen05.cp of the stage's scales shared memory -> tensor memory (32 lanes
+//               x 16 bytes, replicated to the four lane quarters), then up to four MMAs of 64 elements
+//   warps 2-5   scales: one thread per weight row and per activation row (two of these from 129 tokens on) takes 32
+//               exponent bytes (1024 elements, four stages) at a time from global memory, a span ahead, and writes the
+//               4-byte words of a stage into the layout tcgen05.cp reads: row r at (r % 32) * 16 + (r / 32) * 4.
+//               Scale rows have any pitch (gpt-oss: 90 bytes), so they cannot come by TMA
+//   warps 6-13  epilogue, two per TMEM lane quarter taking alternate 32-token chunks, as in tensor_fwd_kernel.cuh
+//
+// Work item = (group, balanced chunk of <= tok_cap rows, rows_w weight rows), weight tile fastest.  With few rows per
+// group the kernel streams weights and rows_w < 128 evens out the items over the SMs (the MMA still multiplies 128
+// lanes; the lanes above rows_w hold stale bytes with zero scales and are not read back).
+#pragma once
+
+#include "tensor_kernel.cuh"
+
+namespace gnf4b {
+
+constexpr int kQStageK = 256;                  // contraction elements per stage
+constexpr int kQRowBytes = kQStageK / 2;       // 128 bytes: one swizzle row
+constexpr int kQWTile = 128 * kQRowBytes;      // 16 KiB, whatever rows_w: the MMA reads 128 rows
+constexpr int kQMaxStages = 12;
+constexpr int kQMaxGroups = 512;               // groups per launch (longer lists take several)
+constexpr int kQScaleWarps = 4, kQEpiWarps = 8;
+constexpr int kQScaleWarp0 = 2, kQEpiWarp0 = kQScaleWarp0 + kQScaleWarps;
+constexpr int kQThreads = (kQEpiWarp0 + kQEpiWarps) * 32;
+constexpr int kQTmemCols = 512;
+constexpr int kQTableBytes = kQMaxGroups * 16 + (kQMaxGroups + 1) * 8 + 16 * 8 + 8;
+
+struct W4A4Args {
+    const uint8_t* xs;          // activation scales, rows of K / 32 bytes
+    const uint8_t* ws;          // weight scales, byte strides ws_se, ws_sn
+    const int32_t* off;
+    const int32_t* eids;
+    int32_t* status;
+    uint16_t* out;
+    int64_t ws_se, ws_sn;
+    int64_t T, N, K;
+    int32_t G, E;
+    int32_t rows_w;             // weight rows per item, a multiple of 8, <= 128
+    int32_t n_tiles;            // ceil(N / rows_w)
+    int32_t k_stages;           // ceil(K / 256)
+    int32_t tok_cap;            // activation rows per item, a multiple of 16, <= 256
+    int32_t xbox;               // activation rows per TMA box
+    int32_t x_bytes;            // shared memory of a stage's activations, whole boxes
+    int32_t stages;
+    int32_t acc_bufs;           // 1 or 2 accumulators
+    int32_t x_blocks;           // ceil(tok_cap / 128): 512-byte scale blocks per 128 elements
+};
+
+// scales of a stage: two 128-element halves of [weights 512 B][activations x_blocks * 512 B]
+__host__ __device__ inline int w4a4_scale_bytes(int x_blocks) { return 2 * 512 * (1 + x_blocks); }
+__host__ __device__ inline int w4a4_stage_bytes(int x_bytes, int x_blocks) { return kQWTile + x_bytes + w4a4_scale_bytes(x_blocks); }
+__host__ __device__ inline size_t w4a4_fixed_bytes() { return 1024 /*alignment*/ + kQTableBytes + 512 /*barriers*/; }
+
+__device__ __forceinline__ void tma_load_3d(void* dst_smem, const CUtensorMap* map, int32_t c0, int32_t c1, int32_t c2,
+                                            uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(smem_u32(dst_smem)), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ void tc_mma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa,
+                                            uint32_t sfb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+// 32 rows x 16 bytes of shared memory -> 4 tensor-memory columns, the same 32 lanes in each of the four lane quarters
+__device__ __forceinline__ void tc_cp_scales(uint32_t taddr, uint64_t s_desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(s_desc) : "memory");
+}
+// descriptor of that source: no swizzle, 8-row groups of 128 bytes one after the other
+__device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
+    return (uint64_t)((smem_addr >> 4) & 0x3fffu) | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+}
+// kind::mxf4 instruction descriptor: e2m1 x e2m1, both K-major, e8m0 scales, M = 128; the byte pair of the 4-byte
+// scale words that belongs to this instruction's 64 elements is 0 or 2
+__device__ __forceinline__ uint32_t mxf4_idesc(uint32_t n_umma, uint32_t sf_id) {
+    return (sf_id << 4) | (1u << 7) | (1u << 10) | ((n_umma >> 3) << 17) | (1u << 23) | (8u << 24) | (sf_id << 29);
+}
+
+struct QGroup {
+    int32_t row0, rows, eid, chunk_rows;
+};
+struct QTable {
+    const QGroup* grp;       // [G]
+    const int64_t* base;     // [G + 1] items before group g
+};
+struct QItem {
+    int32_t row0, tokens, eid, n0;
+};
+
+__device__ __forceinline__ bool next_qitem(const W4A4Args& a, const QTable& tb, int32_t& g, int64_t id, QItem* it) {
+    while (g < a.G && id >= tb.base[g + 1]) ++g;
+    if (g >= a.G) return false;
+    const QGroup gr = tb.grp[g];
+    const int64_t local = id - tb.base[g];
+    const int32_t mc = (int32_t)(local / a.n_tiles);
+    it->row0 = gr.row0 + mc * gr.chunk_rows;
+    it->tokens = min(gr.chunk_rows, gr.row0 + gr.rows - it->row0);
+    it->eid = gr.eid;
+    it->n0 = (int32_t)(local - (int64_t)mc * a.n_tiles) * a.rows_w;
+    return true;
+}
+
+// Thread t takes groups 2t and 2t + 1: item counts, then a block-wide inclusive scan.  Groups with a bad expert id or
+// bad offsets are flagged in the status word and get no items.
+__device__ __forceinline__ void build_qtable(const W4A4Args& a, QGroup* grp, int64_t* base, int64_t* warp_tot) {
+    static_assert(kQThreads * 2 >= kQMaxGroups, "one thread per two groups");
+    const int t = threadIdx.x, lane = t & 31, w = t >> 5;
+    int64_t items[2] = {0, 0};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int g = 2 * t + h;
+        if (g >= a.G) continue;
+        QGroup gr;
+        gr.row0 = __ldg(a.off + g);
+        const int64_t rows = (int64_t)__ldg(a.off + g + 1) - gr.row0;
+        gr.eid = __ldg(a.eids + g);
+        const bool pad = gr.eid == GNF4B_PAD_EXPERT;     // padding group: skipped, not an error
+        const bool bad_e = (gr.eid < 0 || gr.eid >= a.E) && !pad;
+        const bool bad_o = rows < 0 || gr.row0 < 0 || gr.row0 + rows > a.T;
+        if ((bad_e || bad_o) && rows != 0 && a.status && blockIdx.x == 0)
+            atomicOr(a.status, bad_e ? GNF4B_ST_BAD_EXPERT : GNF4B_ST_BAD_OFFSETS);
+        gr.rows = (pad || bad_e || bad_o) ? 0 : (int32_t)rows;
+        const int32_t chunks = (int32_t)(((int64_t)gr.rows + a.tok_cap - 1) / a.tok_cap);
+        // equal chunks, a multiple of 16 rows each
+        gr.chunk_rows = chunks ? (((gr.rows + chunks - 1) / chunks + 15) & ~15) : 16;
+        grp[g] = gr;
+        items[h] = (int64_t)((gr.rows + gr.chunk_rows - 1) / gr.chunk_rows) * a.n_tiles;
+    }
+    int64_t incl = items[0] + items[1];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += up;
+    }
+    if (lane == 31) warp_tot[w] = incl;
+    __syncthreads();
+    for (int v = 0; v < w; ++v) incl += warp_tot[v];
+    if (2 * t < a.G) base[2 * t + 1] = incl - items[1];
+    if (2 * t + 1 < a.G) base[2 * t + 2] = incl;
+    if (t == 0) base[0] = 0;
+}
+
+// Up to 32 scale bytes from p (any alignment) into 8 words, zeros behind the first `valid`.  [lo, hi) is the scale
+// tensor: a 4-byte word that would reach outside it is put together from its bytes.
+__device__ __forceinline__ void load_scale_span(const uint8_t* p, int valid, const uint8_t* lo, const uint8_t* hi, uint32_t* out) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) out[j] = 0;
+    if (valid <= 0) return;
+    if (valid >= 32 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+        const uint4 v0 = __ldg(reinterpret_cast<const uint4*>(p)), v1 = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+        out[0] = v0.x; out[1] = v0.y; out[2] = v0.z; out[3] = v0.w;
+        out[4] = v1.x; out[5] = v1.y; out[6] = v1.z; out[7] = v1.w;
+        return;
+    }
+    valid = min(valid, 32);
+    const uint32_t skip = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 3);
+    const uint8_t* a = p - skip;
+    uint32_t w[9];
+#pragma unroll
+    for (int j = 0; j < 9; ++j) {
+        w[j] = 0;
+        const uint8_t* q = a + 4 * j;
+        if (4 * j < (int)skip + valid) {
+            if (q >= lo && q + 4 <= hi) {
+                w[j] = __ldg(reinterpret_cast<const uint32_t*>(q));
+            } else {
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+                    if (q + b >= lo && q + b < hi) w[j] |= (uint32_t)__ldg(q + b) << (8 * b);
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t v = __funnelshift_r(w[j], w[j + 1], 8 * skip);
+        const int left = valid - 4 * j;
+        out[j] = left >= 4 ? v : left <= 0 ? 0u : v & ((1u << (8 * left)) - 1u);
+    }
+}
+
+__global__ void __launch_bounds__(kQThreads, 1)
+w4a4_kernel(const W4A4Args a, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    // tiles of all stages (each a multiple of 1024 bytes), then the scales of all stages, then the tables
+    const int tile_bytes = kQWTile + a.x_bytes;
+    const int scale_bytes = w4a4_scale_bytes(a.x_blocks);
+    uint8_t* s_scale = smem + (size_t)a.stages * tile_bytes;
+    uint8_t* grp_raw = s_scale + (size_t)a.stages * scale_bytes;
+    QGroup* s_grp = reinterpret_cast<QGroup*>(grp_raw);
+    int64_t* s_base = reinterpret_cast<int64_t*>(grp_raw + kQMaxGroups * 16);
+    int64_t* s_wtot = s_base + kQMaxGroups + 1;
+    // full[s]: tiles landed (TMA bytes + the producer's arrival) and scales written (one arrival per scale warp);
+    // done[s]: the stage's copies and MMAs have completed, shared memory and tensor-memory scale slot may be refilled
+    uint64_t* full = reinterpret_cast<uint64_t*>(grp_raw + ((kQTableBytes + 15) & ~15));
+    uint64_t* done = full + kQMaxStages;
+    uint64_t* acc_full = done + kQMaxStages;
+    uint64_t* acc_empty = acc_full + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t stages = (uint32_t)a.stages;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kQMaxStages; ++s) {
+            mbar_init(full + s, 1 + kQScaleWarps);
+            mbar_init(done + s, 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(acc_full + b, 1);
+            mbar_init(acc_empty + b, kQEpiWarps);
+        }
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, kQTmemCols);
+        tmem_relinquish();
+    }
+    pdl_wait();                      // group tables, operands and the output belong to earlier kernels until here
+    pdl_launch_dependents();         // not before: a successor may read, ahead of its own wait, what OUR predecessor wrote
+    build_qtable(a, s_grp, s_base, s_wtot);
+    const QTable tb{s_grp, s_base};
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t tmem_sf0 = tmem_base + (uint32_t)(a.acc_bufs * a.tok_cap);      // scale slots behind the accumulators
+    const uint32_t slot_cols = 8u * (1u + (uint32_t)a.x_blocks);
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ TMA producer
+        if (lane == 0) {
+            int32_t g = 0;
+            QItem it;
+            uint32_t s = 0, phase = 0;
+            bool ok = true;
+            for (int64_t id = blockIdx.x; ok && next_qitem(a, tb, g, id, &it); id += gridDim.x) {
+                const int boxes = (it.tokens + a.xbox - 1) / a.xbox;
+                const uint32_t bytes = (uint32_t)((a.rows_w + boxes * a.xbox) * kQRowBytes);
+                for (int rb = 0; rb < a.k_stages; ++rb) {
+                    ok = mbar_wait_bounded(done + s, phase ^ 1, abort_flag);       // the first round passes at once
+                    if (!ok) break;
+                    uint8_t* st = smem + (size_t)s * tile_bytes;
+                    mbar_arrive_expect_tx(full + s, bytes);
+                    tma_load_3d(st, &w_map, rb * kQRowBytes, it.n0, it.eid, full + s);
+                    for (int b = 0; b < boxes; ++b)
+                        tma_load_2d(st + kQWTile + b * a.xbox * kQRowBytes, &x_map, rb * kQRowBytes, it.row0 + b * a.xbox, full + s);
+                    if (++s == stages) { s = 0; phase ^= 1; }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA issuer
+        if (lane == 0) {
+            int32_t g = 0;
+            QItem it;
+            uint32_t s = 0, phase = 0, buf = 0, acc_phase = 0;
+            bool ok = true;
+            for (int64_t id = blockIdx.x; ok && next_qitem(a, tb, g, id, &it); id += gridDim.x) {
+                const uint32_t n_umma = (uint32_t)((it.tokens + 15) & ~15);
+                const uint32_t id0 = mxf4_idesc(n_umma, 0), id2 = mxf4_idesc(n_umma, 2);
+                const int xb = (it.tokens + 127) >> 7;
+                const uint32_t acc = tmem_base + buf * (uint32_t)a.tok_cap;
+                ok = mbar_wait_bounded(acc_empty + buf, acc_phase ^ 1, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                for (int rb = 0; rb < a.k_stages; ++rb) {
+                    ok = mbar_wait_bounded(full + s, phase, abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t wt = smem_u32(smem + (size_t)s * tile_bytes), xt = wt + kQWTile;
+                    const uint32_t sc = smem_u32(s_scale + (size_t)s * scale_bytes);
+                    const uint32_t sf = tmem_sf0 + s * slot_cols;
+                    // steps of 64 elements that exist (a trailing half step is zero elements)
+                    const int steps = (int)min((int64_t)4, (a.K - (int64_t)rb * kQStageK + 63) >> 6);
+                    for (int h = 0; 2 * h < steps; ++h) {
+                        const uint32_t src = sc + (uint32_t)(h * 512 * (1 + a.x_blocks));
+                        const uint32_t sfa = sf + (uint32_t)(h * 4 * (1 + a.x_blocks)), sfb = sfa + 4;
+                        tc_cp_scales(sfa, scale_desc(src));
+                        for (int b = 0; b < xb; ++b) tc_cp_scales(sfb + b * 4, scale_desc(src + 512 * (1 + b)));
+                        for (int j = 2 * h; j < steps && j < 2 * h + 2; ++j)
+                            tc_mma_mxf4(acc, umma_desc(wt + j * 32, 16, 1024), umma_desc(xt + j * 32, 16, 1024),
+                                        (j & 1) ? id2 : id0, sfa, sfb, (rb > 0 || j > 0) ? 1u : 0u);
+                    }
+                    tc_commit(done + s);
+                    if (++s == stages) { s = 0; phase ^= 1; }
+                }
+                if (ok) tc_commit(acc_full + buf);
+                if (++buf == (uint32_t)a.acc_bufs) { buf = 0; acc_phase ^= 1; }
+            }
+        }
+    } else if (warp < kQEpiWarp0) {
+        // ------------------------------------------------------------ scales: global -> registers -> shared memory
+        const int t = threadIdx.x - kQScaleWarp0 * 32;
+        const int64_t kb = a.K / 32;
+        const uint8_t* w_lo = a.ws;
+        const uint8_t* w_hi = a.ws + (int64_t)(a.E - 1) * a.ws_se + (a.N - 1) * a.ws_sn + kb;
+        const uint8_t* x_lo = a.xs;
+        const uint8_t* x_hi = a.xs + a.T * kb;
+        const int spans = (a.k_stages + 3) >> 2;
+        const uint32_t at = (uint32_t)((t & 31) * 16 + (t >> 5) * 4);
+        int32_t g = 0;
+        QItem it;
+        int64_t id = blockIdx.x;
+        bool have = next_qitem(a, tb, g, id, &it);
+        int sp = 0;
+        uint32_t nxt[3][8];
+        auto fetch = [&]() {                       // span sp of item `it`
+            const int valid = (int)min((int64_t)32, kb - (int64_t)sp * 32);
+            const int64_t n = (int64_t)it.n0 + t;
+            load_scale_span(a.ws + (int64_t)it.eid * a.ws_se + n * a.ws_sn + sp * 32, (t < a.rows_w && n < a.N) ? valid : 0,
+                            w_lo, w_hi, nxt[0]);
+            load_scale_span(a.xs + ((int64_t)it.row0 + t) * kb + sp * 32, t < it.tokens ? valid : 0, x_lo, x_hi, nxt[1]);
+            load_scale_span(a.xs + ((int64_t)it.row0 + t + 128) * kb + sp * 32, t + 128 < it.tokens ? valid : 0, x_lo, x_hi, nxt[2]);
+        };
+        if (have) fetch();
+        uint32_t s = 0, phase = 0;
+        bool ok = true;
+        while (have && ok) {
+            uint32_t cur[3][8];
+#pragma unroll
+            for (int r = 0; r < 3; ++r)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) cur[r][j] = nxt[r][j];
+            const int n_st = min(4, a.k_stages - sp * 4);
+            if (++sp == spans) {
+                sp = 0;
+                id += gridDim.x;
+                have = next_qitem(a, tb, g, id, &it);
+            }
+            if (have) fetch();
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (q >= n_st || !ok) continue;
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(done + s, phase ^ 1, abort_flag));
+                if (!ok) continue;
+                uint8_t* dst = s_scale + (size_t)s * scale_bytes + at;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint8_t* d = dst + h * 512 * (1 + a.x_blocks);
+                    *reinterpret_cast<uint32_t*>(d) = cur[0][2 * q + h];
+                    *reinterpret_cast<uint32_t*>(d + 512) = cur[1][2 * q + h];
+                    if (a.x_blocks == 2) *reinterpret_cast<uint32_t*>(d + 1024) = cur[2][2 * q + h];
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full + s);
+                if (++s == stages) { s = 0; phase ^= 1; }
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ epilogue
+        const int q = warp & 3;
+        const int e = (warp - kQEpiWarp0) >> 2;              // takes chunks e, e + 2, ...
+        int32_t g = 0;
+        QItem it;
+        uint32_t buf = 0, acc_phase = 0;
+        bool ok = true;
+        const bool pair_ok = (a.N % 2) == 0;
+        for (int64_t id = blockIdx.x; ok && next_qitem(a, tb, g, id, &it); id += gridDim.x) {
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(acc_full + buf, acc_phase, abort_flag));
+            if (!ok) break;
+            tc_fence_after();
+            const int r_local = q * 32 + lane;
+            const int64_t n = (int64_t)it.n0 + r_local;             // this lane's output column
+            const bool mine = r_local < a.rows_w && n < a.N;
+            const int chunks = q * 32 < a.rows_w ? (it.tokens + 31) >> 5 : 0;
+            auto release_acc = [&]() {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acc_empty + buf);
+            };
+            if (e >= chunks) release_acc();              // nothing to drain for this warp
+            for (int c = e; c < chunks; c += 2) {
+                uint32_t r[32];
+                tmem_ld32(tmem_base + buf * (uint32_t)a.tok_cap + ((uint32_t)(q * 32) << 16) + (uint32_t)(c * 32), r);
+                tmem_ld_wait();
+                if (c + 2 >= chunks) release_acc();      // all this warp needs is in registers
+                const int t0 = c * 32;
+                if (pair_ok) {
+                    // lanes 2i and 2i+1 swap one value: the even lane stores (n, n+1) of token j,
+                    // the odd lane (n-1, n) of token j+1 -- 4-byte stores, 64 bytes per half warp
+                    const int odd = lane & 1;
+                    const int left = mine ? it.tokens - t0 - odd : 0;     // store while j < left
+                    uint16_t* p = a.out + (int64_t)(it.row0 + t0 + odd) * a.N + (n - odd);
+                    const int64_t step = 2 * a.N;
+                    uint32_t v[16];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        const float m0 = __uint_as_float(r[j]), m1 = __uint_as_float(r[j + 1]);
+                        const float got = __shfl_xor_sync(0xffffffffu, odd ? m0 : m1, 1);
+                        v[j >> 1] = odd ? pack_bf16x2(m1, got) : pack_bf16x2(got, m0);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        if (j < left) *reinterpret_cast<uint32_t*>(p) = v[j >> 1];
+                        p += step;
+                    }
+                } else {
+                    const int left = mine ? it.tokens - t0 : 0;
+                    uint16_t* p = a.out + (int64_t)(it.row0 + t0) * a.N + n;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        if (j < left) *p = f32_to_bf16_bits(__uint_as_float(r[j]));
+                        p += a.N;
+                    }
+                }
+            }
+            if (++buf == (uint32_t)a.acc_bufs) { buf = 0; acc_phase ^= 1; }
+        }
+    }
+
+    // ---------------------------------------------------------------- teardown
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag) {               // a wait gave up: give the copies in flight time to land before the memory goes
+        const long long t0 = clock64();
+        while (clock64() - t0 < 20000000ll) {
+        }
+        __syncthreads();
+    }
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem_base, kQTmemCols);
+    }
+    if (threadIdx.x == 0 && *abort_flag && a.status) atomicOr(a.status, GNF4B_ST_TIMEOUT);
+}
+
+struct W4A4Plan {
+    int rows_w, tok_cap, xbox, x_bytes, x_blocks, stages, acc_bufs;
+    size_t smem;
+};
+
+// Tile shape from the row counts alone.  max_rows <= 0: unknown, any group may be long.
+static inline W4A4Plan w4a4_plan(int64_t T, int32_t G, int64_t N, int32_t max_rows, int sm_count, int smem_optin) {
+    W4A4Plan p;
+    const int64_t longest = max_rows > 0 ? (max_rows < T ? max_rows : T) : T;
+    p.tok_cap = (int)round_up(longest < 256 ? longest : 256, 16);
+    p.xbox = p.tok_cap <= 16 ? 16 : p.tok_cap <= 64 ? 32 : 64;
+    p.x_bytes = (int)round_up(p.tok_cap, p.xbox) * kQRowBytes;
+    p.x_blocks = (p.tok_cap + 127) / 128;
+    p.rows_w = 128;
+    if (longest <= 64) {
+        // streaming weights: the tile height that shares the rows out most evenly (each item costs its rows and,
+        // for the pipeline's start and the epilogue, about as much as 8 more)
+        double best = 1e30;
+        for (int r = 128; r >= 32; r -= 8) {
+            const int64_t rounds = ceil_div((int64_t)G * ceil_div(N, r), sm_count);
+            const double cost = (double)rounds * (r + 8);
+            if (cost < best) { best = cost; p.rows_w = r; }
+        }
+    }
+    const size_t room = (size_t)smem_optin - w4a4_fixed_bytes();
+    p.stages = (int)(room / (size_t)w4a4_stage_bytes(p.x_bytes, p.x_blocks));
+    if (p.stages > kQMaxStages) p.stages = kQMaxStages;
+    p.acc_bufs = 2 * p.tok_cap + p.stages * 8 * (1 + p.x_blocks) <= kQTmemCols ? 2 : 1;
+    p.smem = w4a4_fixed_bytes() + (size_t)p.stages * w4a4_stage_bytes(p.x_bytes, p.x_blocks);
+    return p;
+}
+
+}  // namespace gnf4b

@@ -15,8 +15,8 @@ from __future__ import annotations
 import torch
 
 import _gnf4b
-from nf4_grouped import (_dispatch, _launch, _launch_ffn, _launch_host, _prefill_block_m, _require_cuda,  # noqa: F401  (re-exported names)
-                         build_group_tiles)
+from nf4_grouped import (_dispatch, _group_tables, _launch, _launch_ffn, _launch_host, _prefill_block_m,  # noqa: F401  (re-exported names)
+                         _raw_stream, _require_cuda, _status_ptr, build_group_tiles)
 
 # e2m1 codebook, index = (sign << 3) | magnitude (ref :34-35)
 FP4_VALUES = [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0,
@@ -142,3 +142,169 @@ def dequant_stack_cuda(blocks, scales):
                                torch.cuda.current_stream(blocks.device).cuda_stream)
     _gnf4b.check(rc, "gnf4b_dequant")
     return out
+
+
+# --------------------------------------------------------------------------- #
+# both operands in MXFP4: quantiser, product, expert FFN
+# --------------------------------------------------------------------------- #
+_X_DTYPES = {torch.bfloat16: _gnf4b.X_BF16, torch.float16: _gnf4b.X_FP16, torch.float32: _gnf4b.X_FP32}
+
+
+def quantize_mxfp4(x):
+    """Rows to MXFP4 on the GPU: ``x [..., K]`` bf16 / fp16 / fp32 (K a multiple of 32) -> ``(blocks [..., K//2],
+    scales [..., K//32])`` uint8, element 2j in the low nibble.  Per 32 elements the exponent is the least integer
+    e >= -69 with max|x| <= 6 * 2^e and every element takes the nearest e2m1 value, the lower magnitude on a tie: byte
+    for byte what ``mxfp4_pack_ref.quantize_pack_mxfp4`` gives (as ``[..., K//32, 16]``).  A block that holds an
+    infinity or a NaN gets the exponent byte 255.  Rows may be a strided view; other layouts are copied first."""
+    _require_cuda(x, "quantize_mxfp4", "The CPU counterpart is mxfp4_pack_ref.quantize_pack_mxfp4.")
+    if x.dtype not in _X_DTYPES:
+        raise TypeError(f"quantize_mxfp4 takes bfloat16, float16 or float32, got {x.dtype}")
+    if x.dim() == 0 or x.shape[-1] == 0 or x.shape[-1] % MX_BLOCK:
+        raise ValueError(f"the last dimension must be a positive multiple of {MX_BLOCK}, got shape {tuple(x.shape)}")
+    K = x.shape[-1]
+    lead = tuple(x.shape[:-1])
+    x = x.detach()
+    if x.dim() != 2 or x.stride(1) != 1:
+        x = x.reshape(x.numel() // K, K)
+        if x.stride(1) != 1:
+            x = x.contiguous()
+    blocks = torch.empty(*lead, K // 2, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(*lead, K // MX_BLOCK, dtype=torch.uint8, device=x.device)
+    with torch.cuda.device(x.device):
+        rc = _gnf4b.load().gnf4b_quantize_mxfp4(x.data_ptr(), _X_DTYPES[x.dtype], x.shape[0], K, x.stride(0) if x.shape[0] > 1 else K,
+                                                blocks.data_ptr(), scales.data_ptr(), _raw_stream(x.device))
+    _gnf4b.check(rc, "gnf4b_quantize_mxfp4")
+    return blocks, scales
+
+
+def _check_packed(blocks, scales, what: str):
+    if blocks.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise TypeError(f"{what}: blocks and scales must be uint8, got {blocks.dtype} and {scales.dtype}")
+    if blocks.dim() == 0 or blocks.dim() != scales.dim() or blocks.shape[:-1] != scales.shape[:-1] \
+            or blocks.shape[-1] != 16 * scales.shape[-1] or scales.shape[-1] == 0:
+        raise ValueError(f"{what}: blocks {tuple(blocks.shape)} and scales {tuple(scales.shape)} are not [..., K//2] and [..., K//32]")
+    if scales.device != blocks.device:
+        raise ValueError(f"{what}: blocks and scales must live on the same device")
+
+
+def _packed_rows(t, align: int):
+    """``t`` contiguous and its data aligned."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % align else t
+
+
+def dequantize_mxfp4(blocks, scales, dtype=torch.bfloat16):
+    """The values of packed rows, ``blocks [..., K//2]`` and ``scales [..., K//32]`` -> ``[..., K]`` in bf16 or fp32
+    (exact) or fp16 (rounded once).  An exponent byte of 255 reads as 2^128, as in ``mxfp4_pack_ref.dequant_mxfp4``."""
+    _require_cuda(blocks, "dequantize_mxfp4", "The CPU counterpart is mxfp4_pack_ref.dequant_mxfp4.")
+    if dtype not in _X_DTYPES:
+        raise TypeError(f"dequantize_mxfp4 returns bfloat16, float16 or float32, not {dtype}")
+    _check_packed(blocks, scales, "dequantize_mxfp4")
+    blocks, scales = _packed_rows(blocks, 4), scales.contiguous()
+    out = torch.empty(*blocks.shape[:-1], 2 * blocks.shape[-1], dtype=dtype, device=blocks.device)
+    with torch.cuda.device(blocks.device):
+        rc = _gnf4b.load().gnf4b_dequantize_mxfp4(blocks.data_ptr(), scales.data_ptr(), scales.numel(), _X_DTYPES[dtype],
+                                                  out.data_ptr(), _raw_stream(blocks.device))
+    _gnf4b.check(rc, "gnf4b_dequantize_mxfp4")
+    return out
+
+
+def glu_quantize_mxfp4(gate_up, act: str = "silu", bias=None, row_expert=None):
+    """The activation between an expert's two products with its result packed in the same pass: ``gate_up [rows, 2h]``
+    bf16 (h a multiple of 32) -> ``(blocks [rows, h//2], scales [rows, h//32])``, the bytes of ``ep_moe.silu_glu``
+    (``act="silu"``) or ``glu_gpt_oss`` (``act="gpt_oss"``; optional ``bias`` bf16 ``[E, 2h]`` by ``row_expert``) followed
+    by ``quantize_mxfp4``."""
+    if act not in ("gpt_oss", "silu"):
+        raise ValueError("act is 'gpt_oss' or 'silu'")
+    _require_cuda(gate_up, "glu_quantize_mxfp4", "")
+    if gate_up.dtype != torch.bfloat16:
+        raise TypeError(f"gate_up must be bfloat16, got {gate_up.dtype}")
+    if gate_up.dim() != 2 or gate_up.shape[1] == 0 or gate_up.shape[1] % (2 * MX_BLOCK):
+        raise ValueError(f"gate_up must be [rows, 2h] with h a multiple of {MX_BLOCK}, got {tuple(gate_up.shape)}")
+    rows, h = gate_up.shape[0], gate_up.shape[1] // 2
+    dev = gate_up.device
+    gate_up = gate_up.detach().contiguous()
+    E = 0
+    if bias is not None:
+        if act != "gpt_oss" or row_expert is None:
+            raise ValueError("bias goes with act='gpt_oss' and row_expert")
+        if bias.dtype != torch.bfloat16 or bias.dim() != 2 or bias.shape[1] != 2 * h or bias.shape[0] == 0 or bias.device != dev:
+            raise ValueError(f"bias must be a bfloat16 tensor [E, {2 * h}] on {dev}")
+        if tuple(row_expert.shape) != (rows,) or row_expert.device != dev or row_expert.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"row_expert must be an integer tensor of {rows} expert ids on {dev}")
+        E = bias.shape[0]
+        bias, row_expert = bias.detach().contiguous(), row_expert.to(torch.int32).contiguous()
+    blocks = torch.empty(rows, h // 2, dtype=torch.uint8, device=dev)
+    scales = torch.empty(rows, h // MX_BLOCK, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        rc = _gnf4b.load().gnf4b_glu_quantize_mxfp4(
+            gate_up.data_ptr(), rows, h, _gnf4b.ACT_SILU_GLU if act == "silu" else _gnf4b.ACT_GPT_OSS_GLU,
+            bias.data_ptr() if bias is not None else None, row_expert.data_ptr() if bias is not None else None, E,
+            blocks.data_ptr(), scales.data_ptr(), _status_ptr(dev), _raw_stream(dev))
+    _gnf4b.check(rc, "gnf4b_glu_quantize_mxfp4")
+    return blocks, scales
+
+
+def _tma_ready(blocks):
+    """A weight stack as the product's TMA loads take it: 16-byte aligned, positive strides in multiples of 16 bytes."""
+    ok = blocks.stride(2) == 1 and blocks.data_ptr() % 16 == 0
+    for dim in (0, 1):
+        ok = ok and (blocks.shape[dim] == 1 or (blocks.stride(dim) > 0 and blocks.stride(dim) % 16 == 0))
+    return blocks if ok else _packed_rows(blocks, 16)
+
+
+def gemm_mxfp4_grouped_w4a4(a_blocks, a_scales, blocks, scales, sizes, expert_ids, *, group_offsets=None, max_rows=None):
+    """Grouped product of MXFP4 rows with MXFP4 expert stacks: ``out[t] = dequant(a)[t] @ dequant(W[e(t)]).T``, both
+    operands multiplied as they are packed, on the block-scaled tensor cores (fp32 accumulation, one rounding to bf16).
+
+    ``a_blocks [T, K//2]`` / ``a_scales [T, K//32]`` uint8 rows sorted by group (``quantize_mxfp4`` makes them);
+    ``blocks [E, N, K//2]`` / ``scales [E, N, K//32]`` and ``sizes``, ``expert_ids``, ``group_offsets``, ``max_rows`` as in
+    ``gemm_mxfp4_grouped`` (``max_rows`` only shapes the tiles).  An exponent byte of 255 is NaN here, as in the OCP
+    format.  Returns ``[T, N]`` bf16.  A stack whose strides are not positive multiples of 16 bytes is copied first."""
+    _require_cuda(a_blocks, "gemm_mxfp4_grouped_w4a4",
+                  "The CPU-checkable equivalent multiplies mxfp4_pack_ref.dequant_mxfp4 of both operands per group.")
+    if a_blocks.dim() != 2 or blocks.dim() != 3:
+        raise ValueError(f"a_blocks must be [T, K//2] and blocks [E, N, K//2], got {tuple(a_blocks.shape)} and {tuple(blocks.shape)}")
+    _check_packed(a_blocks, a_scales, "gemm_mxfp4_grouped_w4a4 (rows)")
+    _check_packed(blocks, scales, "gemm_mxfp4_grouped_w4a4 (stack)")
+    dev = a_blocks.device
+    if blocks.device != dev:
+        raise ValueError("rows and stack must live on the same device")
+    T, half = a_blocks.shape
+    E, N = blocks.shape[:2]
+    if blocks.shape[2] != half:
+        raise ValueError(f"the rows have K={2 * half} but the stack packs K={2 * blocks.shape[2]}")
+    out = torch.empty(T, N, dtype=torch.bfloat16, device=dev)
+    if T == 0 or N == 0 or E == 0:
+        return out
+    a_blocks, a_scales, blocks = _packed_rows(a_blocks, 16), a_scales.contiguous(), _tma_ready(blocks)
+    if scales.stride(2) != 1:
+        scales = scales.contiguous()
+    with torch.cuda.device(dev):
+        stream_ptr = _raw_stream(dev)
+        off_t, ids_t, G, max_rows = _group_tables(sizes, expert_ids, T, E, dev, group_offsets, max_rows, stream_ptr)
+        if G == 0:
+            return out
+        rc = _gnf4b.load().gnf4b_gemm_grouped_w4a4(
+            a_blocks.data_ptr(), a_scales.data_ptr(), T, blocks.data_ptr(), blocks.stride(0), blocks.stride(1),
+            scales.data_ptr(), scales.stride(0), scales.stride(1), off_t if isinstance(off_t, int) else off_t.data_ptr(),
+            ids_t if isinstance(ids_t, int) else ids_t.data_ptr(), G, E, N, 2 * half, max_rows, out.data_ptr(),
+            _status_ptr(dev), stream_ptr)
+    _gnf4b.check(rc, "gnf4b_gemm_grouped_w4a4")
+    return out
+
+
+def ffn_mxfp4_grouped_w4a4(a_cat, blocks_gu, scales_gu, blocks_dn, scales_dn, sizes, expert_ids, *, act: str = "gpt_oss",
+                           bias_gu=None, row_expert=None, group_offsets=None, max_rows=None):
+    """One MXFP4 expert FFN per row with the rows in MXFP4 too: quantise ``a_cat [T, K]``, gate_up product, activation
+    packed as it is computed, down product -> ``[T, N_dn]`` bf16.  Arguments as in ``ffn_mxfp4_grouped``; ``a_cat`` may
+    also be the packed pair ``(blocks, scales)`` (quantise a token once, gather its bytes to its experts).  ``bias_gu``
+    (bf16 ``[E, N_gu]``, ``act="gpt_oss"``) is added per row by ``row_expert [T]``."""
+    if act not in ("gpt_oss", "silu"):
+        raise ValueError("act is 'gpt_oss' or 'silu'")
+    a_b, a_s = a_cat if isinstance(a_cat, (tuple, list)) else quantize_mxfp4(a_cat)
+    if blocks_gu.shape[1] % 2 or blocks_dn.shape[0] != blocks_gu.shape[0] or blocks_dn.shape[2] * 4 != blocks_gu.shape[1]:
+        raise ValueError(f"down stack {tuple(blocks_dn.shape)} does not follow gate_up {tuple(blocks_gu.shape)}")
+    gu = gemm_mxfp4_grouped_w4a4(a_b, a_s, blocks_gu, scales_gu, sizes, expert_ids, group_offsets=group_offsets, max_rows=max_rows)
+    h_b, h_s = glu_quantize_mxfp4(gu, act, bias_gu, row_expert)
+    return gemm_mxfp4_grouped_w4a4(h_b, h_s, blocks_dn, scales_dn, sizes, expert_ids, group_offsets=group_offsets, max_rows=max_rows)

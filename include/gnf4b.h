@@ -32,6 +32,7 @@ extern "C" {
 /* activation dtypes */
 #define GNF4B_X_BF16    0
 #define GNF4B_X_FP16    1
+#define GNF4B_X_FP32    2   /* quantiser input, dequantiser output, router logits */
 /* scale dtypes */
 #define GNF4B_S_F32     0   /* NF4 absmax, fp32                                  */
 #define GNF4B_S_BF16    1   /* NF4 absmax stored as bf16 (widened exactly)       */
@@ -434,6 +435,38 @@ int gnf4b_gather_rows_by_id(void* dst, int64_t row_bytes, int32_t n_slots, const
 int gnf4b_gather_rows_addr(void* dst, int64_t row_bytes, int32_t n_slots, const int64_t* want_addr,
                            const int64_t* have_addr, const int64_t* pieces, int32_t n_pieces, int64_t max_piece_bytes,
                            void* cuda_stream);
+
+/* MXFP4 on the way in: x [rows, K] (bf16, fp16 or fp32; rows x_stride ELEMENTS apart, K % 32 == 0) -> blocks [rows, K/2]
+ * (element 2j in the low nibble; 4-byte aligned) and scales [rows, K/32].  Per 32 elements e = the least integer >= -69
+ * with max|x| <= 6 * 2^e, scale byte e + 127; code = the e2m1 value nearest to x / 2^e, the lower magnitude on a tie,
+ * +0 for what rounds to zero: byte for byte the rule of quantize_pack_mxfp4 (kernel/mxfp4_pack_ref.py:73-103).  A block
+ * with an infinity or a NaN gets scale byte 255 and codes of +-6.
+ * gnf4b_dequantize_mxfp4: n_blocks blocks of 32 -> out (32 n_blocks elements, 16-byte aligned); exact in bf16 and fp32.
+ * gnf4b_glu_quantize_mxfp4: gate_up bf16 [rows, 2h] (h % 32 == 0) -> the GLU's bf16 result, quantised as above, without
+ * writing it: the bytes of gnf4b_silu_glu / gnf4b_glu_gpt_oss followed by gnf4b_quantize_mxfp4.  bias (bf16 [E, 2h]) and
+ * row_expert only with GNF4B_ACT_GPT_OSS_GLU; a row whose expert is outside [0, E) gets no bias and raises
+ * GNF4B_ST_BAD_EXPERT. */
+int gnf4b_quantize_mxfp4(const void* x, int x_dtype, int64_t rows, int64_t K, int64_t x_stride, uint8_t* blocks,
+                         uint8_t* scales, void* cuda_stream);
+int gnf4b_dequantize_mxfp4(const uint8_t* blocks, const uint8_t* scales, int64_t n_blocks, int out_dtype, void* out,
+                           void* cuda_stream);
+int gnf4b_glu_quantize_mxfp4(const void* gate_up, int64_t rows, int64_t h, int act, const void* bias,
+                             const int32_t* row_expert, int32_t E, uint8_t* blocks, uint8_t* scales,
+                             int32_t* status_word, void* cuda_stream);
+
+/* The grouped product with BOTH operands in MXFP4 (no counterpart in the reference, whose products take 16-bit rows):
+ *   out[t, n] = sum over K of x[t, k] * W[e(t), n, k], exact products, fp32 accumulation, one rounding to bf16,
+ * on the block-scaled tensor cores, nothing decoded.  x_blocks [T, K/2] and x_scales [T, K/32] contiguous, rows sorted
+ * by group; W / S, group_offsets, expert_ids, max_rows, status_word as in gnf4b_gemm_grouped with GNF4B_FMT_MXFP4
+ * (max_rows only shapes the tiles here: understating it costs speed, not rows).  x_blocks and W start on 16 bytes and
+ * W's strides are positive multiples of 16 bytes (GNF4B_EUNSUPPORTED otherwise); the scales may have any alignment and
+ * any non-negative strides.  A scale byte of 255 is NaN here, as the OCP format defines it.  Rows that belong to no
+ * group, or to a padding group, are left as they were. */
+int gnf4b_gemm_grouped_w4a4(const uint8_t* x_blocks, const uint8_t* x_scales, int64_t T,
+                            const uint8_t* W, int64_t w_stride_e, int64_t w_stride_n,
+                            const uint8_t* S, int64_t s_stride_e, int64_t s_stride_n,
+                            const int32_t* group_offsets, const int32_t* expert_ids, int32_t G, int32_t E,
+                            int64_t N, int64_t K, int32_t max_rows, void* out, int32_t* status_word, void* cuda_stream);
 
 /* Device properties this library plans with (SM count, opt-in shared memory). */
 int gnf4b_device_info(int32_t* sm_count, int32_t* smem_optin_bytes);
