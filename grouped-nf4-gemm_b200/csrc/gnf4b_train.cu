@@ -1,0 +1,163 @@
+// C entry points of the training operators: routing with its losses, the GLU with an 8-bit checkpoint (include/gnf4b.h).
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "api_internal.h"
+#include "common.cuh"
+#include "glu_ckpt8.cuh"
+#include "router_train.cuh"
+
+using namespace gnf4b;
+
+namespace {
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+constexpr int kRtWarps = 8;
+
+// CTAs of the forward pass: one while a warp then has few tokens, else all SMs' worth
+int rt_grid(int64_t T, int sm_count) {
+    if (T <= kRtWarps * 16) return 1;
+    return (int)std::min<int64_t>(ceil_div(T, kRtWarps * 2), (int64_t)sm_count * 2);
+}
+
+int rt_check(int dtype, int64_t T, int64_t stride, int32_t E, int32_t k, int32_t mode, int32_t norm) {
+    if (dtype < GNF4B_X_BF16 || dtype > GNF4B_X_FP32 || T < 0 || mode < 0 || mode > 1 || norm < 0 || norm > 1) return GNF4B_EINVAL;
+    if (E <= 0 || k <= 0 || k > E || stride < 0) return GNF4B_ESHAPE;
+    if (E > kRtMaxExperts || k > kRtMaxK || T > INT32_MAX) return GNF4B_ETOOBIG;
+    return GNF4B_OK;
+}
+
+template <int LT, int NE>
+cudaError_t rt_fwd(const RouteTrainArgs& a, int grid, cudaStream_t st) {
+    const size_t smem = (size_t)kRtWarps * a.E * 8;
+    auto kfn = route_train_fwd_kernel<LT, NE, kRtWarps>;
+    static int granted[64];
+    cudaError_t e = ensure_smem(kfn, smem, granted);
+    if (e != cudaSuccess) return e;
+    e = launch_pdl_smem(kfn, (unsigned)grid, (unsigned)(kRtWarps * 32), smem, st, a);
+    if (e != cudaSuccess || grid == 1) return e;
+    return launch_pdl(route_train_finish_kernel, 1u, 1024u, st, a, grid);
+}
+template <int LT, int NE>
+cudaError_t rt_bwd(const RouteTrainBwdArgs& a, int grid, cudaStream_t st) {
+    const size_t smem = (size_t)kRtWarps * a.E * 4;
+    return launch_pdl_smem(route_train_bwd_kernel<LT, NE, kRtWarps>, (unsigned)grid, (unsigned)(kRtWarps * 32), smem, st, a);
+}
+
+template <typename F2, typename F4, typename F8, typename F16, typename F32, typename F1>
+cudaError_t by_experts(int32_t E, F1 f1, F2 f2, F4 f4, F8 f8, F16 f16, F32 f32) {
+    return E <= 32 ? f1() : E <= 64 ? f2() : E <= 128 ? f4() : E <= 256 ? f8() : E <= 512 ? f16() : f32();
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t gnf4b_route_train_scratch_bytes(int64_t T, int32_t E) {
+    DevInfo di;
+    if (T <= 0 || E <= 0 || device_info(&di)) return 0;
+    const int grid = rt_grid(T, di.sm_count);
+    return grid == 1 ? 0 : (size_t)grid * ((size_t)E * 8 + 8);
+}
+
+int gnf4b_route_train_fwd(const void* logits, int dtype, int64_t T, int64_t stride, int32_t E, int32_t k, int32_t mode, int32_t norm,
+                          const uint8_t* token_mask, int64_t* idx, float* weights, float* lse, int32_t* counts, float* balance_loss,
+                          float* z_loss, float* n_tokens, void* scratch, size_t scratch_bytes, void* cuda_stream) {
+    int rc = rt_check(dtype, T, stride, E, k, mode, norm);
+    if (rc) return rc;
+    if (!counts || !balance_loss || !z_loss || !n_tokens || (T > 0 && (!logits || !idx || !weights || !lse))) return GNF4B_EINVAL;
+    DevInfo di;
+    rc = device_info(&di);
+    if (rc) return rc;
+    const int grid = rt_grid(T, di.sm_count);
+    if (grid > 1 && (!scratch || !aligned(scratch, 8) || scratch_bytes < (size_t)grid * ((size_t)E * 8 + 8))) return GNF4B_EWORKSPACE;
+    RouteTrainArgs a;
+    a.logits = logits; a.T = T; a.stride = stride; a.E = E; a.k = k; a.mode = mode; a.norm = norm;
+    a.mask = token_mask; a.idx = idx; a.w = weights; a.lse = lse; a.counts = counts;
+    a.balance = balance_loss; a.z = z_loss; a.n_tokens = n_tokens;
+    a.part_p = static_cast<float*>(scratch);
+    a.part_c = reinterpret_cast<int32_t*>(a.part_p + (size_t)grid * E);
+    a.part_zn = reinterpret_cast<float*>(a.part_c + (size_t)grid * E);
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
+#define GNF4B_RT(L) by_experts(E, [&] { return rt_fwd<L, 1>(a, grid, st); }, [&] { return rt_fwd<L, 2>(a, grid, st); }, \
+        [&] { return rt_fwd<L, 4>(a, grid, st); }, [&] { return rt_fwd<L, 8>(a, grid, st); }, [&] { return rt_fwd<L, 16>(a, grid, st); }, \
+        [&] { return rt_fwd<L, 32>(a, grid, st); })
+    const cudaError_t e = dtype == GNF4B_X_BF16 ? GNF4B_RT(0) : dtype == GNF4B_X_FP16 ? GNF4B_RT(1) : GNF4B_RT(2);
+#undef GNF4B_RT
+    return e == cudaSuccess ? GNF4B_OK : cuda_fail(e, "route_train_fwd launch");
+}
+
+int gnf4b_route_train_bwd(const void* logits, int dtype, int64_t T, int64_t stride, int32_t E, int32_t k, int32_t mode, int32_t norm,
+                          const uint8_t* token_mask, const int64_t* idx, const float* weights, const float* lse, const int32_t* counts,
+                          const float* n_tokens, const float* g_weights, const float* g_balance, const float* g_z, void* grad,
+                          void* cuda_stream) {
+    int rc = rt_check(dtype, T, stride, E, k, mode, norm);
+    if (rc) return rc;
+    if (T == 0) return GNF4B_OK;
+    if (!logits || !idx || !weights || !lse || !counts || !n_tokens || !grad) return GNF4B_EINVAL;
+    DevInfo di;
+    rc = device_info(&di);
+    if (rc) return rc;
+    RouteTrainBwdArgs a;
+    a.logits = logits; a.T = T; a.stride = stride; a.E = E; a.k = k; a.mode = mode; a.norm = norm;
+    a.mask = token_mask; a.idx = idx; a.w = weights; a.lse = lse; a.counts = counts; a.n_tokens = n_tokens;
+    a.g_w = g_weights; a.g_balance = g_balance; a.g_z = g_z; a.grad = grad;
+    const int grid = (int)std::min<int64_t>(ceil_div(T, kRtWarps), (int64_t)di.sm_count * 8);
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
+#define GNF4B_RT(L) by_experts(E, [&] { return rt_bwd<L, 1>(a, grid, st); }, [&] { return rt_bwd<L, 2>(a, grid, st); }, \
+        [&] { return rt_bwd<L, 4>(a, grid, st); }, [&] { return rt_bwd<L, 8>(a, grid, st); }, [&] { return rt_bwd<L, 16>(a, grid, st); }, \
+        [&] { return rt_bwd<L, 32>(a, grid, st); })
+    const cudaError_t e = dtype == GNF4B_X_BF16 ? GNF4B_RT(0) : dtype == GNF4B_X_FP16 ? GNF4B_RT(1) : GNF4B_RT(2);
+#undef GNF4B_RT
+    return e == cudaSuccess ? GNF4B_OK : cuda_fail(e, "route_train_bwd launch");
+}
+
+int gnf4b_glu_ckpt8_fwd(const void* gate_up, int64_t rows, int64_t h, int act, const void* bias, const int32_t* row_expert, int32_t E,
+                        void* out, int8_t* codes, float* steps, int32_t* status_word, void* cuda_stream) {
+    if (rows < 0 || (act != GNF4B_ACT_SILU_GLU && act != GNF4B_ACT_GPT_OSS_GLU)) return GNF4B_EINVAL;
+    if (h <= 0) return GNF4B_ESHAPE;
+    if (bias && (act != GNF4B_ACT_GPT_OSS_GLU || !row_expert || E <= 0)) return GNF4B_EINVAL;
+    if ((codes == nullptr) != (steps == nullptr)) return GNF4B_EINVAL;
+    if (rows == 0) return GNF4B_OK;
+    if (!gate_up || !out || !aligned(gate_up, 2) || !aligned(out, 2) || !aligned(codes, 8) || !aligned(steps, 8)) return GNF4B_EINVAL;
+    const int64_t nb = ceil_div(h, kCkBlock);
+    if (h > (int64_t)1 << 40 || rows > (int64_t)INT32_MAX * kCkThreads / 8 / nb) return GNF4B_ETOOBIG;
+    const unsigned grid = (unsigned)ceil_div(rows * nb * 8, kCkThreads);
+    const bool vec = h % 8 == 0 && aligned(gate_up, 16) && aligned(out, 16);
+    const bool keep = codes != nullptr;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
+    cudaError_t e;
+#define GNF4B_CK(A, V, K) launch_pdl(glu_ckpt8_fwd_kernel<A, V, K>, grid, (unsigned)kCkThreads, st, static_cast<const uint16_t*>(gate_up), rows, h, \
+        static_cast<const uint16_t*>(bias), row_expert, E, static_cast<uint16_t*>(out), reinterpret_cast<uint2*>(codes), \
+        reinterpret_cast<float2*>(steps), status_word)
+    if (act == GNF4B_ACT_SILU_GLU) e = keep ? (vec ? GNF4B_CK(0, true, true) : GNF4B_CK(0, false, true)) : (vec ? GNF4B_CK(0, true, false) : GNF4B_CK(0, false, false));
+    else e = keep ? (vec ? GNF4B_CK(1, true, true) : GNF4B_CK(1, false, true)) : (vec ? GNF4B_CK(1, true, false) : GNF4B_CK(1, false, false));
+#undef GNF4B_CK
+    return e == cudaSuccess ? GNF4B_OK : cuda_fail(e, "glu_ckpt8_fwd launch");
+}
+
+int gnf4b_glu_ckpt8_bwd(const void* grad_out, const int8_t* codes, const float* steps, int64_t rows, int64_t h, int act,
+                        void* grad_gate_up, void* cuda_stream) {
+    if (rows < 0 || (act != GNF4B_ACT_SILU_GLU && act != GNF4B_ACT_GPT_OSS_GLU)) return GNF4B_EINVAL;
+    if (h <= 0) return GNF4B_ESHAPE;
+    if (rows == 0) return GNF4B_OK;
+    if (!grad_out || !codes || !steps || !grad_gate_up || !aligned(grad_out, 2) || !aligned(grad_gate_up, 2) || !aligned(codes, 8) ||
+        !aligned(steps, 8))
+        return GNF4B_EINVAL;
+    const int64_t nb = ceil_div(h, kCkBlock);
+    if (h > (int64_t)1 << 40 || rows > (int64_t)INT32_MAX * kCkThreads / 8 / nb) return GNF4B_ETOOBIG;
+    const unsigned grid = (unsigned)ceil_div(rows * nb * 8, kCkThreads);
+    const bool vec = h % 8 == 0 && aligned(grad_out, 16) && aligned(grad_gate_up, 16);
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
+    cudaError_t e;
+#define GNF4B_CK(A, V) launch_pdl(glu_ckpt8_bwd_kernel<A, V>, grid, (unsigned)kCkThreads, st, static_cast<const uint16_t*>(grad_out), \
+        reinterpret_cast<const uint2*>(codes), reinterpret_cast<const float2*>(steps), rows, h, static_cast<uint16_t*>(grad_gate_up))
+    if (act == GNF4B_ACT_SILU_GLU) e = vec ? GNF4B_CK(0, true) : GNF4B_CK(0, false);
+    else e = vec ? GNF4B_CK(1, true) : GNF4B_CK(1, false);
+#undef GNF4B_CK
+    return e == cudaSuccess ? GNF4B_OK : cuda_fail(e, "glu_ckpt8_bwd launch");
+}
+
+}  // extern "C"

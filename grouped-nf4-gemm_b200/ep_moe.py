@@ -39,6 +39,7 @@ from __future__ import annotations
 import os
 import statistics
 import time
+from typing import NamedTuple
 
 import torch
 import torch.distributed as dist
@@ -110,6 +111,140 @@ def route_topk(logits: torch.Tensor, k: int, mode: int = 0, norm: bool = False):
     else:
         w = torch.softmax(top, dim=-1)
     return idx, w
+
+
+class RoutingTrain(NamedTuple):
+    """What ``route_topk_train`` returns; ``weights``, ``balance_loss`` and ``z_loss`` carry gradients to the logits."""
+    idx: torch.Tensor             # [M, k] int64
+    weights: torch.Tensor         # [M, k] fp32
+    counts: torch.Tensor          # [E] int32, tokens that chose each expert
+    balance_loss: torch.Tensor    # fp32 scalar
+    z_loss: torch.Tensor          # fp32 scalar
+
+
+class _RouteTopkTrain(torch.autograd.Function):
+    """One kernel forward (two from 129 tokens on), one backward; kept between them: the logits (as given), the log-sums
+    [M], ids, weights and counts."""
+
+    @staticmethod
+    def forward(ctx, logits, k, mode, norm, token_mask):
+        import _gnf4b
+        from nf4_grouped import _call_on
+        lib = _gnf4b.load()
+        dev = logits.device
+        M, E = logits.shape
+        idx = torch.empty(M, k, dtype=torch.int64, device=dev)
+        w = torch.empty(M, k, dtype=torch.float32, device=dev)
+        lse = torch.empty(M + 1, dtype=torch.float32, device=dev)          # and the number of tokens that count
+        counts = torch.empty(E, dtype=torch.int32, device=dev)
+        balance = torch.empty((), dtype=torch.float32, device=dev)
+        z = torch.empty((), dtype=torch.float32, device=dev)
+        need = _route_scratch(lib, dev, M, E)
+        scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        stride = logits.stride(0) if M > 1 else E
+        rc = _call_on(dev, lib.gnf4b_route_train_fwd, logits.data_ptr(), _ROUTE_DTYPES[logits.dtype], M, stride, E, k, mode, norm,
+                      token_mask.data_ptr() if token_mask is not None else None, idx.data_ptr(), w.data_ptr(), lse.data_ptr(),
+                      counts.data_ptr(), balance.data_ptr(), z.data_ptr(), lse.data_ptr() + 4 * M,
+                      scratch.data_ptr() if need else None, need)
+        if rc:
+            _gnf4b.check(rc, "gnf4b_route_train_fwd")
+        ctx.save_for_backward(logits, token_mask, idx, w, lse, counts)
+        ctx.rule = (k, mode, norm)
+        ctx.mark_non_differentiable(idx, counts)
+        ctx.set_materialize_grads(False)
+        return idx, w, counts, balance, z
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, _g_idx, g_w, _g_counts, g_balance, g_z):
+        import _gnf4b
+        from nf4_grouped import _call_on
+        logits, token_mask, idx, w, lse, counts = ctx.saved_tensors
+        k, mode, norm = ctx.rule
+        M, E = logits.shape
+        if g_w is not None:
+            g_w = g_w.contiguous()
+        grad = torch.empty(M, E, dtype=logits.dtype, device=logits.device)
+        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+        rc = _call_on(logits.device, _gnf4b.load().gnf4b_route_train_bwd, logits.data_ptr(), _ROUTE_DTYPES[logits.dtype], M,
+                      logits.stride(0) if M > 1 else E, E, k, mode, norm, ptr(token_mask), idx.data_ptr(), w.data_ptr(),
+                      lse.data_ptr(), counts.data_ptr(), lse.data_ptr() + 4 * M, ptr(g_w), ptr(g_balance), ptr(g_z),
+                      grad.data_ptr())
+        if rc:
+            _gnf4b.check(rc, "gnf4b_route_train_bwd")
+        return grad, None, None, None, None
+
+
+_ROUTE_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}        # GNF4B_X_*
+ROUTE_TRAIN_MAX_EXPERTS, ROUTE_TRAIN_MAX_K = 1024, 32
+
+
+def _route_scratch(lib, dev, M, E):
+    key = (dev.index, M, E)
+    need = _ROUTE_SCRATCH.get(key)
+    if need is None:
+        with torch.cuda.device(dev):
+            need = lib.gnf4b_route_train_scratch_bytes(M, E)
+        if len(_ROUTE_SCRATCH) < 4096:
+            _ROUTE_SCRATCH[key] = need
+    return need
+
+
+_ROUTE_SCRATCH: dict = {}        # (device, tokens, experts) -> bytes
+
+
+def route_topk_train(logits: torch.Tensor, k: int, mode: int = 0, norm: bool = False, *, token_mask=None) -> RoutingTrain:
+    """``route_topk`` for training: the same selection and weights on ``logits [M, E]`` (bf16, fp16 or fp32), the
+    per-expert counts and two losses, all differentiable in the logits but the ids and counts (constants of the loss).
+    Over the n tokens that count -- all, or those where the bool ``token_mask [M]`` is true, never one whose logits are
+    all -inf --
+
+        balance_loss = E * sum_e (counts_e / (n k)) * mean_t softmax(logits_t)_e        (1 when even)
+        z_loss       = mean_t logsumexp(logits_t)^2
+
+    and both are 0 when no token counts.  A masked token is routed and weighted all the same (a batch's padding; mask
+    its result, not its route).  A token whose logits are all -inf gets weights 0 and no gradient.  On a GPU one kernel
+    each way (E <= 1024, k <= 32); on the CPU the same in tensor operations."""
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be [tokens, experts], got shape {tuple(logits.shape)}")
+    if logits.dtype not in _ROUTE_DTYPES:
+        raise TypeError(f"logits must be bfloat16, float16 or float32, got {logits.dtype}")
+    M, E = logits.shape
+    if not 1 <= k <= E:
+        raise ValueError(f"k={k} is not in 1 .. {E} (the number of experts)")
+    if mode not in (0, 1):
+        raise ValueError(f"mode is 0 (softmax over all experts) or 1 (over the chosen), got {mode}")
+    if token_mask is not None and (token_mask.dtype != torch.bool or tuple(token_mask.shape) != (M,) or token_mask.device != logits.device):
+        raise ValueError(f"token_mask must be a bool tensor of {M} tokens on {logits.device}")
+    if not logits.is_cuda:
+        return _route_train_ops(logits, k, mode, norm, token_mask)
+    if E > ROUTE_TRAIN_MAX_EXPERTS or k > ROUTE_TRAIN_MAX_K:
+        raise ValueError(f"route_topk_train takes up to {ROUTE_TRAIN_MAX_EXPERTS} experts and k up to {ROUTE_TRAIN_MAX_K}, got {E} and {k}")
+    if logits.stride(1) != 1 and E > 1:
+        logits = logits.contiguous()
+    if token_mask is not None:
+        token_mask = token_mask.contiguous()
+    return RoutingTrain(*_RouteTopkTrain.apply(logits, int(k), int(mode), int(bool(norm)), token_mask))
+
+
+def _route_train_ops(logits, k, mode, norm, token_mask):
+    """The same in tensor operations (CPU tensors)."""
+    lg = logits.float()
+    E = lg.shape[1]
+    idx = torch.argsort(-lg.detach(), dim=-1, stable=True)[:, :k]
+    dead = (lg.detach() == float("-inf")).all(1)
+    keep = ~dead if token_mask is None else token_mask & ~dead
+    safe = lg.masked_fill(dead[:, None], 0.0)
+    logp = torch.log_softmax(safe, dim=-1)
+    w = torch.softmax(torch.gather(safe, 1, idx), dim=-1) if mode == 1 or norm else torch.exp(torch.gather(logp, 1, idx))
+    w = w.masked_fill(dead[:, None], 0.0)
+    n = keep.sum().clamp_min(1).float()
+    chosen = torch.zeros_like(lg).scatter_(1, idx, 1.0)
+    counts = (chosen * keep[:, None]).sum(0).to(torch.int32)
+    mean_p = torch.exp(logp)[keep].sum(0) / n
+    balance = E * (counts.float() / (n * k) * mean_p).sum()
+    z = torch.logsumexp(lg[keep], dim=-1).square().sum() / n
+    return RoutingTrain(idx, w, counts, balance, z)
 
 
 def plan_dispatch(idx: torch.Tensor, n_experts: int, world: int):

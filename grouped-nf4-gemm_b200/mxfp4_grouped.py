@@ -15,7 +15,7 @@ from __future__ import annotations
 import torch
 
 import _gnf4b
-from nf4_grouped import (_dispatch, _group_tables, _launch, _launch_ffn, _launch_host, _prefill_block_m,  # noqa: F401  (re-exported names)
+from nf4_grouped import (_call_on, _dispatch, _group_tables, _launch, _launch_ffn, _launch_host, _prefill_block_m,  # noqa: F401  (re-exported names)
                          _raw_stream, _require_cuda, _status_ptr, build_group_tiles)
 
 # e2m1 codebook, index = (sign << 3) | magnitude (ref :34-35)
@@ -170,10 +170,10 @@ def quantize_mxfp4(x):
             x = x.contiguous()
     blocks = torch.empty(*lead, K // 2, dtype=torch.uint8, device=x.device)
     scales = torch.empty(*lead, K // MX_BLOCK, dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
-        rc = _gnf4b.load().gnf4b_quantize_mxfp4(x.data_ptr(), _X_DTYPES[x.dtype], x.shape[0], K, x.stride(0) if x.shape[0] > 1 else K,
-                                                blocks.data_ptr(), scales.data_ptr(), _raw_stream(x.device))
-    _gnf4b.check(rc, "gnf4b_quantize_mxfp4")
+    rc = _call_on(x.device, _gnf4b.load().gnf4b_quantize_mxfp4, x.data_ptr(), _X_DTYPES[x.dtype], x.shape[0], K,
+                  x.stride(0) if x.shape[0] > 1 else K, blocks.data_ptr(), scales.data_ptr())
+    if rc:
+        _gnf4b.check(rc, "gnf4b_quantize_mxfp4")
     return blocks, scales
 
 
@@ -202,10 +202,10 @@ def dequantize_mxfp4(blocks, scales, dtype=torch.bfloat16):
     _check_packed(blocks, scales, "dequantize_mxfp4")
     blocks, scales = _packed_rows(blocks, 4), scales.contiguous()
     out = torch.empty(*blocks.shape[:-1], 2 * blocks.shape[-1], dtype=dtype, device=blocks.device)
-    with torch.cuda.device(blocks.device):
-        rc = _gnf4b.load().gnf4b_dequantize_mxfp4(blocks.data_ptr(), scales.data_ptr(), scales.numel(), _X_DTYPES[dtype],
-                                                  out.data_ptr(), _raw_stream(blocks.device))
-    _gnf4b.check(rc, "gnf4b_dequantize_mxfp4")
+    rc = _call_on(blocks.device, _gnf4b.load().gnf4b_dequantize_mxfp4, blocks.data_ptr(), scales.data_ptr(), scales.numel(),
+                  _X_DTYPES[dtype], out.data_ptr())
+    if rc:
+        _gnf4b.check(rc, "gnf4b_dequantize_mxfp4")
     return out
 
 
@@ -236,12 +236,12 @@ def glu_quantize_mxfp4(gate_up, act: str = "silu", bias=None, row_expert=None):
         bias, row_expert = bias.detach().contiguous(), row_expert.to(torch.int32).contiguous()
     blocks = torch.empty(rows, h // 2, dtype=torch.uint8, device=dev)
     scales = torch.empty(rows, h // MX_BLOCK, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        rc = _gnf4b.load().gnf4b_glu_quantize_mxfp4(
-            gate_up.data_ptr(), rows, h, _gnf4b.ACT_SILU_GLU if act == "silu" else _gnf4b.ACT_GPT_OSS_GLU,
-            bias.data_ptr() if bias is not None else None, row_expert.data_ptr() if bias is not None else None, E,
-            blocks.data_ptr(), scales.data_ptr(), _status_ptr(dev), _raw_stream(dev))
-    _gnf4b.check(rc, "gnf4b_glu_quantize_mxfp4")
+    rc = _call_on(dev, _gnf4b.load().gnf4b_glu_quantize_mxfp4, gate_up.data_ptr(), rows, h,
+                  _gnf4b.ACT_SILU_GLU if act == "silu" else _gnf4b.ACT_GPT_OSS_GLU,
+                  bias.data_ptr() if bias is not None else None, row_expert.data_ptr() if bias is not None else None, E,
+                  blocks.data_ptr(), scales.data_ptr(), _status_ptr(dev))
+    if rc:
+        _gnf4b.check(rc, "gnf4b_glu_quantize_mxfp4")
     return blocks, scales
 
 

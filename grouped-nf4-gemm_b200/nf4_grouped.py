@@ -373,6 +373,15 @@ def _raw_stream(dev) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
 
 
+def _call_on(dev, fn, *args) -> int:
+    """A library launch on ``dev`` and torch's current stream there (the stream is the last argument of every entry
+    point); the device is switched only when it is not the current one."""
+    if dev.index == torch.cuda.current_device():
+        return fn(*args, _raw_stream(dev))
+    with torch.cuda.device(dev):
+        return fn(*args, _raw_stream(dev))
+
+
 def _status_ptr(dev) -> int:
     ptr = _STATUS_PTR.get(dev.index)
     if ptr is None:

@@ -14,7 +14,9 @@ Same names, argument meaning and defaults as the reference:
                        scaling=1.0, dgrad_kernel=True)
 
 plus ``gemm_mxfp4_grouped_train`` (the reference's MXFP4 backward is a Python loop over experts; here it is
-the same dgrad kernel with the MXFP4 decode).
+the same dgrad kernel with the MXFP4 decode), ``gemm_mxfp4_grouped_w4a4_train`` (rows in MXFP4 forward, straight-through
+gradient) and the whole expert FFN for training: ``glu_train``, the activation between the two products that keeps its
+input in 8 bits for the backward pass, and ``ffn_4bit_grouped_train`` / ``ffn_mxfp4_grouped_train`` around it.
 """
 from __future__ import annotations
 
@@ -160,3 +162,133 @@ def fused_grouped_lora(a_cat, packed, absmax, sizes, expert_ids, lora_A=None, lo
         return out
     delta = lora_delta_grouped(a_cat, lora_A, lora_B, sizes, expert_ids, scaling)
     return out if delta is None else out + delta.to(out.dtype)
+
+
+# --------------------------------------------------------------------------- #
+# both operands in MXFP4
+# --------------------------------------------------------------------------- #
+class FusedGroupedMxfp4W4A4(torch.autograd.Function):
+    """Forward ``gemm_mxfp4_grouped_w4a4`` on the quantised rows; backward ``dgrad_mxfp4_grouped``, the quantiser taken
+    as the identity (straight-through)."""
+
+    @staticmethod
+    def forward(ctx, a_cat, blocks, scales, sizes, expert_ids):
+        from mxfp4_grouped import gemm_mxfp4_grouped_w4a4, quantize_mxfp4
+        ctx.stack = (blocks, scales)
+        ctx.sizes, ctx.expert_ids = sizes, expert_ids
+        ctx.a_dtype = a_cat.dtype
+        return gemm_mxfp4_grouped_w4a4(*quantize_mxfp4(a_cat), blocks, scales, sizes, expert_ids)
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        if not ctx.needs_input_grad[0]:
+            return (None,) * 5
+        from mxfp4_grouped import dgrad_mxfp4_grouped
+        blocks, scales = ctx.stack
+        grad = dgrad_mxfp4_grouped(grad_out.contiguous(), blocks, scales, ctx.sizes, ctx.expert_ids)
+        return (grad.to(ctx.a_dtype),) + (None,) * 4
+
+
+def gemm_mxfp4_grouped_w4a4_train(a_cat, blocks, scales, sizes, expert_ids):
+    """``quantize_mxfp4`` then ``gemm_mxfp4_grouped_w4a4``, with the gradient of the unquantised product."""
+    return FusedGroupedMxfp4W4A4.apply(a_cat, blocks, scales, sizes, expert_ids)
+
+
+# --------------------------------------------------------------------------- #
+# the activation between an expert's products, its input kept in 8 bits
+# --------------------------------------------------------------------------- #
+CKPT_BLOCK = 64        # gate (or up) values that share one fp32 step
+_GLU_ACTS = {"silu": 0, "gpt_oss": 1}        # GNF4B_ACT_*
+
+
+class _GluTrain(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gate_up, act, bias, row_expert):
+        import _gnf4b
+        from nf4_grouped import _call_on, _status_ptr
+        dev = gate_up.device
+        rows, h = gate_up.shape[0], gate_up.shape[1] // 2
+        out = torch.empty(rows, h, dtype=torch.bfloat16, device=dev)
+        codes = steps = None
+        if ctx.needs_input_grad[0]:
+            nb = -(-h // CKPT_BLOCK)
+            codes = torch.empty(rows, nb, 2, CKPT_BLOCK, dtype=torch.int8, device=dev)
+            steps = torch.empty(rows, nb, 2, dtype=torch.float32, device=dev)
+        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+        rc = _call_on(dev, _gnf4b.load().gnf4b_glu_ckpt8_fwd, gate_up.data_ptr(), rows, h, act, ptr(bias), ptr(row_expert),
+                      bias.shape[0] if bias is not None else 0, out.data_ptr(), ptr(codes), ptr(steps), _status_ptr(dev))
+        if rc:
+            _gnf4b.check(rc, "gnf4b_glu_ckpt8_fwd")
+        if codes is not None:
+            ctx.save_for_backward(codes, steps)
+        ctx.act, ctx.h = act, h
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        import _gnf4b
+        from nf4_grouped import _call_on
+        codes, steps = ctx.saved_tensors
+        grad_out = grad_out.contiguous()
+        rows = codes.shape[0]
+        grad = torch.empty(rows, 2 * ctx.h, dtype=torch.bfloat16, device=codes.device)
+        rc = _call_on(codes.device, _gnf4b.load().gnf4b_glu_ckpt8_bwd, grad_out.data_ptr(), codes.data_ptr(), steps.data_ptr(), rows,
+                      ctx.h, ctx.act, grad.data_ptr())
+        if rc:
+            _gnf4b.check(rc, "gnf4b_glu_ckpt8_bwd")
+        return grad, None, None, None
+
+
+def glu_train(gate_up, act: str = "silu", *, bias=None, row_expert=None):
+    """The activation between an expert's two products, differentiable: ``gate_up [rows, 2h]`` bf16 -> ``[rows, h]`` bf16.
+    ``act="silu"``: SiLU(gate) * up over column halves; ``act="gpt_oss"``: gate and up interleaved, clamped at 7,
+    (up + 1) * gate * sigmoid(1.702 gate), with an optional frozen ``bias`` bf16 ``[E, 2h]`` added by ``row_expert [rows]``.
+    fp32 inside, one rounding.
+
+    What stays until the backward pass is gate and up in 8 bits (per 64 values of a row one fp32 step, their largest
+    magnitude / 127): 2.1 bytes per pair where autograd through tensor operations keeps 10 and more, and neither
+    ``gate_up`` nor the result need stay alive.  The gradient is the formula's, taken at the kept values.  Without a
+    gradient to compute nothing is kept."""
+    from nf4_grouped import _require_cuda
+    if act not in _GLU_ACTS:
+        raise ValueError("act is 'gpt_oss' or 'silu'")
+    _require_cuda(gate_up, "glu_train", "")
+    if gate_up.dtype != torch.bfloat16:
+        raise TypeError(f"gate_up must be bfloat16, got {gate_up.dtype}")
+    if gate_up.dim() != 2 or gate_up.shape[1] == 0 or gate_up.shape[1] % 2:
+        raise ValueError(f"gate_up must be [rows, 2h], got {tuple(gate_up.shape)}")
+    if bias is not None:
+        rows, dev = gate_up.shape[0], gate_up.device
+        if act != "gpt_oss" or row_expert is None:
+            raise ValueError("bias goes with act='gpt_oss' and row_expert")
+        if bias.requires_grad and torch.is_grad_enabled():
+            raise ValueError("the bias of glu_train is frozen: add a trainable one to gate_up before the call")
+        if bias.dtype != torch.bfloat16 or bias.dim() != 2 or bias.shape[1] != gate_up.shape[1] or bias.shape[0] == 0 or bias.device != dev:
+            raise ValueError(f"bias must be a bfloat16 tensor [E, {gate_up.shape[1]}] on {dev}")
+        if tuple(row_expert.shape) != (rows,) or row_expert.device != dev or row_expert.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"row_expert must be an integer tensor of {rows} expert ids on {dev}")
+        bias, row_expert = bias.detach().contiguous(), row_expert.to(torch.int32).contiguous()
+    return _GluTrain.apply(gate_up.contiguous(), _GLU_ACTS[act], bias, row_expert)
+
+
+def ffn_4bit_grouped_train(a_cat, packed_gu, absmax_gu, packed_dn, absmax_dn, sizes, expert_ids, *, act: str = "silu",
+                           lora_gu=None, lora_dn=None, scaling=1.0, dgrad_kernel=True):
+    """One NF4 expert FFN per row for training: gate_up and down through ``fused_grouped_lora`` (frozen stacks,
+    ``lora_gu`` / ``lora_dn`` optional ``(lora_A, lora_B)`` pairs) with ``glu_train`` between them.  ``[T, K]`` bf16 ->
+    ``[T, N_dn]`` bf16; besides the low-rank branch, a layer keeps its gate_up activations in 8 bits and nothing else."""
+    gu = fused_grouped_lora(a_cat, packed_gu, absmax_gu, sizes, expert_ids, *(lora_gu or (None, None)), scaling=scaling,
+                            dgrad_kernel=dgrad_kernel)
+    return fused_grouped_lora(glu_train(gu, act), packed_dn, absmax_dn, sizes, expert_ids, *(lora_dn or (None, None)),
+                              scaling=scaling, dgrad_kernel=dgrad_kernel)
+
+
+def ffn_mxfp4_grouped_train(a_cat, blocks_gu, scales_gu, blocks_dn, scales_dn, sizes, expert_ids, *, act: str = "gpt_oss",
+                            bias_gu=None, row_expert=None, rows: str = "bf16"):
+    """The MXFP4 counterpart on frozen stacks.  ``rows="mxfp4"`` multiplies MXFP4 rows forward
+    (``gemm_mxfp4_grouped_w4a4_train``), ``"bf16"`` the rows as they are."""
+    if rows not in ("bf16", "mxfp4"):
+        raise ValueError("rows is 'bf16' or 'mxfp4'")
+    product = gemm_mxfp4_grouped_train if rows == "bf16" else gemm_mxfp4_grouped_w4a4_train
+    gu = product(a_cat, blocks_gu, scales_gu, sizes, expert_ids)
+    return product(glu_train(gu, act, bias=bias_gu, row_expert=row_expert), blocks_dn, scales_dn, sizes, expert_ids)

@@ -468,6 +468,40 @@ int gnf4b_gemm_grouped_w4a4(const uint8_t* x_blocks, const uint8_t* x_scales, in
                             const int32_t* group_offsets, const int32_t* expert_ids, int32_t G, int32_t E,
                             int64_t N, int64_t K, int32_t max_rows, void* out, int32_t* status_word, void* cuda_stream);
 
+/* Routing for training.  Selection and weights as gnf4b_route_topk, on logits [T, E] of bf16, fp16 or fp32 (rows `stride`
+ * elements apart; E <= 1024, k <= 32), with what a training step needs beside them.  Over the n tokens that count (all,
+ * or those with token_mask[t] != 0; never a token whose logits are all -inf):
+ *   counts[E] tokens that chose the expert;   balance_loss = E sum_e (counts_e / (n k)) mean_t p[t, e]   (1 when even)
+ *   z_loss = mean_t (log sum_e exp logits[t, e])^2;   n_tokens = n as a float;   n = 0: both losses 0
+ * Masked tokens are routed all the same.  A token whose logits are all -inf gets weights 0.  A NaN logit is chosen after
+ * every other one; the token's weights and, if it counts, the losses are NaN.  lse [T] is kept for the backward pass.
+ * scratch: gnf4b_route_train_scratch_bytes(T, E) bytes (8-byte aligned, any content; 0 for small batches), not shared by
+ * calls that overlap.  Deterministic (no floating-point atomics).
+ * gnf4b_route_train_bwd: grad [T, E] (contiguous, the logits' type) from g_weights [T, k] (fp32), g_balance and g_z
+ * (device scalars, fp32), each optional; the counts are constants of the balance loss. */
+size_t gnf4b_route_train_scratch_bytes(int64_t T, int32_t E);
+int gnf4b_route_train_fwd(const void* logits, int dtype, int64_t T, int64_t stride, int32_t E, int32_t k, int32_t mode,
+                          int32_t norm, const uint8_t* token_mask, int64_t* idx, float* weights, float* lse,
+                          int32_t* counts, float* balance_loss, float* z_loss, float* n_tokens, void* scratch,
+                          size_t scratch_bytes, void* cuda_stream);
+int gnf4b_route_train_bwd(const void* logits, int dtype, int64_t T, int64_t stride, int32_t E, int32_t k, int32_t mode,
+                          int32_t norm, const uint8_t* token_mask, const int64_t* idx, const float* weights,
+                          const float* lse, const int32_t* counts, const float* n_tokens, const float* g_weights,
+                          const float* g_balance, const float* g_z, void* grad, void* cuda_stream);
+
+/* The GLU between an expert's two products, for training: out bf16 [rows, h] = act(gate_up bf16 [rows, 2h]) in fp32 with
+ * one rounding (GNF4B_ACT_SILU_GLU: halves; GNF4B_ACT_GPT_OSS_GLU: interleaved, clamped at 7, optional bias bf16 [E, 2h]
+ * by row_expert), and its input kept in 8 bits: with nb = ceil(h / 64), codes int8 [rows, nb, 2, 64] and steps fp32
+ * [rows, nb, 2] (0: gate, 1: up), value = code * step, step = the 64 values' largest magnitude / 127.  codes and steps
+ * are 8-byte aligned, or both null (nothing kept).  A row whose expert is outside [0, E) gets no bias and raises
+ * GNF4B_ST_BAD_EXPERT.
+ * gnf4b_glu_ckpt8_bwd: grad_gate_up bf16 [rows, 2h] from grad_out bf16 [rows, h] and the checkpoint alone, the
+ * derivative taken at the kept values. */
+int gnf4b_glu_ckpt8_fwd(const void* gate_up, int64_t rows, int64_t h, int act, const void* bias, const int32_t* row_expert,
+                        int32_t E, void* out, int8_t* codes, float* steps, int32_t* status_word, void* cuda_stream);
+int gnf4b_glu_ckpt8_bwd(const void* grad_out, const int8_t* codes, const float* steps, int64_t rows, int64_t h, int act,
+                        void* grad_gate_up, void* cuda_stream);
+
 /* Device properties this library plans with (SM count, opt-in shared memory). */
 int gnf4b_device_info(int32_t* sm_count, int32_t* smem_optin_bytes);
 
