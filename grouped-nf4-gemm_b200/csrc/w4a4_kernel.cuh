@@ -94,6 +94,14 @@ __device__ __forceinline__ uint32_t mxf4_idesc(uint32_t n_umma, uint32_t sf_id) 
     return (sf_id << 4) | (1u << 7) | (1u << 10) | ((n_umma >> 3) << 17) | (1u << 23) | (8u << 24) | (sf_id << 29);
 }
 
+// one lane of the warp, always the same one
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.b32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p != 0;
+}
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 struct QGroup {
     int32_t row0, rows, eid, chunk_rows;
 };
@@ -158,41 +166,40 @@ __device__ __forceinline__ void build_qtable(const W4A4Args& a, QGroup* grp, int
     if (t == 0) base[0] = 0;
 }
 
-// Up to 32 scale bytes from p (any alignment) into 8 words, zeros behind the first `valid`.  [lo, hi) is the scale
-// tensor: a 4-byte word that would reach outside it is put together from its bytes.
+// Up to 32 scale bytes from p (any alignment) into 8 words, zeros behind the first `valid` (the same for all lanes).
+// [lo, hi) is the scale tensor: aligned words around the bytes are read where they lie inside it (all rows but its
+// first and last), single bytes otherwise.
 __device__ __forceinline__ void load_scale_span(const uint8_t* p, int valid, const uint8_t* lo, const uint8_t* hi, uint32_t* out) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) out[j] = 0;
-    if (valid <= 0) return;
     if (valid >= 32 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
         const uint4 v0 = __ldg(reinterpret_cast<const uint4*>(p)), v1 = __ldg(reinterpret_cast<const uint4*>(p) + 1);
         out[0] = v0.x; out[1] = v0.y; out[2] = v0.z; out[3] = v0.w;
         out[4] = v1.x; out[5] = v1.y; out[6] = v1.z; out[7] = v1.w;
         return;
     }
-    valid = min(valid, 32);
     const uint32_t skip = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 3);
     const uint8_t* a = p - skip;
-    uint32_t w[9];
+    if (a >= lo && a + 36 <= hi) {
+        const uint32_t* q = reinterpret_cast<const uint32_t*>(a);
+        uint32_t w[9];
 #pragma unroll
-    for (int j = 0; j < 9; ++j) {
-        w[j] = 0;
-        const uint8_t* q = a + 4 * j;
-        if (4 * j < (int)skip + valid) {
-            if (q >= lo && q + 4 <= hi) {
-                w[j] = __ldg(reinterpret_cast<const uint32_t*>(q));
-            } else {
+        for (int j = 0; j < 9; ++j) w[j] = __ldg(q + j);
 #pragma unroll
-                for (int b = 0; b < 4; ++b)
-                    if (q + b >= lo && q + b < hi) w[j] |= (uint32_t)__ldg(q + b) << (8 * b);
-            }
+        for (int j = 0; j < 8; ++j) out[j] = __funnelshift_r(w[j], w[j + 1], 8 * skip);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            out[j] = 0;
+#pragma unroll 1
+            for (int b = 0; b < 4; ++b)
+                if (4 * j + b < valid) out[j] |= (uint32_t)__ldg(p + 4 * j + b) << (8 * b);
         }
     }
+    if (valid < 32) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const uint32_t v = __funnelshift_r(w[j], w[j + 1], 8 * skip);
-        const int left = valid - 4 * j;
-        out[j] = left >= 4 ? v : left <= 0 ? 0u : v & ((1u << (8 * left)) - 1u);
+        for (int j = 0; j < 8; ++j) {
+            const int left = valid - 4 * j;
+            out[j] = left >= 4 ? out[j] : left <= 0 ? 0u : out[j] & ((1u << (8 * left)) - 1u);
+        }
     }
 }
 
@@ -217,7 +224,7 @@ w4a4_kernel(const W4A4Args a, const __grid_constant__ CUtensorMap x_map, const _
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = uniform(threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     const uint32_t stages = (uint32_t)a.stages;
     if (threadIdx.x == 0) {
@@ -247,67 +254,81 @@ w4a4_kernel(const W4A4Args a, const __grid_constant__ CUtensorMap x_map, const _
     const uint32_t tmem_sf0 = tmem_base + (uint32_t)(a.acc_bufs * a.tok_cap);      // scale slots behind the accumulators
     const uint32_t slot_cols = 8u * (1u + (uint32_t)a.x_blocks);
 
+    // The producer's and the issuer's loops are run by their whole warp, with votes for the waits' results and one
+    // elected lane around the instructions: TMA and tcgen05 instructions take their operands from uniform registers,
+    // and inside a divergent branch (if (lane == 0) around the loop) every one of them is preceded by a chain of moves
+    // into those -- about 100 cycles per instruction, which alone made a stage take 1 us whatever its size.
     if (warp == 0) {
         // ------------------------------------------------------------ TMA producer
-        if (lane == 0) {
-            int32_t g = 0;
-            QItem it;
-            uint32_t s = 0, phase = 0;
-            bool ok = true;
-            for (int64_t id = blockIdx.x; ok && next_qitem(a, tb, g, id, &it); id += gridDim.x) {
-                const int boxes = (it.tokens + a.xbox - 1) / a.xbox;
-                const uint32_t bytes = (uint32_t)((a.rows_w + boxes * a.xbox) * kQRowBytes);
-                for (int rb = 0; rb < a.k_stages; ++rb) {
-                    ok = mbar_wait_bounded(done + s, phase ^ 1, abort_flag);       // the first round passes at once
-                    if (!ok) break;
+        int32_t g = 0;
+        QItem it;
+        uint32_t s = 0, phase = 0;
+        bool ok = true;
+        for (int64_t id = blockIdx.x; ok && next_qitem(a, tb, g, id, &it); id += gridDim.x) {
+            const int row0 = uniform(it.row0), n0 = uniform(it.n0), eid = uniform(it.eid);
+            const int boxes = (uniform(it.tokens) + a.xbox - 1) / a.xbox;
+            const uint32_t bytes = (uint32_t)((a.rows_w + boxes * a.xbox) * kQRowBytes);
+            for (int rb = 0; rb < a.k_stages; ++rb) {
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(done + s, phase ^ 1, abort_flag));   // the first round passes at once
+                if (!ok) break;
+                if (elect_one()) {
                     uint8_t* st = smem + (size_t)s * tile_bytes;
                     mbar_arrive_expect_tx(full + s, bytes);
-                    tma_load_3d(st, &w_map, rb * kQRowBytes, it.n0, it.eid, full + s);
+                    tma_load_3d(st, &w_map, rb * kQRowBytes, n0, eid, full + s);
                     for (int b = 0; b < boxes; ++b)
-                        tma_load_2d(st + kQWTile + b * a.xbox * kQRowBytes, &x_map, rb * kQRowBytes, it.row0 + b * a.xbox, full + s);
-                    if (++s == stages) { s = 0; phase ^= 1; }
+                        tma_load_2d(st + kQWTile + b * a.xbox * kQRowBytes, &x_map, rb * kQRowBytes, row0 + b * a.xbox, full + s);
                 }
+                if (++s == stages) { s = 0; phase ^= 1; }
             }
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer
-        if (lane == 0) {
-            int32_t g = 0;
-            QItem it;
-            uint32_t s = 0, phase = 0, buf = 0, acc_phase = 0;
-            bool ok = true;
-            for (int64_t id = blockIdx.x; ok && next_qitem(a, tb, g, id, &it); id += gridDim.x) {
-                const uint32_t n_umma = (uint32_t)((it.tokens + 15) & ~15);
-                const uint32_t id0 = mxf4_idesc(n_umma, 0), id2 = mxf4_idesc(n_umma, 2);
-                const int xb = (it.tokens + 127) >> 7;
-                const uint32_t acc = tmem_base + buf * (uint32_t)a.tok_cap;
-                ok = mbar_wait_bounded(acc_empty + buf, acc_phase ^ 1, abort_flag);
+        int32_t g = 0;
+        QItem it;
+        uint32_t s = 0, phase = 0, buf = 0, acc_phase = 0;
+        bool ok = true;
+        const uint32_t tile0 = smem_u32(smem), scale0 = smem_u32(s_scale);
+        const uint32_t half_smem = 512u * (1u + (uint32_t)a.x_blocks), half_cols = 4u * (1u + (uint32_t)a.x_blocks);
+        for (int64_t id = blockIdx.x; ok && next_qitem(a, tb, g, id, &it); id += gridDim.x) {
+            const uint32_t tokens = (uint32_t)uniform(it.tokens);
+            const uint32_t n_umma = (tokens + 15u) & ~15u;
+            const uint32_t id0 = mxf4_idesc(n_umma, 0), id2 = mxf4_idesc(n_umma, 2);
+            const bool two = tokens > 128u;
+            const uint32_t acc = tmem_base + buf * (uint32_t)a.tok_cap;
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(acc_empty + buf, acc_phase ^ 1, abort_flag));
+            if (!ok) break;
+            tc_fence_after();
+            for (int rb = 0; rb < a.k_stages; ++rb) {
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(full + s, phase, abort_flag));
                 if (!ok) break;
                 tc_fence_after();
-                for (int rb = 0; rb < a.k_stages; ++rb) {
-                    ok = mbar_wait_bounded(full + s, phase, abort_flag);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t wt = smem_u32(smem + (size_t)s * tile_bytes), xt = wt + kQWTile;
-                    const uint32_t sc = smem_u32(s_scale + (size_t)s * scale_bytes);
+                if (elect_one()) {
+                    const uint32_t wt = tile0 + s * (uint32_t)tile_bytes;
+                    const uint64_t da = umma_desc(wt, 16, 1024), db = umma_desc(wt + kQWTile, 16, 1024);
+                    const uint64_t dsc = scale_desc(scale0 + s * (uint32_t)scale_bytes);
                     const uint32_t sf = tmem_sf0 + s * slot_cols;
                     // steps of 64 elements that exist (a trailing half step is zero elements)
                     const int steps = (int)min((int64_t)4, (a.K - (int64_t)rb * kQStageK + 63) >> 6);
-                    for (int h = 0; 2 * h < steps; ++h) {
-                        const uint32_t src = sc + (uint32_t)(h * 512 * (1 + a.x_blocks));
-                        const uint32_t sfa = sf + (uint32_t)(h * 4 * (1 + a.x_blocks)), sfb = sfa + 4;
-                        tc_cp_scales(sfa, scale_desc(src));
-                        for (int b = 0; b < xb; ++b) tc_cp_scales(sfb + b * 4, scale_desc(src + 512 * (1 + b)));
-                        for (int j = 2 * h; j < steps && j < 2 * h + 2; ++j)
-                            tc_mma_mxf4(acc, umma_desc(wt + j * 32, 16, 1024), umma_desc(xt + j * 32, 16, 1024),
-                                        (j & 1) ? id2 : id0, sfa, sfb, (rb > 0 || j > 0) ? 1u : 0u);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (2 * h >= steps) break;
+                        const uint64_t src = dsc + (uint64_t)(h * (half_smem >> 4));
+                        const uint32_t sfa = sf + h * half_cols, sfb = sfa + 4;
+                        tc_cp_scales(sfa, src);
+                        tc_cp_scales(sfb, src + (512 >> 4));
+                        if (two) tc_cp_scales(sfb + 4, src + (1024 >> 4));
+#pragma unroll
+                        for (int j = 2 * h; j < 2 * h + 2; ++j) {
+                            if (j >= steps) break;
+                            tc_mma_mxf4(acc, da + 2 * j, db + 2 * j, (j & 1) ? id2 : id0, sfa, sfb, (rb > 0 || j > 0) ? 1u : 0u);
+                        }
                     }
                     tc_commit(done + s);
-                    if (++s == stages) { s = 0; phase ^= 1; }
+                    if (rb + 1 == a.k_stages) tc_commit(acc_full + buf);
                 }
-                if (ok) tc_commit(acc_full + buf);
-                if (++buf == (uint32_t)a.acc_bufs) { buf = 0; acc_phase ^= 1; }
+                if (++s == stages) { s = 0; phase ^= 1; }
             }
+            if (++buf == (uint32_t)a.acc_bufs) { buf = 0; acc_phase ^= 1; }
         }
     } else if (warp < kQEpiWarp0) {
         // ------------------------------------------------------------ scales: global -> registers -> shared memory
@@ -328,10 +349,14 @@ w4a4_kernel(const W4A4Args a, const __grid_constant__ CUtensorMap x_map, const _
         auto fetch = [&]() {                       // span sp of item `it`
             const int valid = (int)min((int64_t)32, kb - (int64_t)sp * 32);
             const int64_t n = (int64_t)it.n0 + t;
-            load_scale_span(a.ws + (int64_t)it.eid * a.ws_se + n * a.ws_sn + sp * 32, (t < a.rows_w && n < a.N) ? valid : 0,
-                            w_lo, w_hi, nxt[0]);
-            load_scale_span(a.xs + ((int64_t)it.row0 + t) * kb + sp * 32, t < it.tokens ? valid : 0, x_lo, x_hi, nxt[1]);
-            load_scale_span(a.xs + ((int64_t)it.row0 + t + 128) * kb + sp * 32, t + 128 < it.tokens ? valid : 0, x_lo, x_hi, nxt[2]);
+#pragma unroll
+            for (int r = 0; r < 3; ++r)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) nxt[r][j] = 0;
+            if (t < a.rows_w && n < a.N)
+                load_scale_span(a.ws + (int64_t)it.eid * a.ws_se + n * a.ws_sn + sp * 32, valid, w_lo, w_hi, nxt[0]);
+            if (t < it.tokens) load_scale_span(a.xs + ((int64_t)it.row0 + t) * kb + sp * 32, valid, x_lo, x_hi, nxt[1]);
+            if (t + 128 < it.tokens) load_scale_span(a.xs + ((int64_t)it.row0 + t + 128) * kb + sp * 32, valid, x_lo, x_hi, nxt[2]);
         };
         if (have) fetch();
         uint32_t s = 0, phase = 0;
