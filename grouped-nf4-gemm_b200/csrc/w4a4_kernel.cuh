@@ -13,9 +13,10 @@
 //               [rows_w x 128 B] and the item's activation rows in boxes of xbox rows
 //   warp 1      MMA issuer (one lane): tcgen05.cp of the stage's scales shared memory -> tensor memory (32 lanes
 //               x 16 bytes, replicated to the four lane quarters), then up to four MMAs of 64 elements
-//   warps 2-5   scales: one thread per weight row and per activation row (two of these from 129 tokens on) takes 32
-//               exponent bytes (1024 elements, four stages) at a time from global memory, a span ahead, and writes the
-//               4-byte words of a stage into the layout tcgen05.cp reads: row r at (r % 32) * 16 + (r / 32) * 4.
+//   warps 2-5   scales, a span of 1024 elements (32 exponent bytes a row, four stages) at a time in a ring of two: one
+//               thread per weight row and per activation row (two of these from 129 tokens on) reads the row's 32 bytes
+//               with two or three 16-byte loads, the loads of all its rows and of the next span in flight while a span is
+//               written as the 4-byte words of 128 elements that tcgen05.cp takes (row r at (r % 32) * 16 + (r / 32) * 4).
 //               Scale rows have any pitch (gpt-oss: 90 bytes), so they cannot come by TMA
 //   warps 6-13  epilogue, two per TMEM lane quarter taking alternate 32-token chunks, as in tensor_fwd_kernel.cuh
 //
@@ -32,7 +33,7 @@ constexpr int kQStageK = 256;                  // contraction elements per stage
 constexpr int kQRowBytes = kQStageK / 2;       // 128 bytes: one swizzle row
 constexpr int kQWTile = 128 * kQRowBytes;      // 16 KiB, whatever rows_w: the MMA reads 128 rows
 constexpr int kQMaxStages = 12;
-constexpr int kQMaxGroups = 512;               // groups per launch (longer lists take several)
+constexpr int kQMaxGroups = 256;               // groups per launch (longer lists take several)
 constexpr int kQScaleWarps = 4, kQEpiWarps = 8;
 constexpr int kQScaleWarp0 = 2, kQEpiWarp0 = kQScaleWarp0 + kQScaleWarps;
 constexpr int kQThreads = (kQEpiWarp0 + kQEpiWarps) * 32;
@@ -60,10 +61,12 @@ struct W4A4Args {
     int32_t x_blocks;           // ceil(tok_cap / 128): 512-byte scale blocks per 128 elements
 };
 
-// scales of a stage: two 128-element halves of [weights 512 B][activations x_blocks * 512 B]
-__host__ __device__ inline int w4a4_scale_bytes(int x_blocks) { return 2 * 512 * (1 + x_blocks); }
-__host__ __device__ inline int w4a4_stage_bytes(int x_bytes, int x_blocks) { return kQWTile + x_bytes + w4a4_scale_bytes(x_blocks); }
-__host__ __device__ inline size_t w4a4_fixed_bytes() { return 1024 /*alignment*/ + kQTableBytes + 512 /*barriers*/; }
+// scales of 128 elements: [weights 512 B][activations x_blocks * 512 B]; eight of these are a span
+__host__ __device__ inline int w4a4_half_bytes(int x_blocks) { return 512 * (1 + x_blocks); }
+__host__ __device__ inline int w4a4_span_bytes(int x_blocks) { return 8 * w4a4_half_bytes(x_blocks); }
+__host__ __device__ inline size_t w4a4_fixed_bytes(int x_blocks) {
+    return 1024 /*alignment*/ + 2 * (size_t)w4a4_span_bytes(x_blocks) + kQTableBytes + 512 /*barriers*/;
+}
 
 __device__ __forceinline__ void tma_load_3d(void* dst_smem, const CUtensorMap* map, int32_t c0, int32_t c1, int32_t c2,
                                             uint64_t* bar) {
@@ -166,34 +169,45 @@ __device__ __forceinline__ void build_qtable(const W4A4Args& a, QGroup* grp, int
     if (t == 0) base[0] = 0;
 }
 
-// Up to 32 scale bytes from p (any alignment) into 8 words, zeros behind the first `valid` (the same for all lanes).
-// [lo, hi) is the scale tensor: aligned words around the bytes are read where they lie inside it (all rows but its
-// first and last), single bytes otherwise.
-__device__ __forceinline__ void load_scale_span(const uint8_t* p, int valid, const uint8_t* lo, const uint8_t* hi, uint32_t* out) {
-    if (valid >= 32 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-        const uint4 v0 = __ldg(reinterpret_cast<const uint4*>(p)), v1 = __ldg(reinterpret_cast<const uint4*>(p) + 1);
-        out[0] = v0.x; out[1] = v0.y; out[2] = v0.z; out[3] = v0.w;
-        out[4] = v1.x; out[5] = v1.y; out[6] = v1.z; out[7] = v1.w;
-        return;
-    }
-    const uint32_t skip = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 3);
-    const uint8_t* a = p - skip;
-    if (a >= lo && a + 36 <= hi) {
-        const uint32_t* q = reinterpret_cast<const uint32_t*>(a);
-        uint32_t w[9];
-#pragma unroll
-        for (int j = 0; j < 9; ++j) w[j] = __ldg(q + j);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) out[j] = __funnelshift_r(w[j], w[j + 1], 8 * skip);
+// Up to 32 scale bytes from p (any alignment): the aligned 16-byte pieces they lie in go into raw, their place in them
+// into *at; nothing is computed from the loads here, so that several rows' can be in flight.  Where the pieces would reach
+// over an end of the scale tensor [lo, hi) (its first and last rows) the bytes are read one by one.
+__device__ __forceinline__ void fetch_scale_row(const uint8_t* p, int valid, const uint8_t* lo, const uint8_t* hi, uint32_t* raw, uint32_t* at) {
+    const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 15);
+    const uint4* q = reinterpret_cast<const uint4*>(p - off);
+    *at = off;
+    if (off == 0 && valid >= 32) {
+        const uint4 v0 = __ldg(q), v1 = __ldg(q + 1);
+        raw[0] = v0.x; raw[1] = v0.y; raw[2] = v0.z; raw[3] = v0.w;
+        raw[4] = v1.x; raw[5] = v1.y; raw[6] = v1.z; raw[7] = v1.w;
+    } else if (p - off >= lo && p - off + 48 <= hi) {
+        const uint4 v0 = __ldg(q), v1 = __ldg(q + 1), v2 = __ldg(q + 2);
+        raw[0] = v0.x; raw[1] = v0.y; raw[2] = v0.z; raw[3] = v0.w;
+        raw[4] = v1.x; raw[5] = v1.y; raw[6] = v1.z; raw[7] = v1.w;
+        raw[8] = v2.x; raw[9] = v2.y; raw[10] = v2.z; raw[11] = v2.w;
     } else {
+        *at = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            out[j] = 0;
-#pragma unroll 1
+            raw[j] = 0;
+#pragma unroll
             for (int b = 0; b < 4; ++b)
-                if (4 * j + b < valid) out[j] |= (uint32_t)__ldg(p + 4 * j + b) << (8 * b);
+                if (4 * j + b < valid) raw[j] |= (uint32_t)__ldg(p + 4 * j + b) << (8 * b);
         }
     }
+}
+// The 32 bytes at offset `at` (0..15) of the 48 in raw as 8 words, zeros behind the first `valid`.
+__device__ __forceinline__ void align_scale_row(const uint32_t* raw, uint32_t at, int valid, uint32_t* out) {
+    uint32_t w[9];
+    const bool by2 = at & 8, by1 = at & 4;
+#pragma unroll
+    for (int j = 0; j < 9; ++j) {
+        const uint32_t v0 = by2 ? raw[j + 2] : raw[j];
+        const uint32_t v1 = j + 3 < 12 ? (by2 ? raw[j + 3] : raw[j + 1]) : 0u;
+        w[j] = by1 ? v1 : v0;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) out[j] = __funnelshift_r(w[j], w[j + 1], 8 * (at & 3));
     if (valid < 32) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -207,21 +221,23 @@ __global__ void __launch_bounds__(kQThreads, 1)
 w4a4_kernel(const W4A4Args a, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    // tiles of all stages (each a multiple of 1024 bytes), then the scales of all stages, then the tables
+    // tiles of all stages (each a multiple of 1024 bytes), then two spans of scales, then the tables
     const int tile_bytes = kQWTile + a.x_bytes;
-    const int scale_bytes = w4a4_scale_bytes(a.x_blocks);
+    const int half_bytes = w4a4_half_bytes(a.x_blocks), span_bytes = 8 * half_bytes;
     uint8_t* s_scale = smem + (size_t)a.stages * tile_bytes;
-    uint8_t* grp_raw = s_scale + (size_t)a.stages * scale_bytes;
+    uint8_t* grp_raw = s_scale + 2 * (size_t)span_bytes;
     QGroup* s_grp = reinterpret_cast<QGroup*>(grp_raw);
     int64_t* s_base = reinterpret_cast<int64_t*>(grp_raw + kQMaxGroups * 16);
     int64_t* s_wtot = s_base + kQMaxGroups + 1;
-    // full[s]: tiles landed (TMA bytes + the producer's arrival) and scales written (one arrival per scale warp);
-    // done[s]: the stage's copies and MMAs have completed, shared memory and tensor-memory scale slot may be refilled
+    // full[s]: tiles landed (TMA bytes + the producer's arrival); done[s]: the stage's copies and MMAs have completed,
+    // its shared memory and its tensor-memory scale slot may be refilled; sc_full / sc_done: the same for a span of scales
     uint64_t* full = reinterpret_cast<uint64_t*>(grp_raw + ((kQTableBytes + 15) & ~15));
     uint64_t* done = full + kQMaxStages;
     uint64_t* acc_full = done + kQMaxStages;
     uint64_t* acc_empty = acc_full + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    uint64_t* sc_full = acc_empty + 2;
+    uint64_t* sc_done = sc_full + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sc_done + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = uniform(threadIdx.x >> 5);
@@ -229,12 +245,14 @@ w4a4_kernel(const W4A4Args a, const __grid_constant__ CUtensorMap x_map, const _
     const uint32_t stages = (uint32_t)a.stages;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kQMaxStages; ++s) {
-            mbar_init(full + s, 1 + kQScaleWarps);
+            mbar_init(full + s, 1);
             mbar_init(done + s, 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full + b, 1);
             mbar_init(acc_empty + b, kQEpiWarps);
+            mbar_init(sc_full + b, kQScaleWarps);
+            mbar_init(sc_done + b, 1);
         }
         *abort_flag = 0;
         fence_barrier_init();
@@ -285,10 +303,10 @@ w4a4_kernel(const W4A4Args a, const __grid_constant__ CUtensorMap x_map, const _
         // ------------------------------------------------------------ MMA issuer
         int32_t g = 0;
         QItem it;
-        uint32_t s = 0, phase = 0, buf = 0, acc_phase = 0;
+        uint32_t s = 0, phase = 0, buf = 0, acc_phase = 0, sp = 0, sp_phase = 0;
         bool ok = true;
         const uint32_t tile0 = smem_u32(smem), scale0 = smem_u32(s_scale);
-        const uint32_t half_smem = 512u * (1u + (uint32_t)a.x_blocks), half_cols = 4u * (1u + (uint32_t)a.x_blocks);
+        const uint32_t half_cols = 4u * (1u + (uint32_t)a.x_blocks);
         for (int64_t id = blockIdx.x; ok && next_qitem(a, tb, g, id, &it); id += gridDim.x) {
             const uint32_t tokens = (uint32_t)uniform(it.tokens);
             const uint32_t n_umma = (tokens + 15u) & ~15u;
@@ -299,20 +317,21 @@ w4a4_kernel(const W4A4Args a, const __grid_constant__ CUtensorMap x_map, const _
             if (!ok) break;
             tc_fence_after();
             for (int rb = 0; rb < a.k_stages; ++rb) {
-                ok = __all_sync(0xffffffffu, mbar_wait_bounded(full + s, phase, abort_flag));
+                if ((rb & 3) == 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(sc_full + sp, sp_phase, abort_flag));
+                ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(full + s, phase, abort_flag));
                 if (!ok) break;
                 tc_fence_after();
                 if (elect_one()) {
                     const uint32_t wt = tile0 + s * (uint32_t)tile_bytes;
                     const uint64_t da = umma_desc(wt, 16, 1024), db = umma_desc(wt + kQWTile, 16, 1024);
-                    const uint64_t dsc = scale_desc(scale0 + s * (uint32_t)scale_bytes);
+                    const uint64_t dsc = scale_desc(scale0 + sp * (uint32_t)span_bytes + (uint32_t)((rb & 3) * 2 * half_bytes));
                     const uint32_t sf = tmem_sf0 + s * slot_cols;
                     // steps of 64 elements that exist (a trailing half step is zero elements)
                     const int steps = (int)min((int64_t)4, (a.K - (int64_t)rb * kQStageK + 63) >> 6);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         if (2 * h >= steps) break;
-                        const uint64_t src = dsc + (uint64_t)(h * (half_smem >> 4));
+                        const uint64_t src = dsc + (uint64_t)(h * (half_bytes >> 4));
                         const uint32_t sfa = sf + h * half_cols, sfb = sfa + 4;
                         tc_cp_scales(sfa, src);
                         tc_cp_scales(sfb, src + (512 >> 4));
@@ -324,74 +343,76 @@ w4a4_kernel(const W4A4Args a, const __grid_constant__ CUtensorMap x_map, const _
                         }
                     }
                     tc_commit(done + s);
+                    if ((rb & 3) == 3 || rb + 1 == a.k_stages) tc_commit(sc_done + sp);
                     if (rb + 1 == a.k_stages) tc_commit(acc_full + buf);
                 }
                 if (++s == stages) { s = 0; phase ^= 1; }
+                if ((rb & 3) == 3 || rb + 1 == a.k_stages) { sp ^= 1; sp_phase ^= sp ^ 1; }
             }
             if (++buf == (uint32_t)a.acc_bufs) { buf = 0; acc_phase ^= 1; }
         }
     } else if (warp < kQEpiWarp0) {
         // ------------------------------------------------------------ scales: global -> registers -> shared memory
-        const int t = threadIdx.x - kQScaleWarp0 * 32;
+        const int r = threadIdx.x - kQScaleWarp0 * 32;      // this thread's weight row and activation rows r, r + 128
         const int64_t kb = a.K / 32;
-        const uint8_t* w_lo = a.ws;
         const uint8_t* w_hi = a.ws + (int64_t)(a.E - 1) * a.ws_se + (a.N - 1) * a.ws_sn + kb;
-        const uint8_t* x_lo = a.xs;
         const uint8_t* x_hi = a.xs + a.T * kb;
         const int spans = (a.k_stages + 3) >> 2;
-        const uint32_t at = (uint32_t)((t & 31) * 16 + (t >> 5) * 4);
         int32_t g = 0;
         QItem it;
         int64_t id = blockIdx.x;
         bool have = next_qitem(a, tb, g, id, &it);
         int sp = 0;
-        uint32_t nxt[3][8];
-        auto fetch = [&]() {                       // span sp of item `it`
+        uint32_t raw[3][12], at[3];
+        bool live[3];                                       // 0: weights, 1, 2: activations
+#pragma unroll
+        for (int op = 0; op < 3; ++op) {
+            at[op] = 0;
+#pragma unroll
+            for (int j = 0; j < 12; ++j) raw[op][j] = 0;
+        }
+        auto fetch = [&]() {                                // span sp of item `it`
             const int valid = (int)min((int64_t)32, kb - (int64_t)sp * 32);
-            const int64_t n = (int64_t)it.n0 + t;
-#pragma unroll
-            for (int r = 0; r < 3; ++r)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) nxt[r][j] = 0;
-            if (t < a.rows_w && n < a.N)
-                load_scale_span(a.ws + (int64_t)it.eid * a.ws_se + n * a.ws_sn + sp * 32, valid, w_lo, w_hi, nxt[0]);
-            if (t < it.tokens) load_scale_span(a.xs + ((int64_t)it.row0 + t) * kb + sp * 32, valid, x_lo, x_hi, nxt[1]);
-            if (t + 128 < it.tokens) load_scale_span(a.xs + ((int64_t)it.row0 + t + 128) * kb + sp * 32, valid, x_lo, x_hi, nxt[2]);
+            live[0] = r < a.rows_w && it.n0 + r < a.N;
+            live[1] = r < it.tokens;
+            live[2] = r + 128 < it.tokens;
+            if (live[0])
+                fetch_scale_row(a.ws + (int64_t)it.eid * a.ws_se + (int64_t)(it.n0 + r) * a.ws_sn + sp * 32, valid, a.ws, w_hi, raw[0], &at[0]);
+            if (live[1]) fetch_scale_row(a.xs + ((int64_t)it.row0 + r) * kb + sp * 32, valid, a.xs, x_hi, raw[1], &at[1]);
+            if (live[2]) fetch_scale_row(a.xs + ((int64_t)it.row0 + r + 128) * kb + sp * 32, valid, a.xs, x_hi, raw[2], &at[2]);
         };
         if (have) fetch();
-        uint32_t s = 0, phase = 0;
+        uint32_t slot = 0, phase = 0;
         bool ok = true;
         while (have && ok) {
-            uint32_t cur[3][8];
+            const int valid = (int)min((int64_t)32, kb - (int64_t)sp * 32);
+            uint32_t out[3][8];
+            bool put[3];
 #pragma unroll
-            for (int r = 0; r < 3; ++r)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) cur[r][j] = nxt[r][j];
-            const int n_st = min(4, a.k_stages - sp * 4);
+            for (int op = 0; op < 3; ++op) {
+                put[op] = live[op];                         // stale bytes of other rows belong to accumulator entries
+                align_scale_row(raw[op], at[op], valid, out[op]);      // that nobody reads
+            }
             if (++sp == spans) {
                 sp = 0;
                 id += gridDim.x;
                 have = next_qitem(a, tb, g, id, &it);
             }
             if (have) fetch();
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(sc_done + slot, phase ^ 1, abort_flag));
+            if (!ok) break;
+            uint8_t* dst = s_scale + slot * span_bytes + (r & 31) * 16 + (r >> 5) * 4;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                if (q >= n_st || !ok) continue;
-                ok = __all_sync(0xffffffffu, mbar_wait_bounded(done + s, phase ^ 1, abort_flag));
-                if (!ok) continue;
-                uint8_t* dst = s_scale + (size_t)s * scale_bytes + at;
+            for (int op = 0; op < 3; ++op) {
+                if (!put[op]) continue;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint8_t* d = dst + h * 512 * (1 + a.x_blocks);
-                    *reinterpret_cast<uint32_t*>(d) = cur[0][2 * q + h];
-                    *reinterpret_cast<uint32_t*>(d + 512) = cur[1][2 * q + h];
-                    if (a.x_blocks == 2) *reinterpret_cast<uint32_t*>(d + 1024) = cur[2][2 * q + h];
-                }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(full + s);
-                if (++s == stages) { s = 0; phase ^= 1; }
+                for (int j = 0; j < 8; ++j) *reinterpret_cast<uint32_t*>(dst + j * half_bytes + op * 512) = out[op][j];
             }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sc_full + slot);
+            slot ^= 1;
+            phase ^= slot ^ 1;
         }
     } else {
         // ------------------------------------------------------------ epilogue
@@ -497,11 +518,11 @@ static inline W4A4Plan w4a4_plan(int64_t T, int32_t G, int64_t N, int32_t max_ro
             if (cost < best) { best = cost; p.rows_w = r; }
         }
     }
-    const size_t room = (size_t)smem_optin - w4a4_fixed_bytes();
-    p.stages = (int)(room / (size_t)w4a4_stage_bytes(p.x_bytes, p.x_blocks));
+    const size_t room = (size_t)smem_optin - w4a4_fixed_bytes(p.x_blocks);
+    p.stages = (int)(room / (size_t)(kQWTile + p.x_bytes));
     if (p.stages > kQMaxStages) p.stages = kQMaxStages;
     p.acc_bufs = 2 * p.tok_cap + p.stages * 8 * (1 + p.x_blocks) <= kQTmemCols ? 2 : 1;
-    p.smem = w4a4_fixed_bytes() + (size_t)p.stages * w4a4_stage_bytes(p.x_bytes, p.x_blocks);
+    p.smem = w4a4_fixed_bytes(p.x_blocks) + (size_t)p.stages * (kQWTile + p.x_bytes);
     return p;
 }
 

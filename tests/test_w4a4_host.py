@@ -65,8 +65,9 @@ def test_tile_plan_fits(T, G, N, max_rows):
         box = 16 if cap <= 16 else 32 if cap <= 64 else 64
         x_rows = (cap + box - 1) // box * box
         blocks = (cap + 127) // 128
-        stage = 16384 + x_rows * 128 + 1024 * (1 + blocks)
-        fixed = 1024 + 512 * 16 + 513 * 8 + 16 * 8 + 8 + 512
+        stage = 16384 + x_rows * 128
+        span = 8 * 512 * (1 + blocks)
+        fixed = 1024 + 2 * span + 256 * 16 + 257 * 8 + 16 * 8 + 8 + 512
         stages = min(12, (232448 - fixed) // stage)
         assert stages >= 4 and fixed + stages * stage <= 232448
         slots = stages * 8 * (1 + blocks)
