@@ -111,7 +111,9 @@ int gnf4b_gemm_grouped_w4a4(const uint8_t* x_blocks, const uint8_t* x_scales, in
     EncodeTiledFn enc = encode_tiled_fn();
     if (!enc) return GNF4B_EUNSUPPORTED;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
-    const W4A4Plan p = w4a4_plan(T, G, N, max_rows, di.sm_count, di.smem_optin);
+    const W4A4Plan p = w4a4_plan(T, G, N, K, max_rows, di.sm_count, di.smem_optin);
+    // items are numbered in 31 bits (a group adds at most one chunk beyond its share)
+    if ((ceil_div(T, 16) + G) * ceil_div(N, p.rows_w) > INT32_MAX) return GNF4B_ETOOBIG;
     W4A4Args a;
     a.xs = x_scales;
     a.ws = S;

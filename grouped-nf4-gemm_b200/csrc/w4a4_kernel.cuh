@@ -8,17 +8,17 @@
 // zero element times any finite scale is zero, so ragged ends need no mask: TMA fills what lies outside the tensors
 // with zero bytes.  An exponent byte of 255 is NaN, as the OCP format has it.
 //
-// Roles (448 threads, one CTA per SM, persistent):
+// Roles (512 threads, one CTA per SM, persistent):
 //   warp 0      TMA producer: per stage of 256 contraction elements (128 bytes a row, 128-byte swizzle) the weight tile
 //               [rows_w x 128 B] and the item's activation rows in boxes of xbox rows
 //   warp 1      MMA issuer (one lane): tcgen05.cp of the stage's scales shared memory -> tensor memory (32 lanes
 //               x 16 bytes, replicated to the four lane quarters), then up to four MMAs of 64 elements
-//   warps 2-5   scales, a span of 1024 elements (32 exponent bytes a row, four stages) at a time in a ring of two: one
-//               thread per weight row and per activation row (two of these from 129 tokens on) reads the row's 32 bytes
-//               with two or three 16-byte loads, the loads of all its rows and of the next span in flight while a span is
-//               written as the 4-byte words of 128 elements that tcgen05.cp takes (row r at (r % 32) * 16 + (r / 32) * 4).
-//               Scale rows have any pitch (gpt-oss: 90 bytes), so they cannot come by TMA
-//   warps 6-13  epilogue, two per TMEM lane quarter taking alternate 32-token chunks, as in tensor_fwd_kernel.cuh
+//   warps 2-7   scales, a span of 1024 elements (32 exponent bytes a row, four stages) at a time in a ring of two: every
+//               thread has two of the 128 + 256 rows and reads a row's 32 bytes with two or three 16-byte loads, those of
+//               the next span in flight while a span is written as the 4-byte words of 128 elements that tcgen05.cp
+//               takes (row r at (r % 32) * 16 + (r / 32) * 4).  Scale rows have any pitch (gpt-oss: 90 bytes), so they
+//               cannot come by TMA
+//   warps 8-15  epilogue, two per TMEM lane quarter taking alternate 32-token chunks, as in tensor_fwd_kernel.cuh
 //
 // Work item = (group, balanced chunk of <= tok_cap rows, rows_w weight rows), weight tile fastest.  With few rows per
 // group the kernel streams weights and rows_w < 128 evens out the items over the SMs (the MMA still multiplies 128
@@ -34,11 +34,12 @@ constexpr int kQRowBytes = kQStageK / 2;       // 128 bytes: one swizzle row
 constexpr int kQWTile = 128 * kQRowBytes;      // 16 KiB, whatever rows_w: the MMA reads 128 rows
 constexpr int kQMaxStages = 12;
 constexpr int kQMaxGroups = 256;               // groups per launch (longer lists take several)
-constexpr int kQScaleWarps = 4, kQEpiWarps = 8;
+constexpr int kQScaleWarps = 6, kQEpiWarps = 8;      // 16 warps in all: 128 registers a thread
+constexpr int kQEpiChunks = 4;                 // 32-token chunks per epilogue warp, at most
 constexpr int kQScaleWarp0 = 2, kQEpiWarp0 = kQScaleWarp0 + kQScaleWarps;
 constexpr int kQThreads = (kQEpiWarp0 + kQEpiWarps) * 32;
 constexpr int kQTmemCols = 512;
-constexpr int kQTableBytes = kQMaxGroups * 16 + (kQMaxGroups + 1) * 8 + 16 * 8 + 8;
+constexpr int kQTableBytes = kQMaxGroups * 16 + (kQMaxGroups + 1) * 4 + 16 * 4 + 4;
 
 struct W4A4Args {
     const uint8_t* xs;          // activation scales, rows of K / 32 bytes
@@ -87,6 +88,15 @@ __device__ __forceinline__ void tc_mma_mxf4(uint32_t d_tmem, uint64_t a_desc, ui
 __device__ __forceinline__ void tc_cp_scales(uint32_t taddr, uint64_t s_desc) {
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(s_desc) : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
 // descriptor of that source: no swizzle, 8-row groups of 128 bytes one after the other
 __device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
     return (uint64_t)((smem_addr >> 4) & 0x3fffu) | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
@@ -110,31 +120,31 @@ struct QGroup {
 };
 struct QTable {
     const QGroup* grp;       // [G]
-    const int64_t* base;     // [G + 1] items before group g
+    const uint32_t* base;    // [G + 1] items before group g (the host sees to it that all items fit 31 bits)
 };
 struct QItem {
     int32_t row0, tokens, eid, n0;
 };
 
-__device__ __forceinline__ bool next_qitem(const W4A4Args& a, const QTable& tb, int32_t& g, int64_t id, QItem* it) {
+__device__ __forceinline__ bool next_qitem(const W4A4Args& a, const QTable& tb, int32_t& g, uint32_t id, QItem* it) {
     while (g < a.G && id >= tb.base[g + 1]) ++g;
     if (g >= a.G) return false;
     const QGroup gr = tb.grp[g];
-    const int64_t local = id - tb.base[g];
-    const int32_t mc = (int32_t)(local / a.n_tiles);
-    it->row0 = gr.row0 + mc * gr.chunk_rows;
+    const uint32_t local = id - tb.base[g];
+    const uint32_t mc = local / (uint32_t)a.n_tiles;
+    it->row0 = gr.row0 + (int32_t)mc * gr.chunk_rows;
     it->tokens = min(gr.chunk_rows, gr.row0 + gr.rows - it->row0);
     it->eid = gr.eid;
-    it->n0 = (int32_t)(local - (int64_t)mc * a.n_tiles) * a.rows_w;
+    it->n0 = (int32_t)(local - mc * (uint32_t)a.n_tiles) * a.rows_w;
     return true;
 }
 
 // Thread t takes groups 2t and 2t + 1: item counts, then a block-wide inclusive scan.  Groups with a bad expert id or
 // bad offsets are flagged in the status word and get no items.
-__device__ __forceinline__ void build_qtable(const W4A4Args& a, QGroup* grp, int64_t* base, int64_t* warp_tot) {
+__device__ __forceinline__ void build_qtable(const W4A4Args& a, QGroup* grp, uint32_t* base, uint32_t* warp_tot) {
     static_assert(kQThreads * 2 >= kQMaxGroups, "one thread per two groups");
     const int t = threadIdx.x, lane = t & 31, w = t >> 5;
-    int64_t items[2] = {0, 0};
+    uint32_t items[2] = {0, 0};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int g = 2 * t + h;
@@ -153,12 +163,12 @@ __device__ __forceinline__ void build_qtable(const W4A4Args& a, QGroup* grp, int
         // equal chunks, a multiple of 16 rows each
         gr.chunk_rows = chunks ? (((gr.rows + chunks - 1) / chunks + 15) & ~15) : 16;
         grp[g] = gr;
-        items[h] = (int64_t)((gr.rows + gr.chunk_rows - 1) / gr.chunk_rows) * a.n_tiles;
+        items[h] = (uint32_t)(((int64_t)gr.rows + gr.chunk_rows - 1) / gr.chunk_rows) * (uint32_t)a.n_tiles;
     }
-    int64_t incl = items[0] + items[1];
+    uint32_t incl = items[0] + items[1];
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, incl, d);
+        const uint32_t up = __shfl_up_sync(0xffffffffu, incl, d);
         if (lane >= d) incl += up;
     }
     if (lane == 31) warp_tot[w] = incl;
@@ -169,6 +179,13 @@ __device__ __forceinline__ void build_qtable(const W4A4Args& a, QGroup* grp, int
     if (t == 0) base[0] = 0;
 }
 
+// 16 bytes; on an L2 miss the 256 bytes around them are fetched, which hold the row's next spans and its neighbours
+__device__ __forceinline__ uint4 load_scale16(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
 // Up to 32 scale bytes from p (any alignment): the aligned 16-byte pieces they lie in go into raw, their place in them
 // into *at; nothing is computed from the loads here, so that several rows' can be in flight.  Where the pieces would reach
 // over an end of the scale tensor [lo, hi) (its first and last rows) the bytes are read one by one.
@@ -177,11 +194,11 @@ __device__ __forceinline__ void fetch_scale_row(const uint8_t* p, int valid, con
     const uint4* q = reinterpret_cast<const uint4*>(p - off);
     *at = off;
     if (off == 0 && valid >= 32) {
-        const uint4 v0 = __ldg(q), v1 = __ldg(q + 1);
+        const uint4 v0 = load_scale16(q), v1 = load_scale16(q + 1);
         raw[0] = v0.x; raw[1] = v0.y; raw[2] = v0.z; raw[3] = v0.w;
         raw[4] = v1.x; raw[5] = v1.y; raw[6] = v1.z; raw[7] = v1.w;
     } else if (p - off >= lo && p - off + 48 <= hi) {
-        const uint4 v0 = __ldg(q), v1 = __ldg(q + 1), v2 = __ldg(q + 2);
+        const uint4 v0 = load_scale16(q), v1 = load_scale16(q + 1), v2 = load_scale16(q + 2);
         raw[0] = v0.x; raw[1] = v0.y; raw[2] = v0.z; raw[3] = v0.w;
         raw[4] = v1.x; raw[5] = v1.y; raw[6] = v1.z; raw[7] = v1.w;
         raw[8] = v2.x; raw[9] = v2.y; raw[10] = v2.z; raw[11] = v2.w;
@@ -218,7 +235,7 @@ __device__ __forceinline__ void align_scale_row(const uint32_t* raw, uint32_t at
 }
 
 __global__ void __launch_bounds__(kQThreads, 1)
-w4a4_kernel(const W4A4Args a, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map) {
+w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     // tiles of all stages (each a multiple of 1024 bytes), then two spans of scales, then the tables
@@ -227,8 +244,8 @@ w4a4_kernel(const W4A4Args a, const __grid_constant__ CUtensorMap x_map, const _
     uint8_t* s_scale = smem + (size_t)a.stages * tile_bytes;
     uint8_t* grp_raw = s_scale + 2 * (size_t)span_bytes;
     QGroup* s_grp = reinterpret_cast<QGroup*>(grp_raw);
-    int64_t* s_base = reinterpret_cast<int64_t*>(grp_raw + kQMaxGroups * 16);
-    int64_t* s_wtot = s_base + kQMaxGroups + 1;
+    uint32_t* s_base = reinterpret_cast<uint32_t*>(grp_raw + kQMaxGroups * 16);
+    uint32_t* s_wtot = s_base + kQMaxGroups + 1;
     // full[s]: tiles landed (TMA bytes + the producer's arrival); done[s]: the stage's copies and MMAs have completed,
     // its shared memory and its tensor-memory scale slot may be refilled; sc_full / sc_done: the same for a span of scales
     uint64_t* full = reinterpret_cast<uint64_t*>(grp_raw + ((kQTableBytes + 15) & ~15));
@@ -272,20 +289,20 @@ w4a4_kernel(const W4A4Args a, const __grid_constant__ CUtensorMap x_map, const _
     const uint32_t tmem_sf0 = tmem_base + (uint32_t)(a.acc_bufs * a.tok_cap);      // scale slots behind the accumulators
     const uint32_t slot_cols = 8u * (1u + (uint32_t)a.x_blocks);
 
-    // The producer's and the issuer's loops are run by their whole warp, with votes for the waits' results and one
-    // elected lane around the instructions: TMA and tcgen05 instructions take their operands from uniform registers,
-    // and inside a divergent branch (if (lane == 0) around the loop) every one of them is preceded by a chain of moves
-    // into those -- about 100 cycles per instruction, which alone made a stage take 1 us whatever its size.
+    // The producer's and the issuer's loops are run by their whole warp, every loop condition a vote, with one elected
+    // lane around the instructions: TMA and tcgen05 instructions take their operands from uniform registers, and in
+    // control flow that the compiler cannot see to be the same for all lanes every one of them is preceded by a chain of
+    // moves into those -- about 100 cycles per instruction, which alone made a stage take 1 us whatever its size.
     if (warp == 0) {
         // ------------------------------------------------------------ TMA producer
         int32_t g = 0;
         QItem it;
-        uint32_t s = 0, phase = 0;
-        bool ok = true;
-        for (int64_t id = blockIdx.x; ok && next_qitem(a, tb, g, id, &it); id += gridDim.x) {
+        uint32_t s = 0, phase = 0, id = blockIdx.x;
+        while (__all_sync(0xffffffffu, next_qitem(a, tb, g, id, &it))) {
             const int row0 = uniform(it.row0), n0 = uniform(it.n0), eid = uniform(it.eid);
             const int boxes = (uniform(it.tokens) + a.xbox - 1) / a.xbox;
             const uint32_t bytes = (uint32_t)((a.rows_w + boxes * a.xbox) * kQRowBytes);
+            bool ok = true;
             for (int rb = 0; rb < a.k_stages; ++rb) {
                 ok = __all_sync(0xffffffffu, mbar_wait_bounded(done + s, phase ^ 1, abort_flag));   // the first round passes at once
                 if (!ok) break;
@@ -298,115 +315,117 @@ w4a4_kernel(const W4A4Args a, const __grid_constant__ CUtensorMap x_map, const _
                 }
                 if (++s == stages) { s = 0; phase ^= 1; }
             }
+            if (!ok) break;
+            id += gridDim.x;
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer
         int32_t g = 0;
         QItem it;
-        uint32_t s = 0, phase = 0, buf = 0, acc_phase = 0, sp = 0, sp_phase = 0;
-        bool ok = true;
-        const uint32_t tile0 = smem_u32(smem), scale0 = smem_u32(s_scale);
+        uint32_t s = 0, phase = 0, buf = 0, acc_phase = 0, sp = 0, sp_phase = 0, id = blockIdx.x;
         const uint32_t half_cols = 4u * (1u + (uint32_t)a.x_blocks);
-        for (int64_t id = blockIdx.x; ok && next_qitem(a, tb, g, id, &it); id += gridDim.x) {
+        const uint64_t w_desc0 = umma_desc(smem_u32(smem), 16, 1024), sc_desc0 = scale_desc(smem_u32(s_scale));
+        const uint32_t tile_step = (uint32_t)tile_bytes >> 4, half_step = (uint32_t)half_bytes >> 4, span_step = (uint32_t)span_bytes >> 4;
+        const int tail = (int)((a.K - (int64_t)(a.k_stages - 1) * kQStageK + 63) >> 6);   // 64-element steps of the last stage
+        while (__all_sync(0xffffffffu, next_qitem(a, tb, g, id, &it))) {
             const uint32_t tokens = (uint32_t)uniform(it.tokens);
             const uint32_t n_umma = (tokens + 15u) & ~15u;
             const uint32_t id0 = mxf4_idesc(n_umma, 0), id2 = mxf4_idesc(n_umma, 2);
             const bool two = tokens > 128u;
             const uint32_t acc = tmem_base + buf * (uint32_t)a.tok_cap;
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(acc_empty + buf, acc_phase ^ 1, abort_flag));
+            bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(acc_empty + buf, acc_phase ^ 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
             for (int rb = 0; rb < a.k_stages; ++rb) {
                 if ((rb & 3) == 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(sc_full + sp, sp_phase, abort_flag));
-                ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(full + s, phase, abort_flag));
+                ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(full + s, phase, abort_flag));
                 if (!ok) break;
                 tc_fence_after();
+                const bool last = rb + 1 == a.k_stages;
+                const bool span_end = last || (rb & 3) == 3;
+                const int steps = last ? tail : 4;          // steps that exist (a trailing half step is zero elements)
+                const uint64_t da = w_desc0 + s * tile_step, db = da + (kQWTile >> 4);
+                const uint64_t src = sc_desc0 + sp * span_step + (uint32_t)(rb & 3) * (2 * half_step);
+                const uint32_t sf = tmem_sf0 + s * slot_cols, sf1 = sf + half_cols;
                 if (elect_one()) {
-                    const uint32_t wt = tile0 + s * (uint32_t)tile_bytes;
-                    const uint64_t da = umma_desc(wt, 16, 1024), db = umma_desc(wt + kQWTile, 16, 1024);
-                    const uint64_t dsc = scale_desc(scale0 + sp * (uint32_t)span_bytes + (uint32_t)((rb & 3) * 2 * half_bytes));
-                    const uint32_t sf = tmem_sf0 + s * slot_cols;
-                    // steps of 64 elements that exist (a trailing half step is zero elements)
-                    const int steps = (int)min((int64_t)4, (a.K - (int64_t)rb * kQStageK + 63) >> 6);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (2 * h >= steps) break;
-                        const uint64_t src = dsc + (uint64_t)(h * (half_bytes >> 4));
-                        const uint32_t sfa = sf + h * half_cols, sfb = sfa + 4;
-                        tc_cp_scales(sfa, src);
-                        tc_cp_scales(sfb, src + (512 >> 4));
-                        if (two) tc_cp_scales(sfb + 4, src + (1024 >> 4));
-#pragma unroll
-                        for (int j = 2 * h; j < 2 * h + 2; ++j) {
-                            if (j >= steps) break;
-                            tc_mma_mxf4(acc, da + 2 * j, db + 2 * j, (j & 1) ? id2 : id0, sfa, sfb, (rb > 0 || j > 0) ? 1u : 0u);
-                        }
+                    tc_cp_scales(sf, src);
+                    tc_cp_scales(sf + 4, src + (512 >> 4));
+                    if (two) tc_cp_scales(sf + 8, src + (1024 >> 4));
+                    tc_mma_mxf4(acc, da, db, id0, sf, sf + 4, rb > 0 ? 1u : 0u);
+                    if (steps > 1) tc_mma_mxf4(acc, da + 2, db + 2, id2, sf, sf + 4, 1u);
+                    if (steps > 2) {
+                        tc_cp_scales(sf1, src + half_step);
+                        tc_cp_scales(sf1 + 4, src + half_step + (512 >> 4));
+                        if (two) tc_cp_scales(sf1 + 8, src + half_step + (1024 >> 4));
+                        tc_mma_mxf4(acc, da + 4, db + 4, id0, sf1, sf1 + 4, 1u);
+                        if (steps > 3) tc_mma_mxf4(acc, da + 6, db + 6, id2, sf1, sf1 + 4, 1u);
                     }
                     tc_commit(done + s);
-                    if ((rb & 3) == 3 || rb + 1 == a.k_stages) tc_commit(sc_done + sp);
-                    if (rb + 1 == a.k_stages) tc_commit(acc_full + buf);
+                    if (span_end) tc_commit(sc_done + sp);
+                    if (last) tc_commit(acc_full + buf);
                 }
                 if (++s == stages) { s = 0; phase ^= 1; }
-                if ((rb & 3) == 3 || rb + 1 == a.k_stages) { sp ^= 1; sp_phase ^= sp ^ 1; }
+                if (span_end) { sp ^= 1; sp_phase ^= sp ^ 1; }
             }
+            if (!ok) break;
             if (++buf == (uint32_t)a.acc_bufs) { buf = 0; acc_phase ^= 1; }
+            id += gridDim.x;
         }
     } else if (warp < kQEpiWarp0) {
         // ------------------------------------------------------------ scales: global -> registers -> shared memory
-        const int r = threadIdx.x - kQScaleWarp0 * 32;      // this thread's weight row and activation rows r, r + 128
+        // rows 0..127 are the weight tile's, 128.. the activations'; this thread has rows u and u + 192
+        constexpr int kRows = kQScaleWarps * 32;
+        static_assert(2 * kRows == 128 + 256, "two rows per thread");
+        const int u = threadIdx.x - kQScaleWarp0 * 32;
         const int64_t kb = a.K / 32;
         const uint8_t* w_hi = a.ws + (int64_t)(a.E - 1) * a.ws_se + (a.N - 1) * a.ws_sn + kb;
         const uint8_t* x_hi = a.xs + a.T * kb;
         const int spans = (a.k_stages + 3) >> 2;
         int32_t g = 0;
         QItem it;
-        int64_t id = blockIdx.x;
+        uint32_t id = blockIdx.x;
         bool have = next_qitem(a, tb, g, id, &it);
         int sp = 0;
-        uint32_t raw[3][12], at[3];
-        bool live[3];                                       // 0: weights, 1, 2: activations
-#pragma unroll
-        for (int op = 0; op < 3; ++op) {
-            at[op] = 0;
-#pragma unroll
-            for (int j = 0; j < 12; ++j) raw[op][j] = 0;
-        }
-        auto fetch = [&]() {                                // span sp of item `it`
+        // the next span of this CTA's items; returns its bytes per row (0: none), one bit in `live` per existing row
+        auto fetch = [&](uint32_t (&raw)[2][12], uint32_t (&at)[2], uint32_t& live) -> int {
+            if (!have) return 0;
             const int valid = (int)min((int64_t)32, kb - (int64_t)sp * 32);
-            live[0] = r < a.rows_w && it.n0 + r < a.N;
-            live[1] = r < it.tokens;
-            live[2] = r + 128 < it.tokens;
-            if (live[0])
-                fetch_scale_row(a.ws + (int64_t)it.eid * a.ws_se + (int64_t)(it.n0 + r) * a.ws_sn + sp * 32, valid, a.ws, w_hi, raw[0], &at[0]);
-            if (live[1]) fetch_scale_row(a.xs + ((int64_t)it.row0 + r) * kb + sp * 32, valid, a.xs, x_hi, raw[1], &at[1]);
-            if (live[2]) fetch_scale_row(a.xs + ((int64_t)it.row0 + r + 128) * kb + sp * 32, valid, a.xs, x_hi, raw[2], &at[2]);
-        };
-        if (have) fetch();
-        uint32_t slot = 0, phase = 0;
-        bool ok = true;
-        while (have && ok) {
-            const int valid = (int)min((int64_t)32, kb - (int64_t)sp * 32);
-            uint32_t out[3][8];
-            bool put[3];
+            live = 0;
 #pragma unroll
-            for (int op = 0; op < 3; ++op) {
-                put[op] = live[op];                         // stale bytes of other rows belong to accumulator entries
-                align_scale_row(raw[op], at[op], valid, out[op]);      // that nobody reads
+            for (int o = 0; o < 2; ++o) {
+                const int x = u + o * kRows - 128;          // activation row, or (negative) weight row x + 128
+                const bool w = x < 0;
+                const bool in = w ? x + 128 < a.rows_w && it.n0 + x + 128 < a.N : x < it.tokens;
+                if (in) {
+                    live |= 1u << o;
+                    const uint8_t* p = w ? a.ws + (int64_t)it.eid * a.ws_se + (int64_t)(it.n0 + x + 128) * a.ws_sn
+                                         : a.xs + ((int64_t)it.row0 + x) * kb;
+                    fetch_scale_row(p + sp * 32, valid, w ? a.ws : a.xs, w ? w_hi : x_hi, raw[o], &at[o]);
+                }
             }
             if (++sp == spans) {
                 sp = 0;
                 id += gridDim.x;
                 have = next_qitem(a, tb, g, id, &it);
             }
-            if (have) fetch();
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(sc_done + slot, phase ^ 1, abort_flag));
-            if (!ok) break;
-            uint8_t* dst = s_scale + slot * span_bytes + (r & 31) * 16 + (r >> 5) * 4;
+            return valid;
+        };
+        uint32_t raw[2][12] = {}, at[2] = {}, live = 0, slot = 0, phase = 0;
+        int valid = fetch(raw, at, live);
+        while (valid) {
+            uint32_t out[2][8];
+            const uint32_t put = live;                      // stale bytes of other rows belong to accumulator entries that
+#pragma unroll                                              // nobody reads
+            for (int o = 0; o < 2; ++o) align_scale_row(raw[o], at[o], valid, out[o]);
+            valid = fetch(raw, at, live);                   // on its way while this span waits for its slot and is written
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(sc_done + slot, phase ^ 1, abort_flag))) break;
 #pragma unroll
-            for (int op = 0; op < 3; ++op) {
-                if (!put[op]) continue;
+            for (int o = 0; o < 2; ++o) {
+                if (!(put & (1u << o))) continue;
+                const int f = u + o * kRows;
+                uint8_t* dst = s_scale + slot * span_bytes + (f >> 7) * 512 + (f & 31) * 16 + ((f >> 5) & 3) * 4;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) *reinterpret_cast<uint32_t*>(dst + j * half_bytes + op * 512) = out[op][j];
+                for (int j = 0; j < 8; ++j) *reinterpret_cast<uint32_t*>(dst + j * half_bytes) = out[o][j];
             }
             fence_proxy_async();
             __syncwarp();
@@ -423,7 +442,7 @@ w4a4_kernel(const W4A4Args a, const __grid_constant__ CUtensorMap x_map, const _
         uint32_t buf = 0, acc_phase = 0;
         bool ok = true;
         const bool pair_ok = (a.N % 2) == 0;
-        for (int64_t id = blockIdx.x; ok && next_qitem(a, tb, g, id, &it); id += gridDim.x) {
+        for (uint32_t id = blockIdx.x; ok && next_qitem(a, tb, g, id, &it); id += gridDim.x) {
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(acc_full + buf, acc_phase, abort_flag));
             if (!ok) break;
             tc_fence_after();
@@ -437,29 +456,38 @@ w4a4_kernel(const W4A4Args a, const __grid_constant__ CUtensorMap x_map, const _
                 if (lane == 0) mbar_arrive(acc_empty + buf);
             };
             if (e >= chunks) release_acc();              // nothing to drain for this warp
-            for (int c = e; c < chunks; c += 2) {
-                uint32_t r[32];
-                tmem_ld32(tmem_base + buf * (uint32_t)a.tok_cap + ((uint32_t)(q * 32) << 16) + (uint32_t)(c * 32), r);
-                tmem_ld_wait();
-                if (c + 2 >= chunks) release_acc();      // all this warp needs is in registers
-                const int t0 = c * 32;
+            // everything this warp drains is packed into registers first, so that the accumulator is free for the next
+            // item before the stores begin: word i of chunk c = tokens 32c + 2i, 2i + 1 of this lane's column
+            uint32_t v[kQEpiChunks][16];
+#pragma unroll
+            for (int k = 0; k < kQEpiChunks; ++k) {
+                if (e + 2 * k >= chunks) break;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t r[16];
+                    tmem_ld16(tmem_base + buf * (uint32_t)a.tok_cap + ((uint32_t)(q * 32) << 16) + (uint32_t)((e + 2 * k) * 32 + h * 16), r);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[k][8 * h + j] = pack_bf16x2(__uint_as_float(r[2 * j + 1]), __uint_as_float(r[2 * j]));
+                }
+            }
+            if (e < chunks) release_acc();
+#pragma unroll
+            for (int k = 0; k < kQEpiChunks; ++k) {
+                if (e + 2 * k >= chunks) break;
+                const int t0 = (e + 2 * k) * 32;
                 if (pair_ok) {
-                    // lanes 2i and 2i+1 swap one value: the even lane stores (n, n+1) of token j,
-                    // the odd lane (n-1, n) of token j+1 -- 4-byte stores, 64 bytes per half warp
+                    // lanes 2i and 2i+1 swap words: the even lane stores columns (n, n+1) of token 2j, the odd lane
+                    // (n-1, n) of token 2j+1 -- 4-byte stores, 64 bytes per half warp
                     const int odd = lane & 1;
-                    const int left = mine ? it.tokens - t0 - odd : 0;     // store while j < left
+                    const int left = mine ? it.tokens - t0 - odd : 0;     // store while 2j < left
                     uint16_t* p = a.out + (int64_t)(it.row0 + t0 + odd) * a.N + (n - odd);
                     const int64_t step = 2 * a.N;
-                    uint32_t v[16];
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        const float m0 = __uint_as_float(r[j]), m1 = __uint_as_float(r[j + 1]);
-                        const float got = __shfl_xor_sync(0xffffffffu, odd ? m0 : m1, 1);
-                        v[j >> 1] = odd ? pack_bf16x2(m1, got) : pack_bf16x2(got, m0);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        if (j < left) *reinterpret_cast<uint32_t*>(p) = v[j >> 1];
+                    for (int j = 0; j < 16; ++j) {
+                        const uint32_t got = __shfl_xor_sync(0xffffffffu, v[k][j], 1);
+                        const uint32_t w = odd ? prmt(got, v[k][j], 0x7632u) : prmt(v[k][j], got, 0x5410u);
+                        if (2 * j < left) *reinterpret_cast<uint32_t*>(p) = w;
                         p += step;
                     }
                 } else {
@@ -467,7 +495,7 @@ w4a4_kernel(const W4A4Args a, const __grid_constant__ CUtensorMap x_map, const _
                     uint16_t* p = a.out + (int64_t)(it.row0 + t0) * a.N + n;
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
-                        if (j < left) *p = f32_to_bf16_bits(__uint_as_float(r[j]));
+                        if (j < left) *p = (uint16_t)(v[k][j >> 1] >> (16 * (j & 1)));
                         p += a.N;
                     }
                 }
@@ -500,7 +528,7 @@ struct W4A4Plan {
 };
 
 // Tile shape from the row counts alone.  max_rows <= 0: unknown, any group may be long.
-static inline W4A4Plan w4a4_plan(int64_t T, int32_t G, int64_t N, int32_t max_rows, int sm_count, int smem_optin) {
+static inline W4A4Plan w4a4_plan(int64_t T, int32_t G, int64_t N, int64_t K, int32_t max_rows, int sm_count, int smem_optin) {
     W4A4Plan p;
     const int64_t longest = max_rows > 0 ? (max_rows < T ? max_rows : T) : T;
     p.tok_cap = (int)round_up(longest < 256 ? longest : 256, 16);
@@ -509,12 +537,12 @@ static inline W4A4Plan w4a4_plan(int64_t T, int32_t G, int64_t N, int32_t max_ro
     p.x_blocks = (p.tok_cap + 127) / 128;
     p.rows_w = 128;
     if (longest <= 64) {
-        // streaming weights: the tile height that shares the rows out most evenly (each item costs its rows and,
-        // for the pipeline's start and the epilogue, about as much as 8 more)
+        // streaming weights: the tile height that shares the rows out most evenly; an item costs its bytes and, for
+        // hand-overs between the roles, about as much time as 9000 bytes more
         double best = 1e30;
-        for (int r = 128; r >= 32; r -= 8) {
+        for (int r = 128; r >= 64; r -= 8) {
             const int64_t rounds = ceil_div((int64_t)G * ceil_div(N, r), sm_count);
-            const double cost = (double)rounds * (r + 8);
+            const double cost = (double)rounds * ((double)r * (double)K * (17.0 / 32.0) + 9000.0);
             if (cost < best) { best = cost; p.rows_w = r; }
         }
     }

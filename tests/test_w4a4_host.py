@@ -67,7 +67,7 @@ def test_tile_plan_fits(T, G, N, max_rows):
         blocks = (cap + 127) // 128
         stage = 16384 + x_rows * 128
         span = 8 * 512 * (1 + blocks)
-        fixed = 1024 + 2 * span + 256 * 16 + 257 * 8 + 16 * 8 + 8 + 512
+        fixed = 1024 + 2 * span + 256 * 16 + 257 * 4 + 16 * 4 + 4 + 512
         stages = min(12, (232448 - fixed) // stage)
         assert stages >= 4 and fixed + stages * stage <= 232448
         slots = stages * 8 * (1 + blocks)
