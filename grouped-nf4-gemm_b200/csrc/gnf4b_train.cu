@@ -16,10 +16,23 @@ bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p
 
 constexpr int kRtWarps = 8;
 
-// CTAs of the forward pass: one while a warp then has few tokens, else all SMs' worth
-int rt_grid(int64_t T, int sm_count) {
-    if (T <= kRtWarps * 16) return 1;
-    return (int)std::min<int64_t>(ceil_div(T, kRtWarps * 2), (int64_t)sm_count * 2);
+// Warps of a forward CTA: as many as their registers let share an SM (a row of up to 512 experts: 16 per CTA)
+constexpr int rt_fwd_warps(int ne) { return ne <= 16 ? 16 : 8; }
+int rt_fwd_warps_of(int32_t E) { return rt_fwd_warps(E <= 512 ? 16 : 32); }
+
+// CTAs of the forward pass: one while a warp then has few tokens, else up to two per SM
+int rt_grid(int64_t T, int32_t E, int sm_count) {
+    const int warps = rt_fwd_warps_of(E);
+    if (T <= warps * 8) return 1;
+    return (int)std::min<int64_t>(ceil_div(T, warps * 2), (int64_t)sm_count * 2);
+}
+
+size_t rt_scratch_bytes(int grid, int32_t E) { return grid == 1 ? 0 : rt_zeroed_bytes(E) + (size_t)grid * 8; }
+
+// whole 16-byte vectors (or as many experts as a lane holds) from every row start on
+bool rt_vec(const void* p, int64_t stride, int32_t E, int dtype) {
+    const int size = dtype == GNF4B_X_FP32 ? 4 : 2;
+    return aligned(p, 16) && (stride * size) % 16 == 0 && (E * size) % 16 == 0;
 }
 
 int rt_check(int dtype, int64_t T, int64_t stride, int32_t E, int32_t k, int32_t mode, int32_t norm) {
@@ -31,19 +44,21 @@ int rt_check(int dtype, int64_t T, int64_t stride, int32_t E, int32_t k, int32_t
 
 template <int LT, int NE>
 cudaError_t rt_fwd(const RouteTrainArgs& a, int grid, cudaStream_t st) {
-    const size_t smem = (size_t)kRtWarps * a.E * 8;
-    auto kfn = route_train_fwd_kernel<LT, NE, kRtWarps>;
+    constexpr int W = rt_fwd_warps(NE);
+    const size_t smem = (size_t)(W + 1) * a.E * 4;
+    auto kfn = route_train_fwd_kernel<LT, NE, W>;
     static int granted[64];
     cudaError_t e = ensure_smem(kfn, smem, granted);
     if (e != cudaSuccess) return e;
-    e = launch_pdl_smem(kfn, (unsigned)grid, (unsigned)(kRtWarps * 32), smem, st, a);
-    if (e != cudaSuccess || grid == 1) return e;
-    return launch_pdl(route_train_finish_kernel, 1u, 1024u, st, a, grid);
+    if (grid > 1) {
+        e = cudaMemsetAsync(a.sum_p, 0, rt_zeroed_bytes(a.E), st);
+        if (e != cudaSuccess) return e;
+    }
+    return launch_pdl_smem(kfn, (unsigned)grid, (unsigned)(W * 32), smem, st, a);
 }
 template <int LT, int NE>
 cudaError_t rt_bwd(const RouteTrainBwdArgs& a, int grid, cudaStream_t st) {
-    const size_t smem = (size_t)kRtWarps * a.E * 4;
-    return launch_pdl_smem(route_train_bwd_kernel<LT, NE, kRtWarps>, (unsigned)grid, (unsigned)(kRtWarps * 32), smem, st, a);
+    return launch_pdl(route_train_bwd_kernel<LT, NE, kRtWarps>, (unsigned)grid, (unsigned)(kRtWarps * 32), st, a);
 }
 
 template <typename F2, typename F4, typename F8, typename F16, typename F32, typename F1>
@@ -58,8 +73,8 @@ extern "C" {
 size_t gnf4b_route_train_scratch_bytes(int64_t T, int32_t E) {
     DevInfo di;
     if (T <= 0 || E <= 0 || device_info(&di)) return 0;
-    const int grid = rt_grid(T, di.sm_count);
-    return grid == 1 ? 0 : (size_t)grid * ((size_t)E * 8 + 8);
+    const int grid = rt_grid(T, E, di.sm_count);
+    return rt_scratch_bytes(grid, E);
 }
 
 int gnf4b_route_train_fwd(const void* logits, int dtype, int64_t T, int64_t stride, int32_t E, int32_t k, int32_t mode, int32_t norm,
@@ -71,15 +86,18 @@ int gnf4b_route_train_fwd(const void* logits, int dtype, int64_t T, int64_t stri
     DevInfo di;
     rc = device_info(&di);
     if (rc) return rc;
-    const int grid = rt_grid(T, di.sm_count);
-    if (grid > 1 && (!scratch || !aligned(scratch, 8) || scratch_bytes < (size_t)grid * ((size_t)E * 8 + 8))) return GNF4B_EWORKSPACE;
+    const int grid = rt_grid(T, E, di.sm_count);
+    if (grid > 1 && (!scratch || !aligned(scratch, 8) || scratch_bytes < rt_scratch_bytes(grid, E))) return GNF4B_EWORKSPACE;
     RouteTrainArgs a;
     a.logits = logits; a.T = T; a.stride = stride; a.E = E; a.k = k; a.mode = mode; a.norm = norm;
     a.mask = token_mask; a.idx = idx; a.w = weights; a.lse = lse; a.counts = counts;
     a.balance = balance_loss; a.z = z_loss; a.n_tokens = n_tokens;
-    a.part_p = static_cast<float*>(scratch);
-    a.part_c = reinterpret_cast<int32_t*>(a.part_p + (size_t)grid * E);
-    a.part_zn = reinterpret_cast<float*>(a.part_c + (size_t)grid * E);
+    a.sum_p = static_cast<unsigned long long*>(scratch);
+    a.sum_c = reinterpret_cast<uint32_t*>(a.sum_p + E);
+    a.arrived = a.sum_c + E;
+    a.not_finite = a.arrived + 1;
+    a.part_zn = reinterpret_cast<float*>(a.not_finite + 1);
+    a.vec = rt_vec(logits, stride, E, dtype);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
 #define GNF4B_RT(L) by_experts(E, [&] { return rt_fwd<L, 1>(a, grid, st); }, [&] { return rt_fwd<L, 2>(a, grid, st); }, \
         [&] { return rt_fwd<L, 4>(a, grid, st); }, [&] { return rt_fwd<L, 8>(a, grid, st); }, [&] { return rt_fwd<L, 16>(a, grid, st); }, \
@@ -103,6 +121,8 @@ int gnf4b_route_train_bwd(const void* logits, int dtype, int64_t T, int64_t stri
     RouteTrainBwdArgs a;
     a.logits = logits; a.T = T; a.stride = stride; a.E = E; a.k = k; a.mode = mode; a.norm = norm;
     a.mask = token_mask; a.idx = idx; a.w = weights; a.lse = lse; a.counts = counts; a.n_tokens = n_tokens;
+    a.vec = rt_vec(logits, stride, E, dtype);
+    a.vec_grad = rt_vec(grad, E, E, dtype);
     a.g_w = g_weights; a.g_balance = g_balance; a.g_z = g_z; a.grad = grad;
     const int grid = (int)std::min<int64_t>(ceil_div(T, kRtWarps), (int64_t)di.sm_count * 8);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);

@@ -8,10 +8,19 @@
 //   dl_e = p_e (G_e - sum_j p_j G_j) + 2 g_z lse p_e / n,   G_e = [e = idx_j] g_w_j + g_b E f_e / n
 //   (f is piecewise constant; renormalised weights instead give w_j (g_j - sum_i w_i g_i) at idx_j)
 //
-// One warp per token, the row in registers (lane = expert mod 32), so the logits are read once forward and once
-// backward and nothing of size [T, E] is written but the gradient.  Forward keeps each warp's probability sums and
-// counts in registers over all its tokens; warps of a CTA, then CTAs, are added in a fixed order: no floating-point
-// atomics, the same bits on every run.
+// One warp per token, the row in registers (16-byte loads: lane l holds V neighbouring experts of every 32 V), so the
+// logits are read once forward and once backward and nothing of size [T, E] is written but the gradient.
+//
+// The k largest: the k-th largest of the lanes' own maxima bounds the k-th largest of the row from below, and in the mean
+// only a few more than k elements reach that bound.  They are gathered in shared memory, one per lane, and each lane
+// counts how many of them come before its own (larger, or equal and of a lower index): that is its place.  Where more
+// than 32 reach the bound (many equal logits) the k are picked one after the other instead.  Picking alone, a scan of
+// the lane's registers per choice, costs about three times the instructions, and instructions are what bounds this pass.
+//
+// Forward keeps each warp's probability sums in registers over all its tokens and the counts as integers in shared
+// memory.  The warps of a CTA are added in a fixed order, the CTAs by integer atomics: counts as they are, probability
+// sums as 64-bit fixed-point numbers in steps of 2^-32 (a sum is at most 2^31; a step is far below the fp32 sums' own
+// rounding), so that the order in which CTAs arrive cannot change a bit.  The last CTA to arrive computes the losses.
 #pragma once
 
 #include "common.cuh"
@@ -21,29 +30,109 @@ namespace gnf4b {
 constexpr int kRtMaxExperts = 1024;
 constexpr int kRtMaxK = 32;
 
-// Order-preserving integer of a float: NaN 1, then -inf .. +inf; 0 is left for "no expert here" and "already taken".
+// Order-preserving integer of a float: -NaN .. -inf .. +inf .. +NaN; a NaN is to come last, see rt_fix_nan.
+constexpr uint32_t kRtKeyInf = 0xff800000u, kRtKeyNegInf = 0x007fffffu;
 __device__ __forceinline__ uint32_t rt_key(float v) {
     const uint32_t b = __float_as_uint(v + 0.0f);                 // -0 and +0 tie
-    if ((b & 0x7fffffffu) > 0x7f800000u) return 1u;
-    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ uint32_t rt_fix_nan(uint32_t key) { return key > kRtKeyInf || key < kRtKeyNegInf ? 1u : key; }
 __device__ __forceinline__ float rt_value(uint32_t key) {
     if (key == 1u) return __uint_as_float(0x7fc00000u);
     return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
 }
+__device__ __forceinline__ float rt_exp(float x) {                // e^x, x <= 0 but for NaN: a few units of 2^-24 times (1 + |x|)
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+    return r;
+}
 
-template <int LT>      // 0 bf16, 1 fp16, 2 fp32
-__device__ __forceinline__ float rt_load(const void* p, int64_t i) {
-    if (LT == 2) return __ldg(static_cast<const float*>(p) + i);
-    const unsigned short b = __ldg(static_cast<const unsigned short*>(p) + i);
-    return LT == 0 ? bf16_bits_to_float(b) : __half2float(__ushort_as_half(b));
-}
-template <int LT>
-__device__ __forceinline__ void rt_store(void* p, int64_t i, float v) {
-    if (LT == 2) static_cast<float*>(p)[i] = v;
-    else if (LT == 0) static_cast<uint16_t*>(p)[i] = f32_to_bf16_bits(v);
-    else static_cast<unsigned short*>(p)[i] = __half_as_ushort(__float2half_rn(v));
-}
+// The row of NE elements per lane: element i of a lane is expert rt_expert(lane, i).  LT 0 bf16, 1 fp16, 2 fp32.
+template <int LT, int NE>
+struct RtRow {
+    static constexpr int V = LT == 2 ? (NE < 4 ? NE : 4) : (NE < 8 ? NE : 8);
+    static constexpr int kWords = V * (LT == 2 ? 4 : 2) / 4;      // 32-bit words of a vector; 0: one 16-bit element
+    __device__ __forceinline__ static int expert(int lane, int i) { return (i / V) * (32 * V) + lane * V + (i % V); }
+    // experts >= E read as -inf.  vec: rows and E allow whole vectors
+    __device__ __forceinline__ static void load(const void* row, int lane, int E, bool vec, float* x) {
+#pragma unroll
+        for (int g = 0; g < NE / V; ++g) {
+            const int e0 = g * 32 * V + lane * V;
+            if (kWords > 0 && vec) {
+                uint32_t w[kWords > 0 ? kWords : 1];
+                const uint8_t* p = static_cast<const uint8_t*>(row) + (int64_t)e0 * (LT == 2 ? 4 : 2);
+                const bool in = e0 < E;
+                if (kWords == 4) {
+                    uint4 q = make_uint4(0, 0, 0, 0);
+                    if (in) q = __ldcs(reinterpret_cast<const uint4*>(p));
+                    w[0] = q.x;
+                    if (kWords > 1) w[kWords > 1 ? 1 : 0] = q.y;
+                    if (kWords > 2) { w[kWords > 2 ? 2 : 0] = q.z; w[kWords > 3 ? 3 : 0] = q.w; }
+                } else if (kWords == 2) {
+                    uint2 q = make_uint2(0, 0);
+                    if (in) q = __ldcs(reinterpret_cast<const uint2*>(p));
+                    w[0] = q.x;
+                    w[kWords > 1 ? 1 : 0] = q.y;
+                } else {
+                    w[0] = in ? __ldcs(reinterpret_cast<const uint32_t*>(p)) : 0u;
+                }
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    float v;
+                    if (LT == 2) v = __uint_as_float(w[j < kWords ? j : 0]);
+                    else {
+                        const uint32_t h = (w[(j >> 1) < kWords ? (j >> 1) : 0] >> (16 * (j & 1))) & 0xffffu;
+                        v = LT == 0 ? bf16_bits_to_float(h) : __half2float(__ushort_as_half((unsigned short)h));
+                    }
+                    x[g * V + j] = in ? v : -INFINITY;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    float v = -INFINITY;
+                    if (e0 + j < E) {
+                        if (LT == 2) v = __ldg(static_cast<const float*>(row) + e0 + j);
+                        else {
+                            const unsigned short h = __ldg(static_cast<const unsigned short*>(row) + e0 + j);
+                            v = LT == 0 ? bf16_bits_to_float(h) : __half2float(__ushort_as_half(h));
+                        }
+                    }
+                    x[g * V + j] = v;
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ static uint32_t bits(float v) {
+        return LT == 2 ? __float_as_uint(v) : LT == 0 ? (uint32_t)f32_to_bf16_bits(v) : (uint32_t)__half_as_ushort(__float2half_rn(v));
+    }
+    __device__ __forceinline__ static void store(void* row, int lane, int E, bool vec, const float* x) {
+#pragma unroll
+        for (int g = 0; g < NE / V; ++g) {
+            const int e0 = g * 32 * V + lane * V;
+            if (kWords > 0 && vec) {
+                uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    if (LT == 2) w[j & 3] = bits(x[g * V + j]);
+                    else w[(j >> 1) & 3] |= bits(x[g * V + j]) << (16 * (j & 1));
+                }
+                uint8_t* p = static_cast<uint8_t*>(row) + (int64_t)e0 * (LT == 2 ? 4 : 2);
+                if (e0 < E) {
+                    if (kWords == 4) __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
+                    else if (kWords == 2) __stcs(reinterpret_cast<uint2*>(p), make_uint2(w[0], w[1]));
+                    else __stcs(reinterpret_cast<uint32_t*>(p), w[0]);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (e0 + j < E) {
+                        if (LT == 2) static_cast<float*>(row)[e0 + j] = x[g * V + j];
+                        else static_cast<uint16_t*>(row)[e0 + j] = (uint16_t)bits(x[g * V + j]);
+                    }
+            }
+        }
+    }
+};
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -55,6 +144,7 @@ struct RouteTrainArgs {
     const void* logits;
     int64_t T, stride;           // elements between rows
     int32_t E, k, mode, norm;
+    int32_t vec;                 // rows and E allow 16-byte loads
     const uint8_t* mask;         // optional, nonzero = counts
     int64_t* idx;
     float* w;
@@ -63,172 +153,233 @@ struct RouteTrainArgs {
     float* balance;
     float* z;
     float* n_tokens;
-    float* part_p;               // [grid][E]
-    int32_t* part_c;             // [grid][E]
+    // scratch of several CTAs, zero before the launch but for part_zn
+    unsigned long long* sum_p;   // [E], steps of 2^-32
+    uint32_t* sum_c;             // [E]
+    uint32_t* arrived;
+    uint32_t* not_finite;        // a probability sum was NaN
     float* part_zn;              // [grid][2]
 };
-
-// sums over the CTAs' parts (or the one CTA's own) -> counts, losses; all threads of one CTA
-__device__ __forceinline__ void rt_finish(const RouteTrainArgs& a, int parts, const float* part_p, const int32_t* part_c,
-                                          const float* part_zn, float* s_red) {
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, warps = blockDim.x >> 5;
-    float z = 0.f, n = 0.f;
-    if (t < 32) {                                    // one warp: part t, t + 32, ... then a fixed tree
-        for (int c = t; c < parts; c += 32) { z += part_zn[2 * c]; n += part_zn[2 * c + 1]; }
-        z = warp_sum(z);
-        n = warp_sum(n);
-        if (t == 0) { s_red[64] = z; s_red[65] = n; }
-    }
-    float bal = 0.f;
-    for (int e = t; e < a.E; e += blockDim.x) {
-        float p = 0.f;
-        int32_t c = 0;
-#pragma unroll 8
-        for (int q = 0; q < parts; ++q) {
-            p += part_p[(int64_t)q * a.E + e];
-            c += part_c[(int64_t)q * a.E + e];
-        }
-        a.counts[e] = c;
-        bal += (float)c * p;
-    }
-    bal = warp_sum(bal);
-    if (lane == 0) s_red[warp] = bal;
-    __syncthreads();
-    if (t == 0) {
-        float sum = 0.f;
-        for (int v = 0; v < warps; ++v) sum += s_red[v];
-        const float nt = s_red[65];
-        *a.n_tokens = nt;
-        *a.balance = nt > 0.f ? (float)a.E * (sum / (nt * (float)a.k)) / nt : 0.f;
-        *a.z = nt > 0.f ? s_red[64] / nt : 0.f;
-    }
-}
+__host__ __device__ inline size_t rt_zeroed_bytes(int32_t E) { return (size_t)E * 12 + 8; }
 
 template <int LT, int NE, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32)
-route_train_fwd_kernel(const RouteTrainArgs a) {
-    extern __shared__ float s_mem[];                 // [WARPS][E] probability sums, then as many counts
+route_train_fwd_kernel(const __grid_constant__ RouteTrainArgs a) {
+    using Row = RtRow<LT, NE>;
+    extern __shared__ __align__(16) float s_mem[];   // [WARPS][E] probability sums, then [E] counts
+    __shared__ uint2 s_cand[WARPS][32];
     __shared__ float s_zn[WARPS][2];
-    __shared__ float s_red[66];
+    __shared__ float s_tot[34];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int32_t* s_c = reinterpret_cast<int32_t*>(s_mem + WARPS * a.E);
+    for (int e = threadIdx.x; e < a.E; e += WARPS * 32) s_c[e] = 0;
+    __syncthreads();
     pdl_wait();
     pdl_launch_dependents();
     float psum[NE];
-    int32_t cnt[NE];
 #pragma unroll
-    for (int i = 0; i < NE; ++i) { psum[i] = 0.f; cnt[i] = 0; }
+    for (int i = 0; i < NE; ++i) psum[i] = 0.f;
     float zsum = 0.f, ntok = 0.f;
     const int64_t step = (int64_t)gridDim.x * WARPS;
+    const int64_t item = LT == 2 ? 4 : 2;
+    const uint8_t* base = static_cast<const uint8_t*>(a.logits);
+    const bool vec = a.vec != 0, renorm = a.mode == 1 || a.norm;
     int64_t t = (int64_t)blockIdx.x * WARPS + warp;
     float v[NE];
-    auto load = [&](int64_t row) {
-#pragma unroll
-        for (int i = 0; i < NE; ++i) {
-            const int e = lane + 32 * i;
-            v[i] = (row < a.T && e < a.E) ? rt_load<LT>(a.logits, row * a.stride + e) : 0.f;
-        }
-    };
-    load(t);
+    if (t < a.T) Row::load(base + t * a.stride * item, lane, a.E, vec, v);
     for (; t < a.T; t += step) {
-        uint32_t key[NE];
         float x[NE];
+        uint32_t key[NE], best = 0;
 #pragma unroll
         for (int i = 0; i < NE; ++i) {
             x[i] = v[i];
-            key[i] = lane + 32 * i < a.E ? rt_key(x[i]) : 0u;
+            key[i] = rt_key(x[i]);
+            best = max(best, key[i]);
         }
         const bool masked = a.mask && __ldg(a.mask + t) == 0;
-        load(t + step);                              // the next row is on its way while this one is worked on
-        uint32_t best = 0;
-#pragma unroll
-        for (int i = 0; i < NE; ++i) best = max(best, key[i]);
-        const uint32_t top_key = __reduce_max_sync(0xffffffffu, best);
-        const float top = rt_value(top_key);
-        const bool dead = top == -INFINITY;          // nothing to choose from: no weight, no loss, no count
-        const bool counted = !masked && !dead;
-        float ex[NE], z = 0.f;
+        if (t + step < a.T) Row::load(base + (t + step) * a.stride * item, lane, a.E, vec, v);     // on its way meanwhile
+        uint32_t top_key = __reduce_max_sync(0xffffffffu, best);
+        float top = rt_value(top_key), z = 0.f;
 #pragma unroll
         for (int i = 0; i < NE; ++i) {
-            ex[i] = (!dead && lane + 32 * i < a.E) ? expf(x[i] - top) : 0.f;
-            z += ex[i];
+            x[i] = rt_exp(x[i] - top);
+            z += x[i];
         }
         z = warp_sum(z);
+        bool dead = false;                           // nothing to choose from: no weight, no loss, no count
+        if (z != z) {                                // a NaN, an infinity or nothing but -inf: rare
+            bool nan = false;
+            best = 0;
+#pragma unroll
+            for (int i = 0; i < NE; ++i) {
+                const uint32_t fixed = rt_fix_nan(key[i]);
+                nan |= fixed != key[i];
+                key[i] = fixed;
+                best = max(best, Row::expert(lane, i) < a.E ? fixed : 0u);
+            }
+            top_key = __reduce_max_sync(0xffffffffu, best);
+            top = rt_value(top_key);
+            dead = !__any_sync(0xffffffffu, nan) && top_key == kRtKeyNegInf;
+            if (dead) {
+#pragma unroll
+                for (int i = 0; i < NE; ++i) x[i] = 0.f;
+            }
+        }
+        const bool counted = !masked && !dead;
         const float lse = dead ? -INFINITY : top + logf(z);
         if (counted) {
             const float rz = 1.0f / z;
 #pragma unroll
-            for (int i = 0; i < NE; ++i) psum[i] += ex[i] * rz;
+            for (int i = 0; i < NE; ++i) psum[i] = fmaf(x[i], rz, psum[i]);
             zsum += lse * lse;
             ntok += 1.f;
         }
-        // the k largest, one after the other: the largest key left, and of its holders the lowest expert
-        float sel = 0.f;
-        int32_t sel_e = 0;
-        uint32_t m = top_key;
-        for (int j = 0; j < a.k; ++j) {
-            if (j) m = __reduce_max_sync(0xffffffffu, best);
-            int at = NE;
-#pragma unroll
-            for (int i = NE - 1; i >= 0; --i)
-                if (key[i] == m) at = i;
-            const uint32_t e = __reduce_min_sync(0xffffffffu, at < NE ? (uint32_t)(lane + 32 * at) : 0xffffffffu);
-            if (lane == j) { sel = rt_value(m); sel_e = (int32_t)e; }
-            const int gone = (int)(e & 31u) == lane ? (int)(e >> 5) : -1;
-            best = 0;
+        // the k largest
+        uint32_t sel_key = 0;
+        int32_t sel_e = 0, place = 32;
+        int found;
+        if (NE == 1) {
+            found = a.E;                             // every lane has one
+            sel_key = key[0];
+            sel_e = lane;
+        } else {
+            uint32_t bound = top_key, left = best;
+            for (int j = 1; j < a.k; ++j) {
+                if (left == bound) left = 0;
+                bound = __reduce_max_sync(0xffffffffu, left);
+            }
+            // (a bound of -inf or less would take in the experts >= E: one after the other then)
+            found = bound > kRtKeyNegInf ? 0 : 33;
 #pragma unroll
             for (int i = 0; i < NE; ++i) {
-                if (i == gone) { key[i] = 0; cnt[i] += counted ? 1 : 0; }
-                best = max(best, key[i]);
+                const int e = Row::expert(lane, i);
+                const bool in = key[i] >= bound;
+                const uint32_t who = __ballot_sync(0xffffffffu, in);
+                const int at = found + __popc(who & ((1u << lane) - 1u));
+                if (in && at < 32) s_cand[warp][at] = make_uint2(key[i], (uint32_t)e);
+                found += __popc(who);
+            }
+            __syncwarp();
+            if (lane < found && found <= 32) {
+                const uint2 c = s_cand[warp][lane];
+                sel_key = c.x;
+                sel_e = (int32_t)c.y;
             }
         }
-        float wj = (lane < a.k && !dead) ? expf(sel - top) : 0.f;
-        if (a.mode == 1 || a.norm) z = warp_sum(wj);
-        wj = dead ? 0.f : wj / z;
-        if (lane < a.k) {
-            a.idx[t * a.k + lane] = sel_e;
-            a.w[t * a.k + lane] = wj;
+        if (found <= 32) {
+            place = 0;
+            for (int j = 0; j < found; ++j) {
+                const uint32_t ok = __shfl_sync(0xffffffffu, sel_key, j);
+                const int32_t oe = __shfl_sync(0xffffffffu, sel_e, j);
+                place += (ok > sel_key || (ok == sel_key && oe < sel_e)) ? 1 : 0;
+            }
+            if (lane >= found) place = 32;
+        } else {
+            // one after the other: the largest key left, and of its holders the lowest expert
+            uint32_t mask = 0;                       // this lane's elements that are taken
+            for (int j = 0; j < a.k; ++j) {
+                uint32_t m = 0;
+#pragma unroll
+                for (int i = 0; i < NE; ++i)
+                    if (!(mask >> i & 1u) && Row::expert(lane, i) < a.E) m = max(m, key[i]);
+                m = __reduce_max_sync(0xffffffffu, m);
+                uint32_t e = 0xffffffffu;
+#pragma unroll
+                for (int i = 0; i < NE; ++i)
+                    if (!(mask >> i & 1u) && key[i] == m && Row::expert(lane, i) < a.E) e = min(e, (uint32_t)Row::expert(lane, i));
+                e = __reduce_min_sync(0xffffffffu, e);
+#pragma unroll
+                for (int i = 0; i < NE; ++i)
+                    if ((uint32_t)Row::expert(lane, i) == e) mask |= 1u << i;
+                if (lane == j) { sel_key = m; sel_e = (int32_t)e; place = j; }
+            }
+        }
+        const bool chosen = place < a.k;
+        const float ej = (chosen && !dead) ? rt_exp(rt_value(sel_key) - top) : 0.f;
+        if (renorm) z = warp_sum(ej);
+        if (chosen) {
+            a.idx[t * a.k + place] = sel_e;
+            a.w[t * a.k + place] = dead ? 0.f : ej / z;
+            if (counted) atomicAdd(s_c + sel_e, 1);
         }
         if (lane == 0) a.lse[t] = lse;
+        __syncwarp();                                // before the candidates' slots are written again
     }
+    __syncthreads();
     float* s_p = s_mem;
-    int32_t* s_c = reinterpret_cast<int32_t*>(s_mem + WARPS * a.E);
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
-        const int e = lane + 32 * i;
-        if (e < a.E) { s_p[warp * a.E + e] = psum[i]; s_c[warp * a.E + e] = cnt[i]; }
+        const int e = Row::expert(lane, i);
+        if (e < a.E) s_p[warp * a.E + e] = psum[i];
     }
     if (lane == 0) { s_zn[warp][0] = zsum; s_zn[warp][1] = ntok; }
     __syncthreads();
-    if (gridDim.x == 1) {                            // a small batch: this CTA has everything
-        rt_finish(a, WARPS, s_p, s_c, &s_zn[0][0], s_red);
-        return;
-    }
+    const bool only = gridDim.x == 1;
     for (int e = threadIdx.x; e < a.E; e += WARPS * 32) {
         float p = 0.f;
-        int32_t c = 0;
-        for (int q = 0; q < WARPS; ++q) { p += s_p[q * a.E + e]; c += s_c[q * a.E + e]; }
-        a.part_p[(int64_t)blockIdx.x * a.E + e] = p;
-        a.part_c[(int64_t)blockIdx.x * a.E + e] = c;
+        for (int q = 0; q < WARPS; ++q) p += s_p[q * a.E + e];
+        s_p[e] = p;                                  // its own column: no other thread reads it
+        if (!only) {
+            if (p == p) atomicAdd(a.sum_p + e, (unsigned long long)((double)p * 4294967296.0));
+            else atomicOr(a.not_finite, 1u);
+            if (s_c[e]) atomicAdd(a.sum_c + e, (uint32_t)s_c[e]);
+        }
     }
+    float z = 0.f, n = 0.f;
     if (threadIdx.x == 0) {
-        float z = 0.f, n = 0.f;
         for (int q = 0; q < WARPS; ++q) { z += s_zn[q][0]; n += s_zn[q][1]; }
-        a.part_zn[2 * blockIdx.x] = z;
-        a.part_zn[2 * blockIdx.x + 1] = n;
+        s_tot[32] = z;
+        s_tot[33] = n;
+        if (!only) {
+            a.part_zn[2 * blockIdx.x] = z;
+            a.part_zn[2 * blockIdx.x + 1] = n;
+        }
     }
-}
-
-static __global__ void __launch_bounds__(1024) route_train_finish_kernel(const RouteTrainArgs a, int parts) {
-    __shared__ float s_red[66];
-    pdl_wait();
-    pdl_launch_dependents();
-    rt_finish(a, parts, a.part_p, a.part_c, a.part_zn, s_red);
+    __shared__ uint32_t s_last;
+    if (!only) {
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) s_last = atomicAdd(a.arrived, 1u) == gridDim.x - 1;
+        __syncthreads();
+        if (!s_last) return;
+        __threadfence();
+        if (warp == 0) {                             // part lane, lane + 32, ... then a fixed tree
+            z = 0.f;
+            n = 0.f;
+            for (int c = lane; c < (int)gridDim.x; c += 32) { z += __ldcg(a.part_zn + 2 * c); n += __ldcg(a.part_zn + 2 * c + 1); }
+            z = warp_sum(z);
+            n = warp_sum(n);
+            if (lane == 0) { s_tot[32] = z; s_tot[33] = n; }
+        }
+        const bool bad = __ldcg(a.not_finite) != 0;
+        for (int e = threadIdx.x; e < a.E; e += WARPS * 32) {
+            s_c[e] = (int32_t)__ldcg(a.sum_c + e);
+            s_p[e] = bad ? __uint_as_float(0x7fc00000u) : (float)((double)__ldcg(a.sum_p + e) * (1.0 / 4294967296.0));
+        }
+    }
+    float bal = 0.f;                                 // each thread its own columns of s_c and s_p
+    for (int e = threadIdx.x; e < a.E; e += WARPS * 32) {
+        a.counts[e] = s_c[e];
+        bal += (float)s_c[e] * s_p[e];
+    }
+    bal = warp_sum(bal);
+    if (lane == 0) s_tot[warp] = bal;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float sum = 0.f;
+        for (int q = 0; q < WARPS; ++q) sum += s_tot[q];
+        const float nt = s_tot[33];
+        *a.n_tokens = nt;
+        *a.balance = nt > 0.f ? (float)a.E * (sum / (nt * (float)a.k)) / nt : 0.f;
+        *a.z = nt > 0.f ? s_tot[32] / nt : 0.f;
+    }
 }
 
 struct RouteTrainBwdArgs {
     const void* logits;
     int64_t T, stride;
     int32_t E, k, mode, norm;
+    int32_t vec, vec_grad;       // rows and E allow 16-byte loads / stores
     const uint8_t* mask;
     const int64_t* idx;
     const float* w;
@@ -243,11 +394,13 @@ struct RouteTrainBwdArgs {
 
 template <int LT, int NE, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32)
-route_train_bwd_kernel(const RouteTrainBwdArgs a) {
-    extern __shared__ float s_sel[];                 // [WARPS][E]: what the weights' gradient adds at the chosen experts
+route_train_bwd_kernel(const __grid_constant__ RouteTrainBwdArgs a) {
+    using Row = RtRow<LT, NE>;
+    __shared__ __align__(16) float s_sel[WARPS][NE * 32];        // what the weights' gradient adds at the chosen experts
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    float* mine = s_sel + warp * a.E;
-    for (int e = lane; e < a.E; e += 32) mine[e] = 0.f;
+    float* mine = s_sel[warp];
+#pragma unroll
+    for (int i = 0; i < NE; ++i) mine[lane + 32 * i] = 0.f;
     pdl_wait();
     pdl_launch_dependents();
     __syncwarp();
@@ -256,52 +409,67 @@ route_train_bwd_kernel(const RouteTrainBwdArgs a) {
     const float gz = (a.g_z && n > 0.f) ? 2.f * __ldg(a.g_z) / n : 0.f;
     float push[NE];                                  // d balance / d p_e of one token
 #pragma unroll
-    for (int i = 0; i < NE; ++i) push[i] = lane + 32 * i < a.E ? gb * (float)__ldg(a.counts + lane + 32 * i) : 0.f;
-    const bool renorm = a.mode == 1 || a.norm;
-    for (int64_t t = (int64_t)blockIdx.x * WARPS + warp; t < a.T; t += (int64_t)gridDim.x * WARPS) {
-        float x[NE];
-#pragma unroll
-        for (int i = 0; i < NE; ++i) {
-            const int e = lane + 32 * i;
-            x[i] = e < a.E ? rt_load<LT>(a.logits, t * a.stride + e) : 0.f;
+    for (int i = 0; i < NE; ++i) {
+        const int e = Row::expert(lane, i);
+        push[i] = e < a.E ? gb * (float)__ldg(a.counts + e) : 0.f;
+    }
+    const bool renorm = a.mode == 1 || a.norm, vec = a.vec != 0, vec_grad = a.vec_grad != 0;
+    const int64_t item = LT == 2 ? 4 : 2;
+    const int64_t step = (int64_t)gridDim.x * WARPS;
+    int64_t t = (int64_t)blockIdx.x * WARPS + warp;
+    // a token's loads are issued while the one before it is worked on
+    float v[NE], lse_n = 0.f, w_n = 0.f, g_n = 0.f;
+    int64_t e_n = -1;
+    bool keep_n = true;
+    auto load = [&](int64_t row) {
+        Row::load(static_cast<const uint8_t*>(a.logits) + row * a.stride * item, lane, a.E, vec, v);
+        lse_n = __ldg(a.lse + row);
+        if (a.mask) keep_n = __ldg(a.mask + row) != 0;
+        if (a.g_w && lane < a.k) {
+            e_n = __ldg(a.idx + row * a.k + lane);
+            w_n = __ldg(a.w + row * a.k + lane);
+            g_n = __ldg(a.g_w + row * a.k + lane);
         }
-        const float lse = __ldg(a.lse + t);
+    };
+    if (t < a.T) load(t);
+    for (; t < a.T; t += step) {
+        const float lse = lse_n, w = w_n, g = g_n;
+        const int64_t e_sel = e_n;
         const bool dead = lse == -INFINITY;
-        const bool counted = !dead && !(a.mask && __ldg(a.mask + t) == 0);
-        int64_t e_sel = 0;
-        float w = 0.f, g = 0.f;
-        const bool has = a.g_w && lane < a.k;
-        if (has) {
-            e_sel = __ldg(a.idx + t * a.k + lane);
-            w = __ldg(a.w + t * a.k + lane);
-            g = __ldg(a.g_w + t * a.k + lane);
-        }
-        // nothing comes back through this token's weights (padding, or weights that are not used): no term, whatever its
-        // logits are -- a NaN in a masked token stays out
-        const bool through_w = __any_sync(0xffffffffu, g != 0.f);
-        const float gw = warp_sum(g * w);
-        if (has && e_sel >= 0 && e_sel < a.E) mine[e_sel] = renorm ? w * (g - gw) : g;
-        __syncwarp();
+        const bool counted = !dead && keep_n;
+        const bool has = e_sel >= 0 && e_sel < a.E;
         float p[NE], ap = 0.f;
 #pragma unroll
         for (int i = 0; i < NE; ++i) {
-            p[i] = (!dead && lane + 32 * i < a.E) ? expf(x[i] - lse) : 0.f;
-            ap += p[i] * push[i];
+            p[i] = dead ? 0.f : rt_exp(v[i] - lse);
+            ap = fmaf(p[i], push[i], ap);
         }
-        ap = warp_sum(ap);
-        const float zc = gz * lse;
+        if (t + step < a.T) load(t + step);
+        // nothing comes back through this token's weights (padding, or weights that are not used): no term, whatever its
+        // logits are -- a NaN in a masked token stays out
+        const bool through_w = __any_sync(0xffffffffu, g != 0.f) && !dead;
+        float gw = g * w;
 #pragma unroll
-        for (int i = 0; i < NE; ++i) {
-            const int e = lane + 32 * i;
-            if (e < a.E) {
-                const float s = mine[e];
-                float d = (dead || !through_w) ? 0.f : renorm ? s : p[i] * (s - gw);
-                if (counted) d += p[i] * (push[i] - ap + zc);
-                rt_store<LT>(a.grad, t * a.E + e, d);
+        for (int o = 16; o > 0; o >>= 1) {
+            gw += __shfl_xor_sync(0xffffffffu, gw, o);
+            ap += __shfl_xor_sync(0xffffffffu, ap, o);
+        }
+        if (through_w && has) mine[e_sel] = renorm ? w * (g - gw) : g;
+        __syncwarp();
+        const float zc = gz * lse - ap;
+        float d[NE];
+#pragma unroll
+        for (int i = 0; i < NE; ++i) d[i] = counted ? p[i] * (push[i] + zc) : 0.f;
+        if (through_w) {
+#pragma unroll
+            for (int i = 0; i < NE; ++i) {
+                const float s = mine[Row::expert(lane, i)];
+                d[i] += renorm ? s : p[i] * (s - gw);
             }
         }
+        Row::store(static_cast<uint8_t*>(a.grad) + t * a.E * item, lane, a.E, vec_grad, d);
         __syncwarp();
-        if (has && e_sel >= 0 && e_sel < a.E) mine[e_sel] = 0.f;
+        if (has) mine[e_sel] = 0.f;
         __syncwarp();
     }
 }

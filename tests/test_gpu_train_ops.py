@@ -134,6 +134,14 @@ def test_routing_nan_rows_keep_to_themselves(T):
     (a.balance_loss + a.z_loss).backward()
     assert torch.isfinite(x.grad).all()
     assert torch.isnan(ep_moe.route_topk_train(x.detach(), 3).balance_loss)
+    for bits in (0x7fc00000, -0x400000):                     # either sign, beside nothing but -inf: a NaN row, not an empty one
+        y = torch.randn(T, 24, generator=gen(9)).to(DEV)
+        y[4] = float("-inf")
+        y[4, 7] = torch.tensor(bits, dtype=torch.int32).view(torch.float32)
+        assert torch.isnan(y[4, 7])
+        r = ep_moe.route_topk_train(y, 3, 0, True)
+        assert r.idx[4].tolist() == [0, 1, 2] and torch.isnan(r.weights[4]).all() and torch.isnan(r.balance_loss)
+        assert torch.isfinite(r.weights[torch.arange(T, device=DEV) != 4]).all()
 
 
 def test_routing_matches_route_topk_and_its_cpu_form():
