@@ -155,26 +155,33 @@ class _RouteTopkTrain(torch.autograd.Function):
         return idx, w, counts, balance, z
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, _g_idx, g_w, _g_counts, g_balance, g_z):
-        import _gnf4b
-        from nf4_grouped import _call_on
-        logits, token_mask, idx, w, lse, counts = ctx.saved_tensors
-        k, mode, norm = ctx.rule
-        M, E = logits.shape
-        if g_w is not None:
-            g_w = g_w.contiguous()
-        grad = torch.empty(M, E, dtype=logits.dtype, device=logits.device)
-        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-        rc = _call_on(logits.device, _gnf4b.load().gnf4b_route_train_bwd, logits.data_ptr(), _ROUTE_DTYPES[logits.dtype], M,
-                      logits.stride(0) if M > 1 else E, E, k, mode, norm, ptr(token_mask), idx.data_ptr(), w.data_ptr(),
-                      lse.data_ptr(), counts.data_ptr(), lse.data_ptr() + 4 * M, ptr(g_w), ptr(g_balance), ptr(g_z),
-                      grad.data_ptr())
-        if rc:
-            _gnf4b.check(rc, "gnf4b_route_train_bwd")
-        return grad, None, None, None, None
+        if torch.is_grad_enabled():                 # create_graph=True: the gradient is no graph
+            return _route_backward_once(ctx, g_w, g_balance, g_z)
+        return _route_backward(ctx, g_w, g_balance, g_z)
 
 
+def _route_backward(ctx, g_w, g_balance, g_z):
+    import _gnf4b
+    from nf4_grouped import _call_on
+    logits, token_mask, idx, w, lse, counts = ctx.saved_tensors
+    k, mode, norm = ctx.rule
+    M, E = logits.shape
+    grad = torch.empty((M, E), dtype=logits.dtype, device=logits.device)
+    n_tokens = lse.data_ptr() + 4 * M
+    if g_w is not None:
+        g_w = g_w.contiguous()
+    rc = _call_on(logits.device, _gnf4b.load().gnf4b_route_train_bwd, logits.data_ptr(), _ROUTE_DTYPES[logits.dtype], M,
+                  logits.stride(0) if M > 1 else E, E, k, mode, norm, None if token_mask is None else token_mask.data_ptr(),
+                  idx.data_ptr(), w.data_ptr(), lse.data_ptr(), counts.data_ptr(), n_tokens,
+                  None if g_w is None else g_w.data_ptr(), None if g_balance is None else g_balance.data_ptr(),
+                  None if g_z is None else g_z.data_ptr(), grad.data_ptr())
+    if rc:
+        _gnf4b.check(rc, "gnf4b_route_train_bwd")
+    return grad, None, None, None, None
+
+
+_route_backward_once = torch.autograd.function.once_differentiable(_route_backward)
 _ROUTE_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}        # GNF4B_X_*
 ROUTE_TRAIN_MAX_EXPERTS, ROUTE_TRAIN_MAX_K = 1024, 32
 

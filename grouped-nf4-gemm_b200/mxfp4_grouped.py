@@ -156,35 +156,41 @@ def quantize_mxfp4(x):
     e >= -69 with max|x| <= 6 * 2^e and every element takes the nearest e2m1 value, the lower magnitude on a tie: byte
     for byte what ``mxfp4_pack_ref.quantize_pack_mxfp4`` gives (as ``[..., K//32, 16]``).  A block that holds an
     infinity or a NaN gets the exponent byte 255.  Rows may be a strided view; other layouts are copied first."""
-    _require_cuda(x, "quantize_mxfp4", "The CPU counterpart is mxfp4_pack_ref.quantize_pack_mxfp4.")
-    if x.dtype not in _X_DTYPES:
+    if not x.is_cuda:
+        _require_cuda(x, "quantize_mxfp4", "The CPU counterpart is mxfp4_pack_ref.quantize_pack_mxfp4.")
+    dtype = _X_DTYPES.get(x.dtype)
+    if dtype is None:
         raise TypeError(f"quantize_mxfp4 takes bfloat16, float16 or float32, got {x.dtype}")
-    if x.dim() == 0 or x.shape[-1] == 0 or x.shape[-1] % MX_BLOCK:
-        raise ValueError(f"the last dimension must be a positive multiple of {MX_BLOCK}, got shape {tuple(x.shape)}")
-    K = x.shape[-1]
-    lead = tuple(x.shape[:-1])
-    x = x.detach()
-    if x.dim() != 2 or x.stride(1) != 1:
+    shape = x.shape
+    K = shape[-1] if shape else 0
+    if K == 0 or K % MX_BLOCK:
+        raise ValueError(f"the last dimension must be a positive multiple of {MX_BLOCK}, got shape {tuple(shape)}")
+    if len(shape) != 2:
         x = x.reshape(x.numel() // K, K)
-        if x.stride(1) != 1:
-            x = x.contiguous()
-    blocks = torch.empty(*lead, K // 2, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(*lead, K // MX_BLOCK, dtype=torch.uint8, device=x.device)
-    rc = _call_on(x.device, _gnf4b.load().gnf4b_quantize_mxfp4, x.data_ptr(), _X_DTYPES[x.dtype], x.shape[0], K,
-                  x.stride(0) if x.shape[0] > 1 else K, blocks.data_ptr(), scales.data_ptr())
+    rows = x.shape[0]
+    pitch, unit = x.stride()
+    if unit != 1:
+        x, pitch = x.contiguous(), K
+    dev = x.device
+    blocks = torch.empty((*shape[:-1], K // 2), dtype=torch.uint8, device=dev)
+    scales = torch.empty((*shape[:-1], K // MX_BLOCK), dtype=torch.uint8, device=dev)
+    rc = _call_on(dev, _gnf4b.load().gnf4b_quantize_mxfp4, x.data_ptr(), dtype, rows, K, pitch if rows > 1 else K,
+                  blocks.data_ptr(), scales.data_ptr())
     if rc:
         _gnf4b.check(rc, "gnf4b_quantize_mxfp4")
     return blocks, scales
 
 
 def _check_packed(blocks, scales, what: str):
+    bs, ss = blocks.shape, scales.shape
+    if blocks.dtype is torch.uint8 and scales.dtype is torch.uint8 and len(bs) == len(ss) > 0 and bs[:-1] == ss[:-1] \
+            and bs[-1] == 16 * ss[-1] > 0 and scales.device == blocks.device:
+        return
     if blocks.dtype != torch.uint8 or scales.dtype != torch.uint8:
         raise TypeError(f"{what}: blocks and scales must be uint8, got {blocks.dtype} and {scales.dtype}")
-    if blocks.dim() == 0 or blocks.dim() != scales.dim() or blocks.shape[:-1] != scales.shape[:-1] \
-            or blocks.shape[-1] != 16 * scales.shape[-1] or scales.shape[-1] == 0:
-        raise ValueError(f"{what}: blocks {tuple(blocks.shape)} and scales {tuple(scales.shape)} are not [..., K//2] and [..., K//32]")
     if scales.device != blocks.device:
         raise ValueError(f"{what}: blocks and scales must live on the same device")
+    raise ValueError(f"{what}: blocks {tuple(bs)} and scales {tuple(ss)} are not [..., K//2] and [..., K//32]")
 
 
 def _packed_rows(t, align: int):
@@ -196,12 +202,13 @@ def _packed_rows(t, align: int):
 def dequantize_mxfp4(blocks, scales, dtype=torch.bfloat16):
     """The values of packed rows, ``blocks [..., K//2]`` and ``scales [..., K//32]`` -> ``[..., K]`` in bf16 or fp32
     (exact) or fp16 (rounded once).  An exponent byte of 255 reads as 2^128, as in ``mxfp4_pack_ref.dequant_mxfp4``."""
-    _require_cuda(blocks, "dequantize_mxfp4", "The CPU counterpart is mxfp4_pack_ref.dequant_mxfp4.")
+    if not blocks.is_cuda:
+        _require_cuda(blocks, "dequantize_mxfp4", "The CPU counterpart is mxfp4_pack_ref.dequant_mxfp4.")
     if dtype not in _X_DTYPES:
         raise TypeError(f"dequantize_mxfp4 returns bfloat16, float16 or float32, not {dtype}")
     _check_packed(blocks, scales, "dequantize_mxfp4")
     blocks, scales = _packed_rows(blocks, 4), scales.contiguous()
-    out = torch.empty(*blocks.shape[:-1], 2 * blocks.shape[-1], dtype=dtype, device=blocks.device)
+    out = torch.empty((*blocks.shape[:-1], 2 * blocks.shape[-1]), dtype=dtype, device=blocks.device)
     rc = _call_on(blocks.device, _gnf4b.load().gnf4b_dequantize_mxfp4, blocks.data_ptr(), scales.data_ptr(), scales.numel(),
                   _X_DTYPES[dtype], out.data_ptr())
     if rc:
@@ -247,10 +254,11 @@ def glu_quantize_mxfp4(gate_up, act: str = "silu", bias=None, row_expert=None):
 
 def _tma_ready(blocks):
     """A weight stack as the product's TMA loads take it: 16-byte aligned, positive strides in multiples of 16 bytes."""
-    ok = blocks.stride(2) == 1 and blocks.data_ptr() % 16 == 0
-    for dim in (0, 1):
-        ok = ok and (blocks.shape[dim] == 1 or (blocks.stride(dim) > 0 and blocks.stride(dim) % 16 == 0))
-    return blocks if ok else _packed_rows(blocks, 16)
+    E, N, _ = blocks.shape
+    se, sn, unit = blocks.stride()
+    if unit == 1 and blocks.data_ptr() % 16 == 0 and (E == 1 or (se > 0 and se % 16 == 0)) and (N == 1 or (sn > 0 and sn % 16 == 0)):
+        return blocks
+    return _packed_rows(blocks, 16)
 
 
 def gemm_mxfp4_grouped_w4a4(a_blocks, a_scales, blocks, scales, sizes, expert_ids, *, group_offsets=None, max_rows=None):
@@ -261,36 +269,46 @@ def gemm_mxfp4_grouped_w4a4(a_blocks, a_scales, blocks, scales, sizes, expert_id
     ``blocks [E, N, K//2]`` / ``scales [E, N, K//32]`` and ``sizes``, ``expert_ids``, ``group_offsets``, ``max_rows`` as in
     ``gemm_mxfp4_grouped`` (``max_rows`` only shapes the tiles).  An exponent byte of 255 is NaN here, as in the OCP
     format.  Returns ``[T, N]`` bf16.  A stack whose strides are not positive multiples of 16 bytes is copied first."""
-    _require_cuda(a_blocks, "gemm_mxfp4_grouped_w4a4",
-                  "The CPU-checkable equivalent multiplies mxfp4_pack_ref.dequant_mxfp4 of both operands per group.")
+    if not a_blocks.is_cuda:
+        _require_cuda(a_blocks, "gemm_mxfp4_grouped_w4a4",
+                      "The CPU-checkable equivalent multiplies mxfp4_pack_ref.dequant_mxfp4 of both operands per group.")
     if a_blocks.dim() != 2 or blocks.dim() != 3:
         raise ValueError(f"a_blocks must be [T, K//2] and blocks [E, N, K//2], got {tuple(a_blocks.shape)} and {tuple(blocks.shape)}")
     _check_packed(a_blocks, a_scales, "gemm_mxfp4_grouped_w4a4 (rows)")
     _check_packed(blocks, scales, "gemm_mxfp4_grouped_w4a4 (stack)")
     dev = a_blocks.device
+    T, half = a_blocks.shape
+    E, N, half_w = blocks.shape
     if blocks.device != dev:
         raise ValueError("rows and stack must live on the same device")
-    T, half = a_blocks.shape
-    E, N = blocks.shape[:2]
-    if blocks.shape[2] != half:
-        raise ValueError(f"the rows have K={2 * half} but the stack packs K={2 * blocks.shape[2]}")
-    out = torch.empty(T, N, dtype=torch.bfloat16, device=dev)
+    if half_w != half:
+        raise ValueError(f"the rows have K={2 * half} but the stack packs K={2 * half_w}")
+    out = torch.empty((T, N), dtype=torch.bfloat16, device=dev)
     if T == 0 or N == 0 or E == 0:
         return out
     a_blocks, a_scales, blocks = _packed_rows(a_blocks, 16), a_scales.contiguous(), _tma_ready(blocks)
-    if scales.stride(2) != 1:
+    s_e, s_n, unit = scales.stride()
+    if unit != 1:
         scales = scales.contiguous()
-    with torch.cuda.device(dev):
+        s_e, s_n, _ = scales.stride()
+    w_e, w_n, _ = blocks.stride()
+    prev = torch.cuda.current_device()
+    if dev.index != prev:
+        torch.cuda.set_device(dev)                      # the C library launches on the current device
+    try:
         stream_ptr = _raw_stream(dev)
         off_t, ids_t, G, max_rows = _group_tables(sizes, expert_ids, T, E, dev, group_offsets, max_rows, stream_ptr)
         if G == 0:
             return out
         rc = _gnf4b.load().gnf4b_gemm_grouped_w4a4(
-            a_blocks.data_ptr(), a_scales.data_ptr(), T, blocks.data_ptr(), blocks.stride(0), blocks.stride(1),
-            scales.data_ptr(), scales.stride(0), scales.stride(1), off_t if isinstance(off_t, int) else off_t.data_ptr(),
-            ids_t if isinstance(ids_t, int) else ids_t.data_ptr(), G, E, N, 2 * half, max_rows, out.data_ptr(),
-            _status_ptr(dev), stream_ptr)
-    _gnf4b.check(rc, "gnf4b_gemm_grouped_w4a4")
+            a_blocks.data_ptr(), a_scales.data_ptr(), T, blocks.data_ptr(), w_e, w_n, scales.data_ptr(), s_e, s_n,
+            off_t if isinstance(off_t, int) else off_t.data_ptr(), ids_t if isinstance(ids_t, int) else ids_t.data_ptr(), G, E, N,
+            2 * half, max_rows, out.data_ptr(), _status_ptr(dev), stream_ptr)
+    finally:
+        if dev.index != prev:
+            torch.cuda.set_device(prev)
+    if rc:
+        _gnf4b.check(rc, "gnf4b_gemm_grouped_w4a4")
     return out
 
 

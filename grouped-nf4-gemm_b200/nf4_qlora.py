@@ -225,19 +225,27 @@ class _GluTrain(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
-        import _gnf4b
-        from nf4_grouped import _call_on
-        codes, steps = ctx.saved_tensors
-        grad_out = grad_out.contiguous()
-        rows = codes.shape[0]
-        grad = torch.empty(rows, 2 * ctx.h, dtype=torch.bfloat16, device=codes.device)
-        rc = _call_on(codes.device, _gnf4b.load().gnf4b_glu_ckpt8_bwd, grad_out.data_ptr(), codes.data_ptr(), steps.data_ptr(), rows,
-                      ctx.h, ctx.act, grad.data_ptr())
-        if rc:
-            _gnf4b.check(rc, "gnf4b_glu_ckpt8_bwd")
-        return grad, None, None, None
+        if torch.is_grad_enabled():                 # create_graph=True: the gradient is no graph
+            return _glu_backward_once(ctx, grad_out)
+        return _glu_backward(ctx, grad_out)
+
+
+def _glu_backward(ctx, grad_out):
+    import _gnf4b
+    from nf4_grouped import _call_on
+    codes, steps = ctx.saved_tensors
+    grad_out = grad_out.contiguous()
+    rows = codes.shape[0]
+    grad = torch.empty((rows, 2 * ctx.h), dtype=torch.bfloat16, device=codes.device)
+    rc = _call_on(codes.device, _gnf4b.load().gnf4b_glu_ckpt8_bwd, grad_out.data_ptr(), codes.data_ptr(), steps.data_ptr(), rows,
+                  ctx.h, ctx.act, grad.data_ptr())
+    if rc:
+        _gnf4b.check(rc, "gnf4b_glu_ckpt8_bwd")
+    return grad, None, None, None
+
+
+_glu_backward_once = torch.autograd.function.once_differentiable(_glu_backward)
 
 
 def glu_train(gate_up, act: str = "silu", *, bias=None, row_expert=None):

@@ -204,6 +204,19 @@ def test_routing_partial_gradients_views_and_determinism():
     assert torch.equal(ga, gb)
 
 
+def test_gradients_are_not_differentiable_twice():
+    x = torch.randn(8, 16, device=DEV, requires_grad=True)
+    r = ep_moe.route_topk_train(x, 2)
+    g, = torch.autograd.grad(r.balance_loss, x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+    gu = torch.randn(4, 64, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    out = Q.glu_train(gu)
+    g, = torch.autograd.grad(out, gu, torch.ones_like(out), create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
 def test_routing_under_graphs_and_on_streams():
     x = torch.randn(512, 64, generator=gen(14)).to(DEV).requires_grad_()
     one = torch.ones((), device=DEV)
