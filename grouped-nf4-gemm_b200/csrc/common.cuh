@@ -203,6 +203,20 @@ __device__ __forceinline__ uint16_t f32_to_bf16_bits(float x) {
     return __bfloat16_as_ushort(__float2bfloat16_rn(x));
 }
 
+// Division of 31-bit numbers by a divisor known to the host: n / d = (n * m) >> 32 >> s with m = ceil(2^(32 + s) / d), s the
+// bit length of d - 1 (Granlund and Montgomery, "Division by invariant integers using multiplication"); m < 2^33, its
+// 33rd bit is added by hand.
+struct FastDiv {
+    uint32_t d, m, s;
+    __host__ static FastDiv of(uint32_t d) {
+        FastDiv f{d, 0, 0};
+        while (((uint64_t)1 << f.s) < d) ++f.s;
+        f.m = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << f.s) - d) + d - 1) / d);      // m - 2^32
+        return f;
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, m) + n) >> s; }    // n < 2^31: no overflow
+};
+
 __device__ __forceinline__ float bf16_round(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
 
 __device__ __forceinline__ float silu_f32(float x) { return x / (1.0f + expf(-x)); }

@@ -59,11 +59,13 @@ int gnf4b_dequantize_mxfp4(const uint8_t* blocks, const uint8_t* scales, int64_t
     if (n_blocks > kMaxItems / 4) return GNF4B_ETOOBIG;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
     const int64_t items = n_blocks * 4;
-    const unsigned grid = (unsigned)ceil_div(items, kMxThreads);
     const uint32_t* codes = reinterpret_cast<const uint32_t*>(blocks);
-    const cudaError_t e = out_dtype == GNF4B_X_BF16 ? launch_pdl(mx_dequantize_kernel<0>, grid, (unsigned)kMxThreads, st, codes, scales, items, out)
-                          : out_dtype == GNF4B_X_FP16 ? launch_pdl(mx_dequantize_kernel<1>, grid, (unsigned)kMxThreads, st, codes, scales, items, out)
-                                                      : launch_pdl(mx_dequantize_kernel<2>, grid, (unsigned)kMxThreads, st, codes, scales, items, out);
+    const bool few = items <= 148 * 2048;
+    const unsigned grid = (unsigned)ceil_div(items, few ? kMxThreads : kMxThreads * 4);
+#define GNF4B_DQ(T) (few ? launch_pdl(mx_dequantize_kernel<T, 1>, grid, (unsigned)kMxThreads, st, codes, scales, items, out) \
+                         : launch_pdl(mx_dequantize_kernel<T, 4>, grid, (unsigned)kMxThreads, st, codes, scales, items, out))
+    const cudaError_t e = out_dtype == GNF4B_X_BF16 ? GNF4B_DQ(0) : out_dtype == GNF4B_X_FP16 ? GNF4B_DQ(1) : GNF4B_DQ(2);
+#undef GNF4B_DQ
     return e == cudaSuccess ? GNF4B_OK : cuda_fail(e, "dequantize_mxfp4 launch");
 }
 

@@ -143,17 +143,25 @@ int gnf4b_glu_ckpt8_fwd(const void* gate_up, int64_t rows, int64_t h, int act, c
     if (rows == 0) return GNF4B_OK;
     if (!gate_up || !out || !aligned(gate_up, 2) || !aligned(out, 2) || !aligned(codes, 8) || !aligned(steps, 8)) return GNF4B_EINVAL;
     const int64_t nb = ceil_div(h, kCkBlock);
-    if (h > (int64_t)1 << 40 || rows > (int64_t)INT32_MAX * kCkThreads / 8 / nb) return GNF4B_ETOOBIG;
-    const unsigned grid = (unsigned)ceil_div(rows * nb * 8, kCkThreads);
+    if (h > INT32_MAX / 4 || rows > INT32_MAX / nb) return GNF4B_ETOOBIG;       // block numbers of 31 bits
+    const uint32_t blocks = (uint32_t)(rows * nb);
+    const unsigned grid = (unsigned)ceil_div(blocks, kCkThreads / 8);
     const bool vec = h % 8 == 0 && aligned(gate_up, 16) && aligned(out, 16);
     const bool keep = codes != nullptr;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
     cudaError_t e;
-#define GNF4B_CK(A, V, K) launch_pdl(glu_ckpt8_fwd_kernel<A, V, K>, grid, (unsigned)kCkThreads, st, static_cast<const uint16_t*>(gate_up), rows, h, \
-        static_cast<const uint16_t*>(bias), row_expert, E, static_cast<uint16_t*>(out), reinterpret_cast<uint2*>(codes), \
-        reinterpret_cast<float2*>(steps), status_word)
-    if (act == GNF4B_ACT_SILU_GLU) e = keep ? (vec ? GNF4B_CK(0, true, true) : GNF4B_CK(0, false, true)) : (vec ? GNF4B_CK(0, true, false) : GNF4B_CK(0, false, false));
-    else e = keep ? (vec ? GNF4B_CK(1, true, true) : GNF4B_CK(1, false, true)) : (vec ? GNF4B_CK(1, true, false) : GNF4B_CK(1, false, false));
+#define GNF4B_CK(A, V, K, B) launch_pdl(glu_ckpt8_fwd_kernel<A, V, K, B>, grid, (unsigned)kCkThreads, st, static_cast<const uint16_t*>(gate_up), \
+        blocks, FastDiv::of((uint32_t)nb), (int)h, static_cast<const uint16_t*>(bias), row_expert, E, static_cast<uint16_t*>(out), \
+        reinterpret_cast<uint2*>(codes), reinterpret_cast<float2*>(steps), status_word)
+    if (act == GNF4B_ACT_SILU_GLU)
+        e = keep ? (vec ? GNF4B_CK(0, true, true, false) : GNF4B_CK(0, false, true, false))
+                 : (vec ? GNF4B_CK(0, true, false, false) : GNF4B_CK(0, false, false, false));
+    else if (bias)
+        e = keep ? (vec ? GNF4B_CK(1, true, true, true) : GNF4B_CK(1, false, true, true))
+                 : (vec ? GNF4B_CK(1, true, false, true) : GNF4B_CK(1, false, false, true));
+    else
+        e = keep ? (vec ? GNF4B_CK(1, true, true, false) : GNF4B_CK(1, false, true, false))
+                 : (vec ? GNF4B_CK(1, true, false, false) : GNF4B_CK(1, false, false, false));
 #undef GNF4B_CK
     return e == cudaSuccess ? GNF4B_OK : cuda_fail(e, "glu_ckpt8_fwd launch");
 }
@@ -167,13 +175,15 @@ int gnf4b_glu_ckpt8_bwd(const void* grad_out, const int8_t* codes, const float* 
         !aligned(steps, 8))
         return GNF4B_EINVAL;
     const int64_t nb = ceil_div(h, kCkBlock);
-    if (h > (int64_t)1 << 40 || rows > (int64_t)INT32_MAX * kCkThreads / 8 / nb) return GNF4B_ETOOBIG;
-    const unsigned grid = (unsigned)ceil_div(rows * nb * 8, kCkThreads);
+    if (h > INT32_MAX / 4 || rows > INT32_MAX / nb) return GNF4B_ETOOBIG;
+    const uint32_t blocks = (uint32_t)(rows * nb);
+    const unsigned grid = (unsigned)ceil_div(blocks, kCkThreads / 8);
     const bool vec = h % 8 == 0 && aligned(grad_out, 16) && aligned(grad_gate_up, 16);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
     cudaError_t e;
 #define GNF4B_CK(A, V) launch_pdl(glu_ckpt8_bwd_kernel<A, V>, grid, (unsigned)kCkThreads, st, static_cast<const uint16_t*>(grad_out), \
-        reinterpret_cast<const uint2*>(codes), reinterpret_cast<const float2*>(steps), rows, h, static_cast<uint16_t*>(grad_gate_up))
+        reinterpret_cast<const uint2*>(codes), reinterpret_cast<const float2*>(steps), blocks, FastDiv::of((uint32_t)nb), (int)h, \
+        static_cast<uint16_t*>(grad_gate_up))
     if (act == GNF4B_ACT_SILU_GLU) e = vec ? GNF4B_CK(0, true) : GNF4B_CK(0, false);
     else e = vec ? GNF4B_CK(1, true) : GNF4B_CK(1, false);
 #undef GNF4B_CK

@@ -167,38 +167,48 @@ __device__ __forceinline__ float2 e2m1x2_to_float2(uint32_t byte) {
 
 // items of eight elements -> OT (0 bf16, 1 fp16, 2 fp32), contiguous.  Exact in bf16 and fp32; the exponent byte 255
 // reads as 2^128 (a zero stays zero), as everywhere in this library but in the product of two MXFP4 operands.
-template <int OT>
+template <int OT, int U>
 __global__ void __launch_bounds__(kMxThreads)
 mx_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t items, void* __restrict__ out) {
     pdl_wait();
     pdl_launch_dependents();
-    const int64_t i = (int64_t)blockIdx.x * kMxThreads + threadIdx.x;
-    if (i >= items) return;
-    const uint32_t c = __ldcs(codes + i);
-    const float sc = load_scale<GNF4B_S_E8M0>(scales, i >> 2);
-    float f[8];
+    const int64_t first = (int64_t)blockIdx.x * (kMxThreads * U) + threadIdx.x;
+    uint32_t c[U];
+    float sc[U];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float2 p = e2m1x2_to_float2((c >> (8 * j)) & 0xffu);
-        f[2 * j] = __fmul_rn(p.x + p.x, sc);
-        f[2 * j + 1] = __fmul_rn(p.y + p.y, sc);
+    for (int k = 0; k < U; ++k) {
+        const int64_t i = first + k * kMxThreads;
+        c[k] = i < items ? __ldcs(codes + i) : 0u;
+        sc[k] = i < items ? load_scale<GNF4B_S_E8M0>(scales, i >> 2) : 0.f;
     }
-    if (OT == 2) {
-        float4* o = static_cast<float4*>(out) + 2 * i;
-        __stcs(o, make_float4(f[0], f[1], f[2], f[3]));
-        __stcs(o + 1, make_float4(f[4], f[5], f[6], f[7]));
-    } else {
-        uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+        const int64_t i = first + k * kMxThreads;
+        if (i >= items) break;
+        float f[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            if (OT == 0) {
-                w[j] = (uint32_t)f32_to_bf16_bits(f[2 * j]) | ((uint32_t)f32_to_bf16_bits(f[2 * j + 1]) << 16);
-            } else {
-                const __half2 h = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
-                w[j] = *reinterpret_cast<const uint32_t*>(&h);
-            }
+            const float2 p = e2m1x2_to_float2((c[k] >> (8 * j)) & 0xffu);
+            f[2 * j] = __fmul_rn(p.x + p.x, sc[k]);
+            f[2 * j + 1] = __fmul_rn(p.y + p.y, sc[k]);
         }
-        __stcs(static_cast<uint4*>(out) + i, make_uint4(w[0], w[1], w[2], w[3]));
+        if (OT == 2) {
+            float4* o = static_cast<float4*>(out) + 2 * i;
+            __stcs(o, make_float4(f[0], f[1], f[2], f[3]));
+            __stcs(o + 1, make_float4(f[4], f[5], f[6], f[7]));
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (OT == 0) {
+                    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[j]) : "f"(f[2 * j + 1]), "f"(f[2 * j]));
+                } else {
+                    const __half2 h = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+                    w[j] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+            }
+            __stcs(static_cast<uint4*>(out) + i, make_uint4(w[0], w[1], w[2], w[3]));
+        }
     }
 }
 
