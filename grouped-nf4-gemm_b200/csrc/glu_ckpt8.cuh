@@ -255,7 +255,7 @@ glu_ckpt8_bwd_kernel(const uint16_t* __restrict__ grad, const uint2* __restrict_
             const float gc = min_nan(g[j], 7.0f), uc = max_nan(min_nan(u[j], 7.0f), -7.0f);
             const float s = ck_sigmoid2(gc * (-kCkAlpha * kCkLog2e)), gs = go[j] * s;
             const float dg = gs * (uc + 1.0f) * fmaf(kCkAlpha * gc, 1.0f - s, 1.0f);
-            u[j] = uc != u[j] && u[j] == u[j] ? 0.f : gs * gc;         // beyond a clamp: no gradient (a NaN is not beyond)
+            u[j] = fabsf(u[j]) > 7.0f ? 0.f : gs * gc;      // beyond a clamp: no gradient (a NaN is not beyond)
             g[j] = g[j] > 7.0f ? 0.f : dg;
         }
     }
