@@ -128,7 +128,7 @@ int gnf4b_gemm_grouped_w4a4(const uint8_t* x_blocks, const uint8_t* x_scales, in
     a.K = K;
     a.E = E;
     a.rows_w = p.rows_w;
-    a.n_tiles = (int32_t)ceil_div(N, p.rows_w);
+    a.n_tiles = (int32_t)ceil_div(N, p.pair ? 256 : p.rows_w);
     a.k_stages = (int32_t)ceil_div(K, kQStageK);
     a.tok_cap = p.tok_cap;
     a.xbox = p.xbox;
@@ -157,15 +157,29 @@ int gnf4b_gemm_grouped_w4a4(const uint8_t* x_blocks, const uint8_t* x_scales, in
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return GNF4B_EUNSUPPORTED;
     }
-    static int granted[64];
-    cudaError_t e = ensure_smem(w4a4_kernel, p.smem, granted);
+    static int granted[64], granted_pair[64];
+    cudaError_t e = p.pair ? ensure_smem(w4a4_kernel<2>, p.smem, granted_pair) : ensure_smem(w4a4_kernel<1>, p.smem, granted);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(w4a4)");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.pair ? di.sm_count & ~1 : di.sm_count));
+    cfg.blockDim = dim3(kQThreads);
+    cfg.dynamicSmemBytes = p.smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.pair ? 2 : 1;
     // a launch's group table lives in shared memory: longer lists take several launches (the offsets are absolute)
     for (int32_t g0 = 0; g0 < G; g0 += kQMaxGroups) {
         a.off = group_offsets + g0;
         a.eids = expert_ids + g0;
         a.G = std::min<int32_t>(kQMaxGroups, G - g0);
-        e = launch_pdl_smem(w4a4_kernel, (unsigned)di.sm_count, (unsigned)kQThreads, p.smem, st, a, x_map, w_map);
+        e = p.pair ? cudaLaunchKernelEx(&cfg, w4a4_kernel<2>, a, x_map, w_map) : cudaLaunchKernelEx(&cfg, w4a4_kernel<1>, a, x_map, w_map);
         if (e != cudaSuccess) return cuda_fail(e, "w4a4 launch");
     }
     return GNF4B_OK;

@@ -20,12 +20,19 @@
 //               cannot come by TMA
 //   warps 8-15  epilogue, two per TMEM lane quarter taking alternate 32-token chunks, as in tensor_fwd_kernel.cuh
 //
+// CG = 2 (long groups): a cluster of two CTAs shares every item -- same rows, neighbouring weight tiles, 256 x 256
+// multiplied by one tcgen05.mma.cta_group::2 that the leader issues.  Each CTA loads its own weight tile and half of the
+// activation rows, 32 KiB a stage instead of 48 for the same product: what bounds long groups is L2 -> shared memory
+// (about 47 bytes per cycle and SM).  Each keeps the scales of its weight rows and of all activation rows; the leader's
+// tcgen05.cp.cta_group::2 copies both CTAs' into their own tensor memory.  The peer's MMA warp forwards "my tiles have
+// landed" to the leader; completions are committed to both.
+//
 // Work item = (group, balanced chunk of <= tok_cap rows, rows_w weight rows), weight tile fastest.  With few rows per
 // group the kernel streams weights and rows_w < 128 evens out the items over the SMs (the MMA still multiplies 128
 // lanes; the lanes above rows_w hold stale bytes with zero scales and are not read back).
 #pragma once
 
-#include "tensor_kernel.cuh"
+#include "tensor_fwd_kernel.cuh"
 
 namespace gnf4b {
 
@@ -52,9 +59,9 @@ struct W4A4Args {
     int64_t T, N, K;
     int32_t G, E;
     int32_t rows_w;             // weight rows per item, a multiple of 8, <= 128
-    int32_t n_tiles;            // ceil(N / rows_w)
+    int32_t n_tiles;            // items per chunk: ceil(N / rows_w), in a pair ceil(N / 256)
     int32_t k_stages;           // ceil(K / 256)
-    int32_t tok_cap;            // activation rows per item, a multiple of 16, <= 256
+    int32_t tok_cap;            // activation rows per item, a multiple of 16 (in a pair 32), <= 256
     int32_t xbox;               // activation rows per TMA box
     int32_t x_bytes;            // shared memory of a stage's activations, whole boxes
     int32_t stages;
@@ -101,10 +108,58 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
 __device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
     return (uint64_t)((smem_addr >> 4) & 0x3fffu) | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
 }
-// kind::mxf4 instruction descriptor: e2m1 x e2m1, both K-major, e8m0 scales, M = 128; the byte pair of the 4-byte
+// kind::mxf4 instruction descriptor: e2m1 x e2m1, both K-major, e8m0 scales, M = m; the byte pair of the 4-byte
 // scale words that belongs to this instruction's 64 elements is 0 or 2
-__device__ __forceinline__ uint32_t mxf4_idesc(uint32_t n_umma, uint32_t sf_id) {
-    return (sf_id << 4) | (1u << 7) | (1u << 10) | ((n_umma >> 3) << 17) | (1u << 23) | (8u << 24) | (sf_id << 29);
+__device__ __forceinline__ uint32_t mxf4_idesc(uint32_t m, uint32_t n_umma, uint32_t sf_id) {
+    return (sf_id << 4) | (1u << 7) | (1u << 10) | ((n_umma >> 3) << 17) | (1u << 23) | ((m >> 4) << 24) | (sf_id << 29);
+}
+
+// ---- the same over a CTA pair
+__device__ __forceinline__ void tc_mma_mxf4_2(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa,
+                                              uint32_t sfb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tc_cp_scales_2(uint32_t taddr, uint64_t s_desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(s_desc) : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_2(uint32_t* dst_smem, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_2(uint32_t addr, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+}
+// arrive on a barrier of the cluster and publish what this thread wrote (the scales)
+__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void q_mma(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    if (CG == 2) tc_mma_mxf4_2(d, ad, bd, idesc, sfa, sfb, accumulate);
+    else tc_mma_mxf4(d, ad, bd, idesc, sfa, sfb, accumulate);
+}
+template <int CG>
+__device__ __forceinline__ void q_cp(uint32_t taddr, uint64_t s_desc) {
+    if (CG == 2) tc_cp_scales_2(taddr, s_desc);
+    else tc_cp_scales(taddr, s_desc);
+}
+// commit to this CTA's barrier, in a pair to the peer's too (peer_off: its shared::cluster address minus this one's)
+template <int CG>
+__device__ __forceinline__ void q_commit(uint64_t* bar, uint32_t peer_base, uint32_t own_base) {
+    if (CG == 2) {
+        tc_commit2(smem_u32(bar));
+        tc_commit2(peer_base + (smem_u32(bar) - own_base));
+    } else {
+        tc_commit(bar);
+    }
+}
+template <int CG>
+__device__ __forceinline__ bool q_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    return CG == 2 ? mbar_wait_bounded_cluster(bar, parity, abort_flag) : mbar_wait_bounded(bar, parity, abort_flag);
 }
 
 // one lane of the warp, always the same one
@@ -126,16 +181,17 @@ struct QItem {
     int32_t row0, tokens, eid, n0;
 };
 
-__device__ __forceinline__ bool next_qitem(const W4A4Args& a, const QTable& tb, int32_t& g, uint32_t id, QItem* it) {
+__device__ __forceinline__ bool next_qitem(const W4A4Args& a, const QTable& tb, int32_t& g, uint32_t id, QItem* it, int32_t tile_rows,
+                                           int32_t tile_first) {
     while (g < a.G && id >= tb.base[g + 1]) ++g;
     if (g >= a.G) return false;
     const QGroup gr = tb.grp[g];
     const uint32_t local = id - tb.base[g];
-    const uint32_t mc = local / (uint32_t)a.n_tiles;
+    const uint32_t mc = local / (uint32_t)a.n_tiles;       // n0: of the item; a pair's second CTA adds 128
     it->row0 = gr.row0 + (int32_t)mc * gr.chunk_rows;
     it->tokens = min(gr.chunk_rows, gr.row0 + gr.rows - it->row0);
     it->eid = gr.eid;
-    it->n0 = (int32_t)(local - mc * (uint32_t)a.n_tiles) * a.rows_w;
+    it->n0 = (int32_t)(local - mc * (uint32_t)a.n_tiles) * tile_rows + tile_first;
     return true;
 }
 
@@ -234,6 +290,7 @@ __device__ __forceinline__ void align_scale_row(const uint32_t* raw, uint32_t at
     }
 }
 
+template <int CG>
 __global__ void __launch_bounds__(kQThreads, 1)
 w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map) {
     extern __shared__ uint8_t smem_raw[];
@@ -254,38 +311,50 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
     uint64_t* acc_empty = acc_full + 2;
     uint64_t* sc_full = acc_empty + 2;
     uint64_t* sc_done = sc_full + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sc_done + 2);
+    uint64_t* landed = sc_done + 2;                        // the peer's own tiles, forwarded to the leader's full[]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(landed + kQMaxStages);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = uniform(threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     const uint32_t stages = (uint32_t)a.stages;
+    const uint32_t rank = CG == 2 ? (uint32_t)uniform((int)cluster_ctarank()) : 0u;
+    const uint32_t worker = CG == 2 ? blockIdx.x >> 1 : blockIdx.x, workers = CG == 2 ? gridDim.x >> 1 : gridDim.x;
+    const int32_t tile_rows = CG == 2 ? 256 : a.rows_w, tile_first = (int32_t)rank * 128;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kQMaxStages; ++s) {
-            mbar_init(full + s, 1);
+            mbar_init(full + s, CG);
             mbar_init(done + s, 1);
+            mbar_init(landed + s, 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full + b, 1);
-            mbar_init(acc_empty + b, kQEpiWarps);
-            mbar_init(sc_full + b, kQScaleWarps);
+            mbar_init(acc_empty + b, kQEpiWarps * CG);
+            mbar_init(sc_full + b, kQScaleWarps * CG);
             mbar_init(sc_done + b, 1);
         }
         *abort_flag = 0;
         fence_barrier_init();
     }
     if (warp == 1) {
-        tmem_alloc(tmem_slot, kQTmemCols);
-        tmem_relinquish();
+        if (CG == 2) {
+            tmem_alloc_2(tmem_slot, kQTmemCols);
+        } else {
+            tmem_alloc(tmem_slot, kQTmemCols);
+            tmem_relinquish();
+        }
     }
     pdl_wait();                      // group tables, operands and the output belong to earlier kernels until here
     pdl_launch_dependents();         // not before: a successor may read, ahead of its own wait, what OUR predecessor wrote
     build_qtable(a, s_grp, s_base, s_wtot);
     const QTable tb{s_grp, s_base};
     tc_fence_before();
-    __syncthreads();
+    if (CG == 2) cluster_sync_all();      // the peer's barriers exist before anything arrives on them
+    else __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    const uint32_t own_base = smem_u32(full);
+    const uint32_t leader_base = CG == 2 ? map_to_cta(own_base, 0) : 0u, peer_base = CG == 2 ? map_to_cta(own_base, 1) : 0u;
     const uint32_t tmem_sf0 = tmem_base + (uint32_t)(a.acc_bufs * a.tok_cap);      // scale slots behind the accumulators
     const uint32_t slot_cols = 8u * (1u + (uint32_t)a.x_blocks);
 
@@ -297,10 +366,13 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
         // ------------------------------------------------------------ TMA producer
         int32_t g = 0;
         QItem it;
-        uint32_t s = 0, phase = 0, id = blockIdx.x;
-        while (__all_sync(0xffffffffu, next_qitem(a, tb, g, id, &it))) {
-            const int row0 = uniform(it.row0), n0 = uniform(it.n0), eid = uniform(it.eid);
-            const int boxes = (uniform(it.tokens) + a.xbox - 1) / a.xbox;
+        uint32_t s = 0, phase = 0, id = worker;
+        while (__all_sync(0xffffffffu, next_qitem(a, tb, g, id, &it, tile_rows, tile_first))) {
+            // a pair's CTA loads half of the MMA's rows (32 and its multiples, so that a half is a multiple of 16)
+            const int half = CG == 2 ? ((uniform(it.tokens) + 31) & ~31) >> 1 : 0;
+            const int row0 = uniform(it.row0) + (CG == 2 ? (int)rank * half : 0), n0 = uniform(it.n0), eid = uniform(it.eid);
+            const int boxes = ((CG == 2 ? half : uniform(it.tokens)) + a.xbox - 1) / a.xbox;
+            uint64_t* const bars = CG == 2 && rank == 1 ? landed : full;
             const uint32_t bytes = (uint32_t)((a.rows_w + boxes * a.xbox) * kQRowBytes);
             bool ok = true;
             for (int rb = 0; rb < a.k_stages; ++rb) {
@@ -308,37 +380,53 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
                 if (!ok) break;
                 if (elect_one()) {
                     uint8_t* st = smem + (size_t)s * tile_bytes;
-                    mbar_arrive_expect_tx(full + s, bytes);
-                    tma_load_3d(st, &w_map, rb * kQRowBytes, n0, eid, full + s);
+                    mbar_arrive_expect_tx(bars + s, bytes);
+                    tma_load_3d(st, &w_map, rb * kQRowBytes, n0, eid, bars + s);
                     for (int b = 0; b < boxes; ++b)
-                        tma_load_2d(st + kQWTile + b * a.xbox * kQRowBytes, &x_map, rb * kQRowBytes, row0 + b * a.xbox, full + s);
+                        tma_load_2d(st + kQWTile + b * a.xbox * kQRowBytes, &x_map, rb * kQRowBytes, row0 + b * a.xbox, bars + s);
                 }
                 if (++s == stages) { s = 0; phase ^= 1; }
             }
             if (!ok) break;
-            id += gridDim.x;
+            id += workers;
+        }
+    } else if (warp == 1 && rank == 1) {
+        // ------------------------------------------------------------ the pair's second CTA: tiles landed -> leader
+        int32_t g = 0;
+        QItem it;
+        uint32_t s = 0, phase = 0, id = worker;
+        while (__all_sync(0xffffffffu, next_qitem(a, tb, g, id, &it, tile_rows, tile_first))) {
+            bool ok = true;
+            for (int rb = 0; rb < a.k_stages; ++rb) {
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(landed + s, phase, abort_flag));
+                if (!ok) break;
+                if (lane == 0) mbar_arrive_cluster(leader_base + s * 8);
+                if (++s == stages) { s = 0; phase ^= 1; }
+            }
+            if (!ok) break;
+            id += workers;
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer
         int32_t g = 0;
         QItem it;
-        uint32_t s = 0, phase = 0, buf = 0, acc_phase = 0, sp = 0, sp_phase = 0, id = blockIdx.x;
+        uint32_t s = 0, phase = 0, buf = 0, acc_phase = 0, sp = 0, sp_phase = 0, id = worker;
         const uint32_t half_cols = 4u * (1u + (uint32_t)a.x_blocks);
         const uint64_t w_desc0 = umma_desc(smem_u32(smem), 16, 1024), sc_desc0 = scale_desc(smem_u32(s_scale));
         const uint32_t tile_step = (uint32_t)tile_bytes >> 4, half_step = (uint32_t)half_bytes >> 4, span_step = (uint32_t)span_bytes >> 4;
         const int tail = (int)((a.K - (int64_t)(a.k_stages - 1) * kQStageK + 63) >> 6);   // 64-element steps of the last stage
-        while (__all_sync(0xffffffffu, next_qitem(a, tb, g, id, &it))) {
+        while (__all_sync(0xffffffffu, next_qitem(a, tb, g, id, &it, tile_rows, tile_first))) {
             const uint32_t tokens = (uint32_t)uniform(it.tokens);
-            const uint32_t n_umma = (tokens + 15u) & ~15u;
-            const uint32_t id0 = mxf4_idesc(n_umma, 0), id2 = mxf4_idesc(n_umma, 2);
+            const uint32_t n_umma = CG == 2 ? (tokens + 31u) & ~31u : (tokens + 15u) & ~15u;
+            const uint32_t id0 = mxf4_idesc(128 * CG, n_umma, 0), id2 = mxf4_idesc(128 * CG, n_umma, 2);
             const bool two = tokens > 128u;
             const uint32_t acc = tmem_base + buf * (uint32_t)a.tok_cap;
-            bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(acc_empty + buf, acc_phase ^ 1, abort_flag));
+            bool ok = __all_sync(0xffffffffu, q_wait<CG>(acc_empty + buf, acc_phase ^ 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
             for (int rb = 0; rb < a.k_stages; ++rb) {
-                if ((rb & 3) == 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(sc_full + sp, sp_phase, abort_flag));
-                ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(full + s, phase, abort_flag));
+                if ((rb & 3) == 0) ok = __all_sync(0xffffffffu, q_wait<CG>(sc_full + sp, sp_phase, abort_flag));
+                ok = __all_sync(0xffffffffu, ok && q_wait<CG>(full + s, phase, abort_flag));
                 if (!ok) break;
                 tc_fence_after();
                 const bool last = rb + 1 == a.k_stages;
@@ -348,28 +436,28 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
                 const uint64_t src = sc_desc0 + sp * span_step + (uint32_t)(rb & 3) * (2 * half_step);
                 const uint32_t sf = tmem_sf0 + s * slot_cols, sf1 = sf + half_cols;
                 if (elect_one()) {
-                    tc_cp_scales(sf, src);
-                    tc_cp_scales(sf + 4, src + (512 >> 4));
-                    if (two) tc_cp_scales(sf + 8, src + (1024 >> 4));
-                    tc_mma_mxf4(acc, da, db, id0, sf, sf + 4, rb > 0 ? 1u : 0u);
-                    if (steps > 1) tc_mma_mxf4(acc, da + 2, db + 2, id2, sf, sf + 4, 1u);
+                    q_cp<CG>(sf, src);
+                    q_cp<CG>(sf + 4, src + (512 >> 4));
+                    if (two) q_cp<CG>(sf + 8, src + (1024 >> 4));
+                    q_mma<CG>(acc, da, db, id0, sf, sf + 4, rb > 0 ? 1u : 0u);
+                    if (steps > 1) q_mma<CG>(acc, da + 2, db + 2, id2, sf, sf + 4, 1u);
                     if (steps > 2) {
-                        tc_cp_scales(sf1, src + half_step);
-                        tc_cp_scales(sf1 + 4, src + half_step + (512 >> 4));
-                        if (two) tc_cp_scales(sf1 + 8, src + half_step + (1024 >> 4));
-                        tc_mma_mxf4(acc, da + 4, db + 4, id0, sf1, sf1 + 4, 1u);
-                        if (steps > 3) tc_mma_mxf4(acc, da + 6, db + 6, id2, sf1, sf1 + 4, 1u);
+                        q_cp<CG>(sf1, src + half_step);
+                        q_cp<CG>(sf1 + 4, src + half_step + (512 >> 4));
+                        if (two) q_cp<CG>(sf1 + 8, src + half_step + (1024 >> 4));
+                        q_mma<CG>(acc, da + 4, db + 4, id0, sf1, sf1 + 4, 1u);
+                        if (steps > 3) q_mma<CG>(acc, da + 6, db + 6, id2, sf1, sf1 + 4, 1u);
                     }
-                    tc_commit(done + s);
-                    if (span_end) tc_commit(sc_done + sp);
-                    if (last) tc_commit(acc_full + buf);
+                    q_commit<CG>(done + s, peer_base, own_base);
+                    if (span_end) q_commit<CG>(sc_done + sp, peer_base, own_base);
+                    if (last) q_commit<CG>(acc_full + buf, peer_base, own_base);
                 }
                 if (++s == stages) { s = 0; phase ^= 1; }
                 if (span_end) { sp ^= 1; sp_phase ^= sp ^ 1; }
             }
             if (!ok) break;
             if (++buf == (uint32_t)a.acc_bufs) { buf = 0; acc_phase ^= 1; }
-            id += gridDim.x;
+            id += workers;
         }
     } else if (warp < kQEpiWarp0) {
         // ------------------------------------------------------------ scales: global -> registers -> shared memory
@@ -383,8 +471,8 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
         const int spans = (a.k_stages + 3) >> 2;
         int32_t g = 0;
         QItem it;
-        uint32_t id = blockIdx.x;
-        bool have = next_qitem(a, tb, g, id, &it);
+        uint32_t id = worker;
+        bool have = next_qitem(a, tb, g, id, &it, tile_rows, tile_first);
         int sp = 0;
         // the next span of this CTA's items; returns its bytes per row (0: none), one bit in `live` per existing row
         auto fetch = [&](uint32_t (&raw)[2][12], uint32_t (&at)[2], uint32_t& live) -> int {
@@ -405,8 +493,8 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
             }
             if (++sp == spans) {
                 sp = 0;
-                id += gridDim.x;
-                have = next_qitem(a, tb, g, id, &it);
+                id += workers;
+                have = next_qitem(a, tb, g, id, &it, tile_rows, tile_first);
             }
             return valid;
         };
@@ -429,7 +517,10 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
             }
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(sc_full + slot);
+            if (lane == 0) {
+                if (CG == 2) mbar_arrive_release_cluster(leader_base + (smem_u32(sc_full + slot) - own_base));
+                else mbar_arrive(sc_full + slot);
+            }
             slot ^= 1;
             phase ^= slot ^ 1;
         }
@@ -442,7 +533,7 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
         uint32_t buf = 0, acc_phase = 0;
         bool ok = true;
         const bool pair_ok = (a.N % 2) == 0;
-        for (uint32_t id = blockIdx.x; ok && next_qitem(a, tb, g, id, &it); id += gridDim.x) {
+        for (uint32_t id = worker; ok && next_qitem(a, tb, g, id, &it, tile_rows, tile_first); id += workers) {
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(acc_full + buf, acc_phase, abort_flag));
             if (!ok) break;
             tc_fence_after();
@@ -453,7 +544,10 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
             auto release_acc = [&]() {
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(acc_empty + buf);
+                if (lane == 0) {
+                    if (CG == 2) mbar_arrive_cluster(leader_base + (smem_u32(acc_empty + buf) - own_base));
+                    else mbar_arrive(acc_empty + buf);
+                }
             };
             if (e >= chunks) release_acc();              // nothing to drain for this warp
             // everything this warp drains is packed into registers first, so that the accumulator is free for the next
@@ -507,7 +601,9 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
     // ---------------------------------------------------------------- teardown
     __syncwarp();
     tc_fence_before();
-    __syncthreads();
+    // in a pair neither CTA may free its tensor memory or leave while the other's MMAs and arrivals can reach it
+    if (CG == 2) cluster_sync_all();
+    else __syncthreads();
     if (*abort_flag) {               // a wait gave up: give the copies in flight time to land before the memory goes
         const long long t0 = clock64();
         while (clock64() - t0 < 20000000ll) {
@@ -517,13 +613,18 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
     if (warp == 1) {
         __syncwarp();
         tc_fence_after();
-        tmem_dealloc(tmem_base, kQTmemCols);
+        if (CG == 2) tmem_dealloc_2(tmem_base, kQTmemCols);
+        else tmem_dealloc(tmem_base, kQTmemCols);
     }
     if (threadIdx.x == 0 && *abort_flag && a.status) atomicOr(a.status, GNF4B_ST_TIMEOUT);
 }
 
+// Groups this long run as CTA pairs
+constexpr int kQPairRows = 128;
+
 struct W4A4Plan {
     int rows_w, tok_cap, xbox, x_bytes, x_blocks, stages, acc_bufs;
+    int pair;           // CTA pairs
     size_t smem;
 };
 
@@ -545,6 +646,12 @@ static inline W4A4Plan w4a4_plan(int64_t T, int32_t G, int64_t N, int64_t K, int
             const double cost = (double)rounds * ((double)r * (double)K * (17.0 / 32.0) + 9000.0);
             if (cost < best) { best = cost; p.rows_w = r; }
         }
+    }
+    p.pair = longest >= kQPairRows;
+    if (p.pair) {
+        p.tok_cap = (int)round_up(p.tok_cap, 32);
+        p.xbox = 64;
+        p.x_bytes = (int)round_up(p.tok_cap / 2, p.xbox) * kQRowBytes;
     }
     const size_t room = (size_t)smem_optin - w4a4_fixed_bytes(p.x_blocks);
     p.stages = (int)(room / (size_t)(kQWTile + p.x_bytes));

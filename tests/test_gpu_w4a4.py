@@ -198,6 +198,25 @@ def test_product_group_sizes(sizes):
     check_product(out, ref, mags, K)
 
 
+@pytest.mark.parametrize("rows", [3, 20, 100, 190])
+def test_product_many_items_per_sm(rows):
+    """Several items, several turns of the stage ring and of the scale ring on every SM (and SM pair, from 128 rows on),
+    an odd number of tiles."""
+    G, E, K = 40, 6, 2080
+    N = 1200 if rows > 50 else 5000
+    sizes = [rows + (7 * i) % 90 if rows > 50 else rows for i in range(G)]
+    ids = [(5 * i) % E for i in range(G)]
+    wb, ws = packed((E, N), K, 40)
+    xb, xs = packed((sum(sizes),), K, 41)
+    out = M.gemm_mxfp4_grouped_w4a4(xb, xs, wb, ws, sizes, ids)
+    w, m = ([values64(b, ws[e]).to(DEV) for e, b in enumerate(v)] for v in (wb, wb & 0x77))
+    x, a = (values64(v, xs).to(DEV).split(sizes) for v in (xb, xb & 0x77))
+    ref = torch.cat([v @ w[e].t() for v, e in zip(x, ids)]).cpu()
+    mags = torch.cat([v @ m[e].t() for v, e in zip(a, ids)]).cpu()
+    check_product(out, ref, mags, K)
+    assert nf4_grouped.last_status(DEV) == 0
+
+
 @pytest.mark.parametrize("max_rows", [None, 1, 7, 40, 300])
 def test_product_device_tables_and_row_hints(max_rows):
     """max_rows shapes the tiles only: unknown, understated and overstated give the same bits."""
