@@ -14,10 +14,12 @@
 //   warp 1      MMA issuer (one lane): tcgen05.cp of the stage's scales shared memory -> tensor memory (32 lanes
 //               x 16 bytes, replicated to the four lane quarters), then up to four MMAs of 64 elements
 //   warps 2-7   scales, a span of 1024 elements (32 exponent bytes a row, four stages) at a time in a ring of two: every
-//               thread has two of the 128 + 256 rows and reads a row's 32 bytes with two or three 16-byte loads, those of
-//               the next span in flight while a span is written as the 4-byte words of 128 elements that tcgen05.cp
-//               takes (row r at (r % 32) * 16 + (r / 32) * 4).  Scale rows have any pitch (gpt-oss: 90 bytes), so they
-//               cannot come by TMA
+//               thread has two of the 128 + 256 rows and reads a row's 32 bytes with two 16-byte loads (three where rows
+//               do not start on 16 bytes: gpt-oss has 90 bytes a row, which is also why they cannot come by TMA), those
+//               of the next span in flight while a span is written as the 4-byte words of 128 elements that tcgen05.cp
+//               takes (row r at (r % 32) * 16 + (r / 32) * 4; a warp's 32 rows are eight of each quarter, so that no two
+//               lanes share a bank).  What counts here is the number of instructions: a warp issues one every five or six
+//               cycles, and all of a span's have to fit the 2000 cycles that the tensor cores take for it
 //   warps 8-15  epilogue, two per TMEM lane quarter taking alternate 32-token chunks, as in tensor_fwd_kernel.cuh
 //
 // CG = 2 (long groups): a cluster of two CTAs shares every item -- same rows, neighbouring weight tiles, 256 x 256
@@ -235,39 +237,14 @@ __device__ __forceinline__ void build_qtable(const W4A4Args& a, QGroup* grp, uin
     if (t == 0) base[0] = 0;
 }
 
-// 16 bytes; on an L2 miss the 256 bytes around them are fetched, which hold the row's next spans and its neighbours
-__device__ __forceinline__ uint4 load_scale16(const uint4* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
-
-// Up to 32 scale bytes from p (any alignment): the aligned 16-byte pieces they lie in go into raw, their place in them
-// into *at; nothing is computed from the loads here, so that several rows' can be in flight.  Where the pieces would reach
-// over an end of the scale tensor [lo, hi) (its first and last rows) the bytes are read one by one.
-__device__ __forceinline__ void fetch_scale_row(const uint8_t* p, int valid, const uint8_t* lo, const uint8_t* hi, uint32_t* raw, uint32_t* at) {
-    const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 15);
-    const uint4* q = reinterpret_cast<const uint4*>(p - off);
-    *at = off;
-    if (off == 0 && valid >= 32) {
-        const uint4 v0 = load_scale16(q), v1 = load_scale16(q + 1);
-        raw[0] = v0.x; raw[1] = v0.y; raw[2] = v0.z; raw[3] = v0.w;
-        raw[4] = v1.x; raw[5] = v1.y; raw[6] = v1.z; raw[7] = v1.w;
-    } else if (p - off >= lo && p - off + 48 <= hi) {
-        const uint4 v0 = load_scale16(q), v1 = load_scale16(q + 1), v2 = load_scale16(q + 2);
-        raw[0] = v0.x; raw[1] = v0.y; raw[2] = v0.z; raw[3] = v0.w;
-        raw[4] = v1.x; raw[5] = v1.y; raw[6] = v1.z; raw[7] = v1.w;
-        raw[8] = v2.x; raw[9] = v2.y; raw[10] = v2.z; raw[11] = v2.w;
-    } else {
-        *at = 0;
+// The aligned 16 bytes at q as far as they lie in the scale tensor [lo, hi), zeros elsewhere: for the pieces of its first
+// and last rows.
+__device__ __noinline__ uint4 load_scale_edge(const uint8_t* q, const uint8_t* lo, const uint8_t* hi) {
+    uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            raw[j] = 0;
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-                if (4 * j + b < valid) raw[j] |= (uint32_t)__ldg(p + 4 * j + b) << (8 * b);
-        }
-    }
+    for (int b = 0; b < 16; ++b)
+        if (q + b >= lo && q + b < hi) w[b >> 2] |= (uint32_t)__ldg(q + b) << (8 * (b & 3));
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 // The 32 bytes at offset `at` (0..15) of the 48 in raw as 8 words, zeros behind the first `valid`.
 __device__ __forceinline__ void align_scale_row(const uint32_t* raw, uint32_t at, int valid, uint32_t* out) {
@@ -330,7 +307,7 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full + b, 1);
             mbar_init(acc_empty + b, kQEpiWarps * CG);
-            mbar_init(sc_full + b, kQScaleWarps * CG);
+            mbar_init(sc_full + b, kQScaleWarps + (CG == 2 && rank == 0 ? 1 : 0));
             mbar_init(sc_done + b, 1);
         }
         *abort_flag = 0;
@@ -391,13 +368,22 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
             id += workers;
         }
     } else if (warp == 1 && rank == 1) {
-        // ------------------------------------------------------------ the pair's second CTA: tiles landed -> leader
+        // ------------------------------------------------------------ the pair's second CTA: tiles landed and scales
+        // written -> leader.  The scale warps' stores are published to the tensor core that reads them, this SM's own, by
+        // their proxy fence; a release at cluster scope in every one of them would cost a thousand cycles per span
         int32_t g = 0;
         QItem it;
-        uint32_t s = 0, phase = 0, id = worker;
+        uint32_t s = 0, phase = 0, sp = 0, sp_phase = 0, id = worker;
         while (__all_sync(0xffffffffu, next_qitem(a, tb, g, id, &it, tile_rows, tile_first))) {
             bool ok = true;
             for (int rb = 0; rb < a.k_stages; ++rb) {
+                if ((rb & 3) == 0) {
+                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(sc_full + sp, sp_phase, abort_flag));
+                    if (!ok) break;
+                    if (lane == 0) mbar_arrive_release_cluster(leader_base + (smem_u32(sc_full + sp) - own_base));
+                    sp ^= 1;
+                    sp_phase ^= sp ^ 1;
+                }
                 ok = __all_sync(0xffffffffu, mbar_wait_bounded(landed + s, phase, abort_flag));
                 if (!ok) break;
                 if (lane == 0) mbar_arrive_cluster(leader_base + s * 8);
@@ -424,36 +410,41 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
             bool ok = __all_sync(0xffffffffu, q_wait<CG>(acc_empty + buf, acc_phase ^ 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
-            for (int rb = 0; rb < a.k_stages; ++rb) {
-                if ((rb & 3) == 0) ok = __all_sync(0xffffffffu, q_wait<CG>(sc_full + sp, sp_phase, abort_flag));
-                ok = __all_sync(0xffffffffu, ok && q_wait<CG>(full + s, phase, abort_flag));
-                if (!ok) break;
-                tc_fence_after();
-                const bool last = rb + 1 == a.k_stages;
-                const bool span_end = last || (rb & 3) == 3;
-                const int steps = last ? tail : 4;          // steps that exist (a trailing half step is zero elements)
-                const uint64_t da = w_desc0 + s * tile_step, db = da + (kQWTile >> 4);
-                const uint64_t src = sc_desc0 + sp * span_step + (uint32_t)(rb & 3) * (2 * half_step);
-                const uint32_t sf = tmem_sf0 + s * slot_cols, sf1 = sf + half_cols;
-                if (elect_one()) {
-                    q_cp<CG>(sf, src);
-                    q_cp<CG>(sf + 4, src + (512 >> 4));
-                    if (two) q_cp<CG>(sf + 8, src + (1024 >> 4));
-                    q_mma<CG>(acc, da, db, id0, sf, sf + 4, rb > 0 ? 1u : 0u);
-                    if (steps > 1) q_mma<CG>(acc, da + 2, db + 2, id2, sf, sf + 4, 1u);
-                    if (steps > 2) {
-                        q_cp<CG>(sf1, src + half_step);
-                        q_cp<CG>(sf1 + 4, src + half_step + (512 >> 4));
-                        if (two) q_cp<CG>(sf1 + 8, src + half_step + (1024 >> 4));
-                        q_mma<CG>(acc, da + 4, db + 4, id0, sf1, sf1 + 4, 1u);
-                        if (steps > 3) q_mma<CG>(acc, da + 6, db + 6, id2, sf1, sf1 + 4, 1u);
+            for (int rb0 = 0; ok && rb0 < a.k_stages; rb0 += 4) {
+                ok = __all_sync(0xffffffffu, q_wait<CG>(sc_full + sp, sp_phase, abort_flag));
+                const uint64_t src0 = sc_desc0 + sp * span_step;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int rb = rb0 + i;
+                    if (rb >= a.k_stages) break;
+                    ok = __all_sync(0xffffffffu, ok && q_wait<CG>(full + s, phase, abort_flag));
+                    if (!ok) break;
+                    tc_fence_after();
+                    const bool last = rb + 1 == a.k_stages;
+                    const int steps = last ? tail : 4;      // steps that exist (a trailing half step is zero elements)
+                    const uint64_t da = w_desc0 + s * tile_step, db = da + (kQWTile >> 4), src = src0 + 2 * i * half_step;
+                    const uint32_t sf = tmem_sf0 + s * slot_cols, sf1 = sf + half_cols;
+                    if (elect_one()) {
+                        q_cp<CG>(sf, src);
+                        q_cp<CG>(sf + 4, src + (512 >> 4));
+                        if (two) q_cp<CG>(sf + 8, src + (1024 >> 4));
+                        q_mma<CG>(acc, da, db, id0, sf, sf + 4, rb > 0 ? 1u : 0u);
+                        if (steps > 1) q_mma<CG>(acc, da + 2, db + 2, id2, sf, sf + 4, 1u);
+                        if (steps > 2) {
+                            q_cp<CG>(sf1, src + half_step);
+                            q_cp<CG>(sf1 + 4, src + half_step + (512 >> 4));
+                            if (two) q_cp<CG>(sf1 + 8, src + half_step + (1024 >> 4));
+                            q_mma<CG>(acc, da + 4, db + 4, id0, sf1, sf1 + 4, 1u);
+                            if (steps > 3) q_mma<CG>(acc, da + 6, db + 6, id2, sf1, sf1 + 4, 1u);
+                        }
+                        q_commit<CG>(done + s, peer_base, own_base);
+                        if (i == 3 || last) q_commit<CG>(sc_done + sp, peer_base, own_base);
+                        if (last) q_commit<CG>(acc_full + buf, peer_base, own_base);
                     }
-                    q_commit<CG>(done + s, peer_base, own_base);
-                    if (span_end) q_commit<CG>(sc_done + sp, peer_base, own_base);
-                    if (last) q_commit<CG>(acc_full + buf, peer_base, own_base);
+                    if (++s == stages) { s = 0; phase ^= 1; }
                 }
-                if (++s == stages) { s = 0; phase ^= 1; }
-                if (span_end) { sp ^= 1; sp_phase ^= sp ^ 1; }
+                sp ^= 1;
+                sp_phase ^= sp ^ 1;
             }
             if (!ok) break;
             if (++buf == (uint32_t)a.acc_bufs) { buf = 0; acc_phase ^= 1; }
@@ -461,66 +452,120 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
         }
     } else if (warp < kQEpiWarp0) {
         // ------------------------------------------------------------ scales: global -> registers -> shared memory
-        // rows 0..127 are the weight tile's, 128.. the activations'; this thread has rows u and u + 192
-        constexpr int kRows = kQScaleWarps * 32;
-        static_assert(2 * kRows == 128 + 256, "two rows per thread");
-        const int u = threadIdx.x - kQScaleWarp0 * 32;
+        // Blocks of 32 rows: 0..3 the weight tile's, 4..11 the activations'; block b of its 128 rows is rows 8b .. 8b + 7 of
+        // each quarter.  This warp has blocks sw and sw + 6.
+        const int sw = warp - kQScaleWarp0;
+        const int quarter = lane >> 3;
         const int64_t kb = a.K / 32;
         const uint8_t* w_hi = a.ws + (int64_t)(a.E - 1) * a.ws_se + (a.N - 1) * a.ws_sn + kb;
         const uint8_t* x_hi = a.xs + a.T * kb;
+        const bool aligned = ((reinterpret_cast<uintptr_t>(a.ws) | reinterpret_cast<uintptr_t>(a.xs) | (uintptr_t)kb | (uintptr_t)a.ws_sn |
+                               (uintptr_t)a.ws_se) & 15) == 0;     // every row starts on 16 bytes
         const int spans = (a.k_stages + 3) >> 2;
         int32_t g = 0;
         QItem it;
         uint32_t id = worker;
-        bool have = next_qitem(a, tb, g, id, &it, tile_rows, tile_first);
+        bool have = __all_sync(0xffffffffu, next_qitem(a, tb, g, id, &it, tile_rows, tile_first));
         int sp = 0;
-        // the next span of this CTA's items; returns its bytes per row (0: none), one bit in `live` per existing row
-        auto fetch = [&](uint32_t (&raw)[2][12], uint32_t (&at)[2], uint32_t& live) -> int {
+        const uint8_t* row[2] = {nullptr, nullptr};         // this lane's rows; those that do not exist read the last that does
+        uint32_t at[2] = {0, 0};                            // their place in 16 bytes
+        uint32_t here = 0;                                  // one bit per block: it has rows
+        int inside[2] = {0, 0};                             // spans whose 48 bytes all lie in the tensor
+        uint32_t raw[2][12];
+#pragma unroll
+        for (int o = 0; o < 2; ++o)
+#pragma unroll
+            for (int j = 0; j < 12; ++j) raw[o][j] = 0;
+        // the next span of this CTA's items; returns its bytes per row (0: none) and which blocks it has
+        auto fetch = [&](uint32_t& blocks) -> int {
             if (!have) return 0;
             const int valid = (int)min((int64_t)32, kb - (int64_t)sp * 32);
-            live = 0;
+            if (sp == 0) {
+                here = 0;
+#pragma unroll
+                for (int o = 0; o < 2; ++o) {
+                    const int b = sw + o * kQScaleWarps;
+                    const bool w = b < 4;
+                    const int first = 8 * (b & 3);
+                    const int rows = w ? (int)min((int64_t)a.rows_w, a.N - it.n0) : it.tokens - ((b >> 2) - 1) * 128;
+                    if (first >= rows) continue;
+                    here |= 1u << o;
+                    const int r = min(quarter * 32 + first + (lane & 7), rows - 1);
+                    const uint8_t* base = w ? a.ws + (int64_t)it.eid * a.ws_se + (int64_t)it.n0 * a.ws_sn
+                                            : a.xs + ((int64_t)it.row0 + ((b >> 2) - 1) * 128) * kb;
+                    const int64_t pitch = w ? a.ws_sn : kb;
+                    row[o] = base + r * pitch;
+                    at[o] = (uint32_t)(reinterpret_cast<uintptr_t>(row[o]) & 15);
+                    const uint8_t* last = base + min(127, rows - 1) * pitch;
+                    inside[o] = base - (reinterpret_cast<uintptr_t>(base) & 15) >= (w ? a.ws : a.xs)
+                                    ? (int)min((int64_t)spans, ((w ? w_hi : x_hi) - last - 16) >> 5) : 0;
+                }
+            }
+            blocks = here;
 #pragma unroll
             for (int o = 0; o < 2; ++o) {
-                const int x = u + o * kRows - 128;          // activation row, or (negative) weight row x + 128
-                const bool w = x < 0;
-                const bool in = w ? x + 128 < a.rows_w && it.n0 + x + 128 < a.N : x < it.tokens;
-                if (in) {
-                    live |= 1u << o;
-                    const uint8_t* p = w ? a.ws + (int64_t)it.eid * a.ws_se + (int64_t)(it.n0 + x + 128) * a.ws_sn
-                                         : a.xs + ((int64_t)it.row0 + x) * kb;
-                    fetch_scale_row(p + sp * 32, valid, w ? a.ws : a.xs, w ? w_hi : x_hi, raw[o], &at[o]);
+                if (!(here >> o & 1u)) continue;
+                const uint8_t* p = row[o] + sp * 32;
+                if (aligned) {
+                    const uint4 v0 = __ldg(reinterpret_cast<const uint4*>(p));
+                    const uint4 v1 = __ldg(reinterpret_cast<const uint4*>(p) + (valid > 16 ? 1 : 0));
+                    raw[o][0] = v0.x; raw[o][1] = v0.y; raw[o][2] = v0.z; raw[o][3] = v0.w;
+                    raw[o][4] = v1.x; raw[o][5] = v1.y; raw[o][6] = v1.z; raw[o][7] = v1.w;
+                } else {
+                    const uint4* q = reinterpret_cast<const uint4*>(p - at[o]);
+                    uint4 v0, v1, v2;
+                    if (sp < inside[o]) {
+                        v0 = __ldg(q); v1 = __ldg(q + 1); v2 = __ldg(q + 2);
+                    } else {
+                        const bool w = sw + o * kQScaleWarps < 4;
+                        const uint8_t* lo = w ? a.ws : a.xs;
+                        const uint8_t* hi = w ? w_hi : x_hi;
+                        v0 = load_scale_edge(reinterpret_cast<const uint8_t*>(q), lo, hi);
+                        v1 = load_scale_edge(reinterpret_cast<const uint8_t*>(q + 1), lo, hi);
+                        v2 = load_scale_edge(reinterpret_cast<const uint8_t*>(q + 2), lo, hi);
+                    }
+                    raw[o][0] = v0.x; raw[o][1] = v0.y; raw[o][2] = v0.z; raw[o][3] = v0.w;
+                    raw[o][4] = v1.x; raw[o][5] = v1.y; raw[o][6] = v1.z; raw[o][7] = v1.w;
+                    raw[o][8] = v2.x; raw[o][9] = v2.y; raw[o][10] = v2.z; raw[o][11] = v2.w;
                 }
             }
             if (++sp == spans) {
                 sp = 0;
                 id += workers;
-                have = next_qitem(a, tb, g, id, &it, tile_rows, tile_first);
+                have = __all_sync(0xffffffffu, next_qitem(a, tb, g, id, &it, tile_rows, tile_first));
             }
             return valid;
         };
-        uint32_t raw[2][12] = {}, at[2] = {}, live = 0, slot = 0, phase = 0;
-        int valid = fetch(raw, at, live);
+        uint32_t slot = 0, phase = 0, blocks = 0;
+        int valid = fetch(blocks);
         while (valid) {
+            // rows behind the last hold bytes of other rows: they belong to accumulator entries that nobody reads
             uint32_t out[2][8];
-            const uint32_t put = live;                      // stale bytes of other rows belong to accumulator entries that
-#pragma unroll                                              // nobody reads
-            for (int o = 0; o < 2; ++o) align_scale_row(raw[o], at[o], valid, out[o]);
-            valid = fetch(raw, at, live);                   // on its way while this span waits for its slot and is written
-            if (!__all_sync(0xffffffffu, mbar_wait_bounded(sc_done + slot, phase ^ 1, abort_flag))) break;
+            const uint32_t put = blocks;
 #pragma unroll
             for (int o = 0; o < 2; ++o) {
-                if (!(put & (1u << o))) continue;
-                const int f = u + o * kRows;
-                uint8_t* dst = s_scale + slot * span_bytes + (f >> 7) * 512 + (f & 31) * 16 + ((f >> 5) & 3) * 4;
+                if (!(put >> o & 1u)) continue;
+                if (aligned && valid >= 32) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) out[o][j] = raw[o][j];
+                } else {
+                    align_scale_row(raw[o], at[o], valid, out[o]);
+                }
+            }
+            valid = fetch(blocks);                          // on its way while this span waits for its slot and is written
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(sc_done + slot, phase ^ 1, abort_flag))) break;
+            uint8_t* dst0 = s_scale + slot * span_bytes + (lane & 7) * 16 + quarter * 4;
+#pragma unroll
+            for (int o = 0; o < 2; ++o) {
+                if (!(put >> o & 1u)) continue;
+                const int b = sw + o * kQScaleWarps;
+                uint8_t* dst = dst0 + (b >> 2) * 512 + (b & 3) * 128;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) *reinterpret_cast<uint32_t*>(dst + j * half_bytes) = out[o][j];
             }
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) {
-                if (CG == 2) mbar_arrive_release_cluster(leader_base + (smem_u32(sc_full + slot) - own_base));
-                else mbar_arrive(sc_full + slot);
-            }
+            if (lane == 0) mbar_arrive(sc_full + slot);     // in a pair the second CTA's MMA warp passes it on
             slot ^= 1;
             phase ^= slot ^ 1;
         }
