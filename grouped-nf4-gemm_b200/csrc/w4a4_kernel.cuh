@@ -183,9 +183,17 @@ struct QItem {
     int32_t row0, tokens, eid, n0;
 };
 
+// Item `id` -> its group, chunk and tile; g: the group of an earlier item.  Called by whole warps.
 __device__ __forceinline__ bool next_qitem(const W4A4Args& a, const QTable& tb, int32_t& g, uint32_t id, QItem* it, int32_t tile_rows,
                                            int32_t tile_first) {
-    while (g < a.G && id >= tb.base[g + 1]) ++g;
+    // all lanes together, 32 groups at a time: one after the other, the dozen groups between two items of an SM cost
+    // every role two thousand cycles per item
+    while (true) {
+        const int32_t next = g + 1 + (int32_t)(threadIdx.x & 31);
+        const uint32_t past = __ballot_sync(0xffffffffu, next <= a.G && id >= tb.base[next]);      // a run from lane 0 on
+        g += __popc(past);
+        if (past != 0xffffffffu) break;
+    }
     if (g >= a.G) return false;
     const QGroup gr = tb.grp[g];
     const uint32_t local = id - tb.base[g];
@@ -665,7 +673,7 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
 }
 
 // Groups this long run as CTA pairs
-constexpr int kQPairRows = 128;
+constexpr int kQPairRows = 384;
 
 struct W4A4Plan {
     int rows_w, tok_cap, xbox, x_bytes, x_blocks, stages, acc_bufs;
