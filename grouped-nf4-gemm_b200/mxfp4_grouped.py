@@ -283,6 +283,9 @@ def gemm_mxfp4_grouped_w4a4(a_blocks, a_scales, blocks, scales, sizes, expert_id
         raise ValueError("rows and stack must live on the same device")
     if half_w != half:
         raise ValueError(f"the rows have K={2 * half} but the stack packs K={2 * half_w}")
+    for table in (group_offsets, expert_ids, sizes):
+        if torch.is_tensor(table) and table.is_cuda and table.device != dev:
+            raise ValueError(f"a group table lives on {table.device}, the rows on {dev}")
     out = torch.empty((T, N), dtype=torch.bfloat16, device=dev)
     if T == 0 or N == 0 or E == 0:
         return out

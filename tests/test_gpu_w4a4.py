@@ -315,6 +315,29 @@ def test_product_extreme_scales_and_nan():
     assert torch.isnan(nan[1]).all() and torch.isfinite(nan[[0, 2, 3, 4]]).all()
 
 
+def test_product_beyond_32_bit_offsets():
+    """A stack of more than 4 GiB: the last expert against its own copy."""
+    E, N, K = 300, 4096, 7168
+    wb = torch.randint(0, 256, (E, N, K // 2), dtype=torch.uint8, device=DEV)
+    ws = torch.randint(120, 126, (E, N, K // 32), dtype=torch.uint8, device=DEV)
+    xb, xs = packed((5,), K, 42)
+    out = M.gemm_mxfp4_grouped_w4a4(xb, xs, wb, ws, [2, 3], [E - 1, 0])
+    for lo, hi, e in ((0, 2, E - 1), (2, 5, 0)):
+        assert torch.equal(out[lo:hi], M.gemm_mxfp4_grouped_w4a4(xb[lo:hi], xs[lo:hi], wb[e:e + 1].clone(), ws[e:e + 1].clone(), [hi - lo], [0]))
+
+
+def test_quantize_beyond_32_bit_offsets():
+    rows, K = 70000, 32 * 1000
+    x = torch.zeros(rows, K, dtype=torch.bfloat16, device=DEV)
+    x[-3:] = torch.randn(3, K, generator=gen(43)).to(torch.bfloat16).to(DEV)
+    b, s = M.quantize_mxfp4(x)
+    rb, rs = pack_ref(x[-3:].cpu())
+    assert torch.equal(b[-3:].cpu(), rb) and torch.equal(s[-3:].cpu(), rs)
+    del x
+    v = M.dequantize_mxfp4(b, s)
+    assert torch.equal(v[-3:].cpu().double(), values64(rb, rs)) and not v[:-3].any()
+
+
 def test_product_empty_calls():
     wb, ws = packed((2, 16), 64, 29)
     xb, xs = packed((0,), 64, 30)
