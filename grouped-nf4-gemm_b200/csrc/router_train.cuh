@@ -21,6 +21,10 @@
 // memory.  The warps of a CTA are added in a fixed order, the CTAs by integer atomics: counts as they are, probability
 // sums as 64-bit fixed-point numbers in steps of 2^-32 (a sum is at most 2^31; a step is far below the fp32 sums' own
 // rounding), so that the order in which CTAs arrive cannot change a bit.  The last CTA to arrive computes the losses.
+//
+// Measured at 65536 tokens x 256 experts, top 8, fp32 (67 MB of logits): forward 55 us, 580 instructions a token at 70 %
+// of the issue slots (115 us with k scans, and 27 to 66 us more for a second kernel over the CTAs' sums); backward 47 us,
+// latency of one row per warp (20 us would be the bytes).
 #pragma once
 
 #include "common.cuh"
