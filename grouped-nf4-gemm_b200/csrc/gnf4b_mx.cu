@@ -98,7 +98,8 @@ int gnf4b_gemm_grouped_w4a4(const uint8_t* x_blocks, const uint8_t* x_scales, in
                             int32_t* status_word, void* cuda_stream) {
     if (T < 0 || G < 0) return GNF4B_EINVAL;
     if (E <= 0 || N <= 0 || K <= 0 || K % 32) return GNF4B_ESHAPE;
-    if (T > INT32_MAX || N > INT32_MAX || K > INT32_MAX) return GNF4B_ETOOBIG;
+    // row and column numbers, tiles included that reach beyond the end, are 32-bit coordinates of the loads
+    if (T > INT32_MAX - 256 || N > INT32_MAX - 256 || K > INT32_MAX) return GNF4B_ETOOBIG;
     if (T == 0 || G == 0) return GNF4B_OK;
     if (!x_blocks || !x_scales || !W || !S || !group_offsets || !expert_ids || !out) return GNF4B_EINVAL;
     if (s_stride_e < 0 || s_stride_n < 0) return GNF4B_EINVAL;

@@ -411,7 +411,57 @@ def test_glu_keeps_eight_bits():
     assert rows * 2 * h <= kept_bytes <= rows * 2 * h * 17 / 16 + 4096
 
 
+def test_glu_under_graphs_and_on_streams():
+    """Two captured forward-and-backward passes of the same buffers, replayed on two streams with other inputs."""
+    x = torch.randn(300, 256, generator=gen(21)).to(torch.bfloat16).to(DEV).requires_grad_()
+    go = torch.randn(300, 128, generator=gen(22)).to(torch.bfloat16).to(DEV)
+
+    def step():
+        out = Q.glu_train(x, "gpt_oss")
+        return out.detach(), torch.autograd.grad(out, x, go)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step())
+        graphs.append(g)
+    with torch.no_grad():
+        x.mul_(-0.75)
+    go.mul_(2)
+    torch.cuda.synchronize()
+    graphs[0].replay()
+    with torch.cuda.stream(side):
+        graphs[1].replay()
+    torch.cuda.synchronize()
+    want = step()
+    for o in outs:
+        assert torch.equal(o[0], want[0]) and torch.equal(o[1], want[1])
+
+
 # ------------------------------------------------------------------------------------------------ together
+def test_w4a4_train_is_the_quantised_product_with_the_plain_gradient():
+    E, N, K = 3, 64, 128
+    g = gen(23)
+    wb, ws = synth.mxfp4_stack(E, N, K, g, device=DEV)
+    x = torch.randn(20, K, generator=g).to(torch.bfloat16).to(DEV).requires_grad_()
+    go = torch.randn(20, N, generator=g).to(torch.bfloat16).to(DEV)
+    sizes, ids = [5, 0, 15], [2, 1, 0]
+    y = Q.gemm_mxfp4_grouped_w4a4_train(x, wb, ws, sizes, ids)
+    assert torch.equal(y, M.gemm_mxfp4_grouped_w4a4(*M.quantize_mxfp4(x), wb, ws, sizes, ids))
+    got, = torch.autograd.grad(y, x, go)
+    assert torch.equal(got, M.dgrad_mxfp4_grouped(go, wb, ws, sizes, ids))
+    half = x.detach().half().requires_grad_()
+    got, = torch.autograd.grad(Q.gemm_mxfp4_grouped_w4a4_train(half, wb, ws, sizes, ids), half, go)
+    assert got.dtype == torch.float16
+
+
 @pytest.mark.parametrize("fmt,rows_fmt", [("nf4", "bf16"), ("mxfp4", "bf16"), ("mxfp4", "mxfp4")])
 def test_layer_training_step(fmt, rows_fmt):
     """Router with its losses, the experts' products on 4-bit stacks, the GLU from its checkpoint, the weighted sum:

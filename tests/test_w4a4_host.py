@@ -49,7 +49,7 @@ def test_c_entry_points_check_before_they_launch():
         return m(xb, xs, T, W, wse, wsn, S, sse, ssn, off, ids, G, E, N, K, -1, out, None, None)
 
     assert call(T=-1) == -1 and call(G=-1) == -1 and call(K=48) == -2 and call(N=0) == -2 and call(E=0) == -2
-    assert call(T=1 << 31) == -6 and call(N=1 << 31) == -6 and call(K=1 << 32) == -6
+    assert call(T=(1 << 31) - 200) == -6 and call(N=(1 << 31) - 200) == -6 and call(K=1 << 32) == -6
     assert call(xb=None) == -1 and call(xs=None) == -1 and call(W=None) == -1 and call(S=None) == -1
     assert call(off=None) == -1 and call(ids=None) == -1 and call(out=None) == -1 and call(out=p + 2) == -1
     assert call(sse=-1) == -1 and call(ssn=-2) == -1
