@@ -610,6 +610,25 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
                 }
             };
             if (e >= chunks) release_acc();              // nothing to drain for this warp
+            const uint32_t acc = tmem_base + buf * (uint32_t)a.tok_cap + ((uint32_t)(q * 32) << 16);
+            if (!pair_ok) {                              // odd N: two-byte stores, chunk by chunk
+#pragma unroll 1
+                for (int c = e; c < chunks; c += 2) {
+                    uint32_t r[32];
+                    tmem_ld32(acc + (uint32_t)(c * 32), r);
+                    tmem_ld_wait();
+                    if (c + 2 >= chunks) release_acc();
+                    const int left = mine ? it.tokens - c * 32 : 0;
+                    uint16_t* p = a.out + (int64_t)(it.row0 + c * 32) * a.N + n;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        if (j < left) *p = f32_to_bf16_bits(__uint_as_float(r[j]));
+                        p += a.N;
+                    }
+                }
+                if (++buf == (uint32_t)a.acc_bufs) { buf = 0; acc_phase ^= 1; }
+                continue;
+            }
             // everything this warp drains is packed into registers first, so that the accumulator is free for the next
             // item before the stores begin: word i of chunk c = tokens 32c + 2i, 2i + 1 of this lane's column
             uint32_t v[kQEpiChunks][16];
@@ -619,40 +638,31 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t r[16];
-                    tmem_ld16(tmem_base + buf * (uint32_t)a.tok_cap + ((uint32_t)(q * 32) << 16) + (uint32_t)((e + 2 * k) * 32 + h * 16), r);
+                    tmem_ld16(acc + (uint32_t)((e + 2 * k) * 32 + h * 16), r);
                     tmem_ld_wait();
 #pragma unroll
                     for (int j = 0; j < 8; ++j) v[k][8 * h + j] = pack_bf16x2(__uint_as_float(r[2 * j + 1]), __uint_as_float(r[2 * j]));
                 }
             }
             if (e < chunks) release_acc();
+            // lanes 2i and 2i+1 swap words: the even lane stores columns (n, n+1) of token 2j, the odd lane (n-1, n) of
+            // token 2j+1 -- 4-byte stores, 64 bytes per half warp
+            const int odd = lane & 1;
+            const uint32_t pick = odd ? 0x3276u : 0x5410u;       // (got.hi, own.hi) or (own.lo, got.lo)
+            uint16_t* p = a.out + (int64_t)(it.row0 + e * 32 + odd) * a.N + (n - odd);
+            const int64_t step = 2 * a.N;
+            int left = mine ? it.tokens - e * 32 - odd : 0;      // store while 2j < left
 #pragma unroll
             for (int k = 0; k < kQEpiChunks; ++k) {
                 if (e + 2 * k >= chunks) break;
-                const int t0 = (e + 2 * k) * 32;
-                if (pair_ok) {
-                    // lanes 2i and 2i+1 swap words: the even lane stores columns (n, n+1) of token 2j, the odd lane
-                    // (n-1, n) of token 2j+1 -- 4-byte stores, 64 bytes per half warp
-                    const int odd = lane & 1;
-                    const int left = mine ? it.tokens - t0 - odd : 0;     // store while 2j < left
-                    uint16_t* p = a.out + (int64_t)(it.row0 + t0 + odd) * a.N + (n - odd);
-                    const int64_t step = 2 * a.N;
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const uint32_t got = __shfl_xor_sync(0xffffffffu, v[k][j], 1);
-                        const uint32_t w = odd ? prmt(got, v[k][j], 0x7632u) : prmt(v[k][j], got, 0x5410u);
-                        if (2 * j < left) *reinterpret_cast<uint32_t*>(p) = w;
-                        p += step;
-                    }
-                } else {
-                    const int left = mine ? it.tokens - t0 : 0;
-                    uint16_t* p = a.out + (int64_t)(it.row0 + t0) * a.N + n;
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        if (j < left) *p = (uint16_t)(v[k][j >> 1] >> (16 * (j & 1)));
-                        p += a.N;
-                    }
+                for (int j = 0; j < 16; ++j) {
+                    const uint32_t got = __shfl_xor_sync(0xffffffffu, v[k][j], 1);
+                    if (2 * j < left) *reinterpret_cast<uint32_t*>(p) = prmt(v[k][j], got, pick);
+                    p += step;
                 }
+                p += 16 * step;                                  // the other warp's chunk
+                left -= 64;
             }
             if (++buf == (uint32_t)a.acc_bufs) { buf = 0; acc_phase ^= 1; }
         }
