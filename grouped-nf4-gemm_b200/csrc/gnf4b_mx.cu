@@ -129,7 +129,7 @@ int gnf4b_gemm_grouped_w4a4(const uint8_t* x_blocks, const uint8_t* x_scales, in
     a.K = K;
     a.E = E;
     a.rows_w = p.rows_w;
-    a.n_tiles = (int32_t)ceil_div(N, p.pair ? 256 : p.rows_w);
+    a.n_tiles = FastDiv::of((uint32_t)ceil_div(N, p.pair ? 256 : p.rows_w));
     a.k_stages = (int32_t)ceil_div(K, kQStageK);
     a.tok_cap = p.tok_cap;
     a.xbox = p.xbox;

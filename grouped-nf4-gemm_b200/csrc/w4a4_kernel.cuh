@@ -68,7 +68,7 @@ struct W4A4Args {
     int64_t T, N, K;
     int32_t G, E;
     int32_t rows_w;             // weight rows per item, a multiple of 8, <= 128
-    int32_t n_tiles;            // items per chunk: ceil(N / rows_w), in a pair ceil(N / 256)
+    FastDiv n_tiles;            // items per chunk: ceil(N / rows_w), in a pair ceil(N / 256)
     int32_t k_stages;           // ceil(K / 256)
     int32_t tok_cap;            // activation rows per item, a multiple of 16 (in a pair 32), <= 256
     int32_t xbox;               // activation rows per TMA box
@@ -204,11 +204,11 @@ __device__ __forceinline__ bool next_qitem(const W4A4Args& a, const QTable& tb, 
     if (g >= a.G) return false;
     const QGroup gr = tb.grp[g];
     const uint32_t local = id - tb.base[g];
-    const uint32_t mc = local / (uint32_t)a.n_tiles;       // n0: of the item; a pair's second CTA adds 128
+    const uint32_t mc = a.n_tiles.div(local);       // n0: of the item; a pair's second CTA adds 128
     it->row0 = gr.row0 + (int32_t)mc * gr.chunk_rows;
     it->tokens = min(gr.chunk_rows, gr.row0 + gr.rows - it->row0);
     it->eid = gr.eid;
-    it->n0 = (int32_t)(local - mc * (uint32_t)a.n_tiles) * tile_rows + tile_first;
+    it->n0 = (int32_t)(local - mc * a.n_tiles.d) * tile_rows + tile_first;
     return true;
 }
 
@@ -236,7 +236,7 @@ __device__ __forceinline__ void build_qtable(const W4A4Args& a, QGroup* grp, uin
         // equal chunks, a multiple of 16 rows each
         gr.chunk_rows = chunks ? (((gr.rows + chunks - 1) / chunks + 15) & ~15) : 16;
         grp[g] = gr;
-        items[h] = (uint32_t)(((int64_t)gr.rows + gr.chunk_rows - 1) / gr.chunk_rows) * (uint32_t)a.n_tiles;
+        items[h] = (uint32_t)(((int64_t)gr.rows + gr.chunk_rows - 1) / gr.chunk_rows) * a.n_tiles.d;
     }
     uint32_t incl = items[0] + items[1];
 #pragma unroll
