@@ -238,17 +238,22 @@ __device__ __forceinline__ void build_qtable(const W4A4Args& a, QGroup* grp, uin
         grp[g] = gr;
         items[h] = (uint32_t)(((int64_t)gr.rows + gr.chunk_rows - 1) / gr.chunk_rows) * a.n_tiles.d;
     }
-    uint32_t incl = items[0] + items[1];
+    // saturating at 2^31 - 1: offsets that go back and forth can name the same rows in many groups, more items than the
+    // host has counted, and a wrapped number would be taken for an item of another group
+    const auto add = [](uint32_t x, uint32_t y) { return min(x + y, 0x7fffffffu); };
+    uint32_t incl = add(items[0], items[1]);
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
         const uint32_t up = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += up;
+        if (lane >= d) incl = add(incl, up);
     }
     if (lane == 31) warp_tot[w] = incl;
+    uint32_t excl = __shfl_up_sync(0xffffffffu, incl, 1);
+    if (lane == 0) excl = 0;
     __syncthreads();
-    for (int v = 0; v < w; ++v) incl += warp_tot[v];
-    if (2 * t < a.G) base[2 * t + 1] = incl - items[1];
-    if (2 * t + 1 < a.G) base[2 * t + 2] = incl;
+    for (int v = 0; v < w; ++v) excl = add(excl, warp_tot[v]);
+    if (2 * t < a.G) base[2 * t + 1] = add(excl, items[0]);
+    if (2 * t + 1 < a.G) base[2 * t + 2] = add(add(excl, items[0]), items[1]);
     if (t == 0) base[0] = 0;
 }
 
