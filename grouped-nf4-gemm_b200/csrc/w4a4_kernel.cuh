@@ -171,6 +171,9 @@ __device__ __forceinline__ bool q_wait(uint64_t* bar, uint32_t parity, volatile 
     return CG == 2 ? mbar_wait_bounded_cluster(bar, parity, abort_flag) : mbar_wait_bounded(bar, parity, abort_flag);
 }
 
+__device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 // one lane of the warp, always the same one
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
@@ -232,11 +235,18 @@ __device__ __forceinline__ void build_qtable(const W4A4Args& a, QGroup* grp, uin
         if ((bad_e || bad_o) && rows != 0 && a.status && blockIdx.x == 0)
             atomicOr(a.status, bad_e ? GNF4B_ST_BAD_EXPERT : GNF4B_ST_BAD_OFFSETS);
         gr.rows = (pad || bad_e || bad_o) ? 0 : (int32_t)rows;
-        const int32_t chunks = (int32_t)(((int64_t)gr.rows + a.tok_cap - 1) / a.tok_cap);
-        // equal chunks, a multiple of 16 rows each
-        gr.chunk_rows = chunks ? (((gr.rows + chunks - 1) / chunks + 15) & ~15) : 16;
+        // equal chunks, a multiple of 16 rows each (a 64-bit division here costs every launch a third of a microsecond)
+        const uint32_t r = (uint32_t)gr.rows;
+        if (r <= (uint32_t)a.tok_cap) {
+            gr.chunk_rows = r ? (int32_t)((r + 15u) & ~15u) : 16;
+            items[h] = r ? a.n_tiles.d : 0u;
+        } else {
+            const uint32_t chunks = (r + (uint32_t)a.tok_cap - 1u) / (uint32_t)a.tok_cap;
+            const uint32_t each = ((r + chunks - 1u) / chunks + 15u) & ~15u;
+            gr.chunk_rows = (int32_t)each;
+            items[h] = (r + each - 1u) / each * a.n_tiles.d;
+        }
         grp[g] = gr;
-        items[h] = (uint32_t)(((int64_t)gr.rows + gr.chunk_rows - 1) / gr.chunk_rows) * a.n_tiles.d;
     }
     // saturating at 2^31 - 1: offsets that go back and forth can name the same rows in many groups, more items than the
     // host has counted, and a wrapped number would be taken for an item of another group
@@ -318,6 +328,10 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
     const uint32_t rank = CG == 2 ? (uint32_t)uniform((int)cluster_ctarank()) : 0u;
     const uint32_t worker = CG == 2 ? blockIdx.x >> 1 : blockIdx.x, workers = CG == 2 ? gridDim.x >> 1 : gridDim.x;
     const int32_t tile_rows = CG == 2 ? 256 : a.rows_w, tile_first = (int32_t)rank * 128;
+    if (threadIdx.x == 32) {         // the descriptors are launch parameters: on their way before anything else
+        tma_prefetch_map(&x_map);
+        tma_prefetch_map(&w_map);
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < kQMaxStages; ++s) {
             mbar_init(full + s, CG);
