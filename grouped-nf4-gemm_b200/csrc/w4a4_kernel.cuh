@@ -505,41 +505,46 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
         uint32_t at[2] = {0, 0};                            // their place in 16 bytes
         uint32_t here = 0;                                  // one bit per block: it has rows
         int inside[2] = {0, 0};                             // spans whose 48 bytes all lie in the tensor
-        uint32_t raw[2][12];
+        uint32_t raw[2][12], raw_at[2] = {0, 0};            // a span's bytes as loaded, and where they begin
 #pragma unroll
         for (int o = 0; o < 2; ++o)
 #pragma unroll
             for (int j = 0; j < 12; ++j) raw[o][j] = 0;
+        // a new item: its rows, and their first bytes on the way to L2 a whole span before they are loaded
+        auto enter = [&]() {
+            if (!have) return;
+            here = 0;
+#pragma unroll
+            for (int o = 0; o < 2; ++o) {
+                const int b = sw + o * kQScaleWarps;
+                const bool w = b < 4;
+                const int first = 8 * (b & 3);
+                const int rows = w ? (int)min((int64_t)a.rows_w, a.N - it.n0) : it.tokens - ((b >> 2) - 1) * 128;
+                if (first >= rows) continue;
+                here |= 1u << o;
+                const int r = min(quarter * 32 + first + (lane & 7), rows - 1);
+                const uint8_t* base = w ? a.ws + (int64_t)it.eid * a.ws_se + (int64_t)it.n0 * a.ws_sn
+                                        : a.xs + ((int64_t)it.row0 + ((b >> 2) - 1) * 128) * kb;
+                const int64_t pitch = w ? a.ws_sn : kb;
+                row[o] = base + r * pitch;
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(row[o]));
+                at[o] = (uint32_t)(reinterpret_cast<uintptr_t>(row[o]) & 15);
+                const uint8_t* last = base + min(127, rows - 1) * pitch;
+                inside[o] = base - (reinterpret_cast<uintptr_t>(base) & 15) >= (w ? a.ws : a.xs)
+                                ? (int)min((int64_t)spans, ((w ? w_hi : x_hi) - last - 16) >> 5) : 0;
+            }
+        };
+        enter();
         // the next span of this CTA's items; returns its bytes per row (0: none) and which blocks it has
         auto fetch = [&](uint32_t& blocks) -> int {
             if (!have) return 0;
             const int valid = (int)min((int64_t)32, kb - (int64_t)sp * 32);
-            if (sp == 0) {
-                here = 0;
-#pragma unroll
-                for (int o = 0; o < 2; ++o) {
-                    const int b = sw + o * kQScaleWarps;
-                    const bool w = b < 4;
-                    const int first = 8 * (b & 3);
-                    const int rows = w ? (int)min((int64_t)a.rows_w, a.N - it.n0) : it.tokens - ((b >> 2) - 1) * 128;
-                    if (first >= rows) continue;
-                    here |= 1u << o;
-                    const int r = min(quarter * 32 + first + (lane & 7), rows - 1);
-                    const uint8_t* base = w ? a.ws + (int64_t)it.eid * a.ws_se + (int64_t)it.n0 * a.ws_sn
-                                            : a.xs + ((int64_t)it.row0 + ((b >> 2) - 1) * 128) * kb;
-                    const int64_t pitch = w ? a.ws_sn : kb;
-                    row[o] = base + r * pitch;
-                    at[o] = (uint32_t)(reinterpret_cast<uintptr_t>(row[o]) & 15);
-                    const uint8_t* last = base + min(127, rows - 1) * pitch;
-                    inside[o] = base - (reinterpret_cast<uintptr_t>(base) & 15) >= (w ? a.ws : a.xs)
-                                    ? (int)min((int64_t)spans, ((w ? w_hi : x_hi) - last - 16) >> 5) : 0;
-                }
-            }
             blocks = here;
 #pragma unroll
             for (int o = 0; o < 2; ++o) {
                 if (!(here >> o & 1u)) continue;
                 const uint8_t* p = row[o] + sp * 32;
+                raw_at[o] = at[o];
                 if (aligned) {
                     const uint4 v0 = __ldg(reinterpret_cast<const uint4*>(p));
                     const uint4 v1 = __ldg(reinterpret_cast<const uint4*>(p) + (valid > 16 ? 1 : 0));
@@ -567,6 +572,7 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
                 sp = 0;
                 id += workers;
                 have = __all_sync(0xffffffffu, next_qitem(a, tb, g, id, &it, tile_rows, tile_first));
+                enter();
             }
             return valid;
         };
@@ -583,7 +589,7 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
 #pragma unroll
                     for (int j = 0; j < 8; ++j) out[o][j] = raw[o][j];
                 } else {
-                    align_scale_row(raw[o], at[o], valid, out[o]);
+                    align_scale_row(raw[o], raw_at[o], valid, out[o]);
                 }
             }
             valid = fetch(blocks);                          // on its way while this span waits for its slot and is written
