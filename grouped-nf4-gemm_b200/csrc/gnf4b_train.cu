@@ -46,9 +46,11 @@ template <int LT, int NE>
 cudaError_t rt_fwd(const RouteTrainArgs& a, int grid, cudaStream_t st) {
     constexpr int W = rt_fwd_warps(NE);
     const size_t smem = (size_t)(W + 1) * a.E * 4;
-    auto kfn = route_train_fwd_kernel<LT, NE, W>;
-    static int granted[64];
-    cudaError_t e = ensure_smem(kfn, smem, granted);
+    constexpr bool kTwo = NE > 1;                    // a row of up to 32 experts has one candidate a lane whatever k is
+    const bool many = kTwo && a.k > kRtFewK;
+    auto kfn = many ? route_train_fwd_kernel<LT, NE, W, kTwo> : route_train_fwd_kernel<LT, NE, W, false>;
+    static int granted[2][64];
+    cudaError_t e = ensure_smem(kfn, smem, granted[many]);
     if (e != cudaSuccess) return e;
     if (grid > 1) {
         e = cudaMemsetAsync(a.sum_p, 0, rt_zeroed_bytes(a.E), st);

@@ -13,18 +13,24 @@
 //
 // The k largest: the k-th largest of the lanes' own maxima bounds the k-th largest of the row from below, and in the mean
 // only a few more than k elements reach that bound.  They are gathered in shared memory, one per lane, and each lane
-// counts how many of them come before its own (larger, or equal and of a lower index): that is its place.  Where more
-// than 32 reach the bound (many equal logits) the k are picked one after the other instead.  Picking alone, a scan of
+// counts how many of them are larger than its own, and only where two are equal how many of those have a lower index: that
+// is its place.  From k = 17 on the mean number that reaches the bound passes 32 (about 130 for k = 32): the bound is then
+// taken from two maxima a lane, and up to 64 candidates are ranked two a lane (16384 x 1024, top 32: 625 -> 102 us).
+// Where still more reach the bound (many equal logits) the k are picked one after the other.  Picking alone, a scan of
 // the lane's registers per choice, costs about three times the instructions, and instructions are what bounds this pass.
+//
+// ex2, lg2 and rcp are the approximate ones (two units of the last fp32 place and less): what is summed stays fp32, and a
+// row's sum of E terms is rounded by more than that.
 //
 // Forward keeps each warp's probability sums in registers over all its tokens and the counts as integers in shared
 // memory.  The warps of a CTA are added in a fixed order, the CTAs by integer atomics: counts as they are, probability
 // sums as 64-bit fixed-point numbers in steps of 2^-32 (a sum is at most 2^31; a step is far below the fp32 sums' own
 // rounding), so that the order in which CTAs arrive cannot change a bit.  The last CTA to arrive computes the losses.
 //
-// Measured at 65536 tokens x 256 experts, top 8, fp32 (67 MB of logits): forward 55 us, 580 instructions a token at 70 %
-// of the issue slots (115 us with k scans, and 27 to 66 us more for a second kernel over the CTAs' sums); backward 47 us,
-// latency of one row per warp (20 us would be the bytes).
+// Measured at 65536 tokens x 256 experts, top 8, fp32 (67 MB of logits, 10 us of reading): forward 50 us, about 500
+// instructions a token at 71 % of the issue slots and 10 us of launches and joining (115 us with k scans, and 27 to 66 us more for
+// a second kernel over the CTAs' sums); backward 34 us, 300 instructions at 53 % (42 us with 24 instead of 32 warps per SM;
+// 20 us would be the bytes).  65536 x 32 bf16, top 4: 27 and 12 us.
 #pragma once
 
 #include "common.cuh"
@@ -33,6 +39,7 @@ namespace gnf4b {
 
 constexpr int kRtMaxExperts = 1024;
 constexpr int kRtMaxK = 32;
+constexpr int kRtFewK = 16;          // up to here one maximum a lane bounds the k-th largest closely enough
 
 // Order-preserving integer of a float: -NaN .. -inf .. +inf .. +NaN; a NaN is to come last, see rt_fix_nan.
 constexpr uint32_t kRtKeyInf = 0xff800000u, kRtKeyNegInf = 0x007fffffu;
@@ -66,29 +73,29 @@ struct RtRow {
                 uint32_t w[kWords > 0 ? kWords : 1];
                 const uint8_t* p = static_cast<const uint8_t*>(row) + (int64_t)e0 * (LT == 2 ? 4 : 2);
                 const bool in = e0 < E;
+                constexpr uint32_t none = LT == 2 ? 0xff800000u : LT == 0 ? 0xff80ff80u : 0xfc00fc00u;       // -inf
                 if (kWords == 4) {
-                    uint4 q = make_uint4(0, 0, 0, 0);
+                    uint4 q = make_uint4(none, none, none, none);
                     if (in) q = __ldcs(reinterpret_cast<const uint4*>(p));
                     w[0] = q.x;
                     if (kWords > 1) w[kWords > 1 ? 1 : 0] = q.y;
                     if (kWords > 2) { w[kWords > 2 ? 2 : 0] = q.z; w[kWords > 3 ? 3 : 0] = q.w; }
                 } else if (kWords == 2) {
-                    uint2 q = make_uint2(0, 0);
+                    uint2 q = make_uint2(none, none);
                     if (in) q = __ldcs(reinterpret_cast<const uint2*>(p));
                     w[0] = q.x;
                     w[kWords > 1 ? 1 : 0] = q.y;
                 } else {
-                    w[0] = in ? __ldcs(reinterpret_cast<const uint32_t*>(p)) : 0u;
+                    w[0] = in ? __ldcs(reinterpret_cast<const uint32_t*>(p)) : none;
                 }
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    float v;
-                    if (LT == 2) v = __uint_as_float(w[j < kWords ? j : 0]);
-                    else {
+                    if (LT == 2) {
+                        x[g * V + j] = __uint_as_float(w[j < kWords ? j : 0]);
+                    } else {
                         const uint32_t h = (w[(j >> 1) < kWords ? (j >> 1) : 0] >> (16 * (j & 1))) & 0xffffu;
-                        v = LT == 0 ? bf16_bits_to_float(h) : __half2float(__ushort_as_half((unsigned short)h));
+                        x[g * V + j] = LT == 0 ? bf16_bits_to_float(h) : __half2float(__ushort_as_half((unsigned short)h));
                     }
-                    x[g * V + j] = in ? v : -INFINITY;
                 }
             } else {
 #pragma unroll
@@ -144,6 +151,23 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
+__device__ __forceinline__ float warp_max(float v) {              // of what is not NaN
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+__device__ __forceinline__ float rt_log(float x) {                // ln x, 1 <= x: off by at most 2^-22 or two units in the last place
+    float r;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r * 0.6931471805599453f;
+}
+__device__ __forceinline__ float rt_rcp(float x) {                // 1 / x to one unit in the last place
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
 struct RouteTrainArgs {
     const void* logits;
     int64_t T, stride;           // elements between rows
@@ -166,12 +190,15 @@ struct RouteTrainArgs {
 };
 __host__ __device__ inline size_t rt_zeroed_bytes(int32_t E) { return (size_t)E * 12 + 8; }
 
-template <int LT, int NE, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32)
+// MANY: k > kRtFewK
+template <int LT, int NE, int WARPS, bool MANY>
+__global__ void __launch_bounds__(WARPS * 32, NE <= 8 ? 2 : 1)
 route_train_fwd_kernel(const __grid_constant__ RouteTrainArgs a) {
     using Row = RtRow<LT, NE>;
+    constexpr int kRtCand = MANY ? 64 : 32;          // candidates for the k places that are ranked together
     extern __shared__ __align__(16) float s_mem[];   // [WARPS][E] probability sums, then [E] counts
-    __shared__ uint2 s_cand[WARPS][32];
+    __shared__ __align__(16) float s_val[WARPS][kRtCand];
+    __shared__ __align__(16) int32_t s_exp[WARPS][kRtCand];
     __shared__ float s_zn[WARPS][2];
     __shared__ float s_tot[34];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -192,36 +219,33 @@ route_train_fwd_kernel(const __grid_constant__ RouteTrainArgs a) {
     float v[NE];
     if (t < a.T) Row::load(base + t * a.stride * item, lane, a.E, vec, v);
     for (; t < a.T; t += step) {
-        float x[NE];
-        uint32_t key[NE], best = 0;
+        float r[NE], x[NE], best = -INFINITY;
 #pragma unroll
         for (int i = 0; i < NE; ++i) {
-            x[i] = v[i];
-            key[i] = rt_key(x[i]);
-            best = max(best, key[i]);
+            r[i] = v[i];
+            best = fmaxf(best, r[i]);
         }
         const bool masked = a.mask && __ldg(a.mask + t) == 0;
         if (t + step < a.T) Row::load(base + (t + step) * a.stride * item, lane, a.E, vec, v);     // on its way meanwhile
-        uint32_t top_key = __reduce_max_sync(0xffffffffu, best);
-        float top = rt_value(top_key), z = 0.f;
+        float top = warp_max(best), z = 0.f;
 #pragma unroll
         for (int i = 0; i < NE; ++i) {
-            x[i] = rt_exp(x[i] - top);
+            x[i] = rt_exp(r[i] - top);
             z += x[i];
         }
         z = warp_sum(z);
         bool dead = false;                           // nothing to choose from: no weight, no loss, no count
-        if (z != z) {                                // a NaN, an infinity or nothing but -inf: rare
+        const bool plain = z == z;
+        if (!plain) {                                // a NaN, an infinity or nothing but -inf: rare
             bool nan = false;
-            best = 0;
+            uint32_t top_key = 0;
 #pragma unroll
             for (int i = 0; i < NE; ++i) {
-                const uint32_t fixed = rt_fix_nan(key[i]);
-                nan |= fixed != key[i];
-                key[i] = fixed;
-                best = max(best, Row::expert(lane, i) < a.E ? fixed : 0u);
+                const uint32_t key = rt_key(r[i]), fixed = rt_fix_nan(key);
+                nan |= fixed != key;
+                top_key = max(top_key, Row::expert(lane, i) < a.E ? fixed : 0u);
             }
-            top_key = __reduce_max_sync(0xffffffffu, best);
+            top_key = __reduce_max_sync(0xffffffffu, top_key);
             top = rt_value(top_key);
             dead = !__any_sync(0xffffffffu, nan) && top_key == kRtKeyNegInf;
             if (dead) {
@@ -230,54 +254,112 @@ route_train_fwd_kernel(const __grid_constant__ RouteTrainArgs a) {
             }
         }
         const bool counted = !masked && !dead;
-        const float lse = dead ? -INFINITY : top + logf(z);
+        const float lse = dead ? -INFINITY : top + rt_log(z);
         if (counted) {
-            const float rz = 1.0f / z;
+            const float rz = rt_rcp(z);
 #pragma unroll
             for (int i = 0; i < NE; ++i) psum[i] = fmaf(x[i], rz, psum[i]);
             zsum += lse * lse;
             ntok += 1.f;
         }
         // the k largest
-        uint32_t sel_key = 0;
+        float sel = 0.f;
         int32_t sel_e = 0, place = 32;
-        int found;
-        if (NE == 1) {
-            found = a.E;                             // every lane has one
-            sel_key = key[0];
-            sel_e = lane;
-        } else {
-            uint32_t bound = top_key, left = best;
-            for (int j = 1; j < a.k; ++j) {
-                if (left == bound) left = 0;
-                bound = __reduce_max_sync(0xffffffffu, left);
-            }
-            // (a bound of -inf or less would take in the experts >= E: one after the other then)
-            found = bound > kRtKeyNegInf ? 0 : 33;
+        int found = kRtCand + 1;
+        if (plain) {
+            float bound = top;
+            if (!MANY) {
+                float left = best;
+#pragma unroll 4
+                for (int j = 1; j < a.k; ++j) {
+                    if (left == bound) left = -INFINITY;
+                    bound = warp_max(left);
+                }
+            } else {                                 // two maxima a lane: of the first and of the second half of its elements
+                float left0 = r[0], left1 = r[NE / 2];
 #pragma unroll
-            for (int i = 0; i < NE; ++i) {
-                const int e = Row::expert(lane, i);
-                const bool in = key[i] >= bound;
-                const uint32_t who = __ballot_sync(0xffffffffu, in);
-                const int at = found + __popc(who & ((1u << lane) - 1u));
-                if (in && at < 32) s_cand[warp][at] = make_uint2(key[i], (uint32_t)e);
-                found += __popc(who);
+                for (int i = 1; i < NE / 2; ++i) {
+                    left0 = fmaxf(left0, r[i]);
+                    left1 = fmaxf(left1, r[NE / 2 + i]);
+                }
+                for (int j = 1; j < a.k; ++j) {
+                    if (left0 == bound) left0 = -INFINITY;
+                    if (left1 == bound) left1 = -INFINITY;
+                    bound = warp_max(fmaxf(left0, left1));
+                }
             }
-            __syncwarp();
-            if (lane < found && found <= 32) {
-                const uint2 c = s_cand[warp][lane];
-                sel_key = c.x;
-                sel_e = (int32_t)c.y;
+            // (a bound of -inf would take in the experts >= E: one after the other then)
+            if (bound > -INFINITY) {
+                int n = 0;
+#pragma unroll
+                for (int i = 0; i < NE; ++i) n += r[i] >= bound ? 1 : 0;
+                // candidates of the lanes before this one and of all, bit by bit of the count
+                const uint32_t before = (1u << lane) - 1u;
+                int at = 0;
+                found = 0;
+#pragma unroll
+                for (int b = 0; (1 << b) <= NE; ++b) {
+                    const uint32_t who = __ballot_sync(0xffffffffu, n >> b & 1);
+                    at += __popc(who & before) << b;
+                    found += __popc(who) << b;
+                }
+                if (found <= kRtCand) {
+#pragma unroll
+                    for (int i = 0; i < NE; ++i)
+                        if (r[i] >= bound) {
+                            s_val[warp][at] = r[i];
+                            s_exp[warp][at] = Row::expert(lane, i);
+                            ++at;
+                        }
+                    // the ranking reads four at a time
+                    for (int j = lane; j < ((found + 3) & ~3) || j < 32; j += 32)
+                        if (j >= found) {
+                            s_val[warp][j] = -INFINITY;
+                            s_exp[warp][j] = INT32_MAX;
+                        }
+                }
             }
         }
-        if (found <= 32) {
-            place = 0;
-            for (int j = 0; j < found; ++j) {
-                const uint32_t ok = __shfl_sync(0xffffffffu, sel_key, j);
-                const int32_t oe = __shfl_sync(0xffffffffu, sel_e, j);
-                place += (ok > sel_key || (ok == sel_key && oe < sel_e)) ? 1 : 0;
+        const auto ranked = [&](float val, int32_t e) {       // candidates before this one
+            int before = 0;
+            for (int j = 0; j < found; j += 4) {
+                const float4 ov = *reinterpret_cast<const float4*>(&s_val[warp][j]);
+                const int4 oe = *reinterpret_cast<const int4*>(&s_exp[warp][j]);
+                before += (ov.x > val || (ov.x == val && oe.x < e)) ? 1 : 0;
+                before += (ov.y > val || (ov.y == val && oe.y < e)) ? 1 : 0;
+                before += (ov.z > val || (ov.z == val && oe.z < e)) ? 1 : 0;
+                before += (ov.w > val || (ov.w == val && oe.w < e)) ? 1 : 0;
             }
+            return before;
+        };
+        if (found <= 32) {
+            __syncwarp();
+            sel = s_val[warp][lane];
+            sel_e = s_exp[warp][lane];
+            place = 0;
+            for (int j = 0; j < found; j += 4) {
+                const float4 ov = *reinterpret_cast<const float4*>(&s_val[warp][j]);
+                place += (ov.x > sel) + (ov.y > sel) + (ov.z > sel) + (ov.w > sel);
+            }
+            // equal ones share a place: once more with the index
+            if (__popc(__reduce_or_sync(0xffffffffu, lane < found ? 1u << place : 0u)) != found) place = ranked(sel, sel_e);
             if (lane >= found) place = 32;
+        } else if (MANY && found <= kRtCand) {       // two a lane; the k then go to their places
+            __syncwarp();
+            const bool second = lane + 32 < found;
+            const int two = lane + (MANY ? 32 : 0);
+            const float v0 = s_val[warp][lane], v1 = second ? s_val[warp][two] : -INFINITY;
+            const int32_t e0 = s_exp[warp][lane], e1 = second ? s_exp[warp][two] : INT32_MAX;
+            const int p0 = ranked(v0, e0), p1 = second ? ranked(v1, e1) : kRtCand;
+            __syncwarp();
+            if (p0 < a.k) { s_val[warp][p0] = v0; s_exp[warp][p0] = e0; }
+            if (p1 < a.k) { s_val[warp][p1] = v1; s_exp[warp][p1] = e1; }
+            __syncwarp();
+            if (lane < a.k) {
+                sel = s_val[warp][lane];
+                sel_e = s_exp[warp][lane];
+                place = lane;
+            }
         } else {
             // one after the other: the largest key left, and of its holders the lowest expert
             uint32_t mask = 0;                       // this lane's elements that are taken
@@ -285,25 +367,25 @@ route_train_fwd_kernel(const __grid_constant__ RouteTrainArgs a) {
                 uint32_t m = 0;
 #pragma unroll
                 for (int i = 0; i < NE; ++i)
-                    if (!(mask >> i & 1u) && Row::expert(lane, i) < a.E) m = max(m, key[i]);
+                    if (!(mask >> i & 1u) && Row::expert(lane, i) < a.E) m = max(m, rt_fix_nan(rt_key(r[i])));
                 m = __reduce_max_sync(0xffffffffu, m);
                 uint32_t e = 0xffffffffu;
 #pragma unroll
                 for (int i = 0; i < NE; ++i)
-                    if (!(mask >> i & 1u) && key[i] == m && Row::expert(lane, i) < a.E) e = min(e, (uint32_t)Row::expert(lane, i));
+                    if (!(mask >> i & 1u) && rt_fix_nan(rt_key(r[i])) == m && Row::expert(lane, i) < a.E) e = min(e, (uint32_t)Row::expert(lane, i));
                 e = __reduce_min_sync(0xffffffffu, e);
 #pragma unroll
                 for (int i = 0; i < NE; ++i)
                     if ((uint32_t)Row::expert(lane, i) == e) mask |= 1u << i;
-                if (lane == j) { sel_key = m; sel_e = (int32_t)e; place = j; }
+                if (lane == j) { sel = rt_value(m); sel_e = (int32_t)e; place = j; }
             }
         }
         const bool chosen = place < a.k;
-        const float ej = (chosen && !dead) ? rt_exp(rt_value(sel_key) - top) : 0.f;
+        const float ej = (chosen && !dead) ? rt_exp(sel - top) : 0.f;
         if (renorm) z = warp_sum(ej);
         if (chosen) {
             a.idx[t * a.k + place] = sel_e;
-            a.w[t * a.k + place] = dead ? 0.f : ej / z;
+            a.w[t * a.k + place] = dead ? 0.f : ej * rt_rcp(z);
             if (counted) atomicAdd(s_c + sel_e, 1);
         }
         if (lane == 0) a.lse[t] = lse;
@@ -397,7 +479,7 @@ struct RouteTrainBwdArgs {
 };
 
 template <int LT, int NE, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32)
+__global__ void __launch_bounds__(WARPS * 32, NE <= 8 ? 4 : NE == 16 ? 2 : 1)
 route_train_bwd_kernel(const __grid_constant__ RouteTrainBwdArgs a) {
     using Row = RtRow<LT, NE>;
     __shared__ __align__(16) float s_sel[WARPS][NE * 32];        // what the weights' gradient adds at the chosen experts

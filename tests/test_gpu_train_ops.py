@@ -85,6 +85,20 @@ def test_routing_types_ties_and_masks(dtype, masked):
     check_routing(logits.to(DEV), k, 1, False, mask)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("E,k", [(48, 17), (64, 32), (100, 24), (256, 16), (256, 17), (256, 32), (512, 20), (1000, 32)])
+def test_routing_many_choices(dtype, E, k):
+    """k around and above the switch to two maxima a lane: distinct logits, few values, neighbours that are all large."""
+    T = 150
+    distinct = torch.stack([torch.randperm(E, generator=gen(90 + i)) for i in range(T)]).float() / 16 - E / 32
+    ties = torch.randint(-3, 4, (T, E), generator=gen(91)).float()
+    block = torch.randn(T, E, generator=gen(92))
+    block[:, E // 2:E // 2 + 33] += 6                       # the choices lie side by side
+    for logits in (distinct, ties, block):
+        check_routing(logits.to(dtype).to(DEV), k, 0, False, None)
+        check_routing(logits.to(dtype).to(DEV), k, 1, False, None)
+
+
 @pytest.mark.parametrize("T", [6, 500])
 def test_routing_excluded_experts_and_dead_tokens(T):
     E, k = 40, 6
