@@ -714,10 +714,18 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
     if (threadIdx.x == 0 && *abort_flag && a.status) atomicOr(a.status, GNF4B_ST_TIMEOUT);
 }
 
-// Groups this long run as CTA pairs.  Pairs / single CTAs in us, gpt-oss gate_up (K = 2880): 128 rows 83 / 69, 256 rows 93 / 97,
-// 300 rows 134 / 141, 512 rows 163 / 178, 1024 rows 304 / 372; Qwen3 gate_up (K = 2048): 128 rows 65-74 / 60, 256 rows 86 / 86,
-// 512 rows 135 / 139.  Shorter groups give a pair too few items and hide less of its accumulator's turn-around.
+// CTA pairs: for groups of kQPairRows and more, where an item has enough stages to pay for handing it over between two
+// CTAs, and, where rows start on 128-byte lines (a 128-byte box row is then one L2 request, else two, and a single CTA's
+// loads hold it up), not so many that the exposed epilogue a pair saves on is small beside them.
+// Single CTAs / pairs in us, 32 experts, N = 4096, 512 and 1024 rows each:
+//   K = 736    55 / 56, 100 / 107    K = 1312   83 / 74, 154 / 134   (rows do not start on 128 bytes)
+//   K = 2880  135 / 123, 243 / 215   K = 4128  268 / 219, 440 / 372
+//   K = 2048   83 / 82, 150 / 141    K = 2816  115 / 114, 210 / 205  (rows do)
+// and with rows on 128 bytes, 64 experts, N = 2048: K = 1024 51 / 52, 95 / 99; K = 1280 67 / 73, 121 / 129; K = 1536 69 / 70,
+// 129 / 127; 16 experts, N = 4096: K = 4096 78 / 80, 142 / 143; K = 7168 117 / 125, 216 / 228.  300 rows (32 experts): K = 2048
+// 66 / 71, K = 2880 106 / 111; 400 rows, N = 5760, K = 2880: 150 / 144.
 constexpr int kQPairRows = 384;
+constexpr int kQPairStages = 6, kQPairStagesAligned = 20;      // K > 1280; K <= 5120 where rows start on 128 bytes
 
 struct W4A4Plan {
     int rows_w, tok_cap, xbox, x_bytes, x_blocks, stages, acc_bufs;
@@ -744,7 +752,8 @@ static inline W4A4Plan w4a4_plan(int64_t T, int32_t G, int64_t N, int64_t K, int
             if (cost < best) { best = cost; p.rows_w = r; }
         }
     }
-    p.pair = longest >= kQPairRows;
+    const int64_t k_stages = ceil_div(K, kQStageK);
+    p.pair = longest >= kQPairRows && k_stages >= kQPairStages && (k_stages <= kQPairStagesAligned || (K / 2) % 128 != 0);
     if (p.pair) {
         p.tok_cap = (int)round_up(p.tok_cap, 32);
         p.xbox = 64;
