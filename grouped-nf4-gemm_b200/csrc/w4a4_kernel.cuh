@@ -11,12 +11,12 @@
 // Roles (512 threads, one CTA per SM, persistent):
 //   warp 0      TMA producer: per stage of 256 contraction elements (128 bytes a row, 128-byte swizzle) the weight tile
 //               [rows_w x 128 B] and the item's activation rows in boxes of xbox rows
-//   warp 1      MMA issuer (one lane): tcgen05.cp of the stage's scales shared memory -> tensor memory (32 lanes
+//   warp 1      MMA issuer: tcgen05.cp of the stage's scales shared memory -> tensor memory (32 lanes
 //               x 16 bytes, replicated to the four lane quarters), then up to four MMAs of 64 elements
 //   warps 2-7   scales, a span of 1024 elements (32 exponent bytes a row, four stages) at a time in a ring of two: every
 //               thread has two of the 128 + 256 rows and reads a row's 32 bytes with two 16-byte loads (three where rows
 //               do not start on 16 bytes: gpt-oss has 90 bytes a row, which is also why they cannot come by TMA), those
-//               of the next span in flight while a span is written as the 4-byte words of 128 elements that tcgen05.cp
+//               of the next span in flight, and the next item's on their way to L2, while a span is written as the 4-byte words of 128 elements that tcgen05.cp
 //               takes (row r at (r % 32) * 16 + (r / 32) * 4; a warp's 32 rows are eight of each quarter, so that no two
 //               lanes share a bank).  What counts here is the number of instructions: a warp issues one every five or six
 //               cycles, and all of a span's have to fit the 2000 cycles that the tensor cores take for it
@@ -33,12 +33,15 @@
 // group the kernel streams weights and rows_w < 128 evens out the items over the SMs (the MMA still multiplies 128
 // lanes; the lanes above rows_w hold stale bytes and scales and are not read back).
 //
-// Measured (kernel alone, CUDA events): gpt-oss gate_up (N = 5760, K = 2880, 32 experts) 4 rows each 58-67 us, 4.9-4.2 TB/s;
-// 1024 rows each 307-322 us, 3.5 PFLOP/s; Qwen3 gate_up (N = 1536, K = 2048, 128 experts) 256 rows each 77-84 us, 2.7
-// PFLOP/s; one gpt-oss token through 4 experts 15-18 us.  (The W4A16 kernels here: 288, 979, 218 us for the first three.)
-// What bounds it: the issuer takes about 31 cycles per tcgen05 instruction and 130 per completed barrier, 670 cycles
-// per stage with few rows and 850 in a pair, where the MMAs of a stage take 512 and shared memory 640 (48 KiB of operands
-// and 32 KiB from TMA at 128 bytes a cycle); single CTAs with 256 rows wait for TMA, 1350 cycles per stage.
+// Measured (kernel alone, graphs of 20 launches): gpt-oss gate_up (N = 5760, K = 2880, 32 experts) 4 rows each 55 us, 5.1 TB/s;
+// 1024 rows each 281-308 us, 3.9-3.5 PFLOP/s; Qwen3 gate_up (N = 1536, K = 2048, 128 experts) 256 rows each 70-79 us, 2.9-2.6
+// PFLOP/s (the lower figures at 1.65 GHz, where the power limit then holds the clock); one gpt-oss token through 4 experts
+// 13 us.  (The W4A16 kernels here: 288, 979, 218 us for the first three.)
+// What bounds it: with few rows the issuer, 635 cycles per stage at about 31 per tcgen05 instruction and 130 per completed
+// barrier (without the MMAs and copies 47 us of the 55, the rate of a plain copy); with 256 rows the tiles' way from L2 into
+// shared memory, 45 to 49 bytes per cycle and SM (without MMAs and copies 58 us of 70, in a pair 170 of 203 for 8 x 2048 rows,
+// K = 7168), and the power limit; scales take 3 to 9 % (rows on 16 bytes the less).  A launch reaches its first MMA after
+// 3.5 us with few rows (1.6 of them launch and group table) and after 6 with many, when every SM loads at once.
 #pragma once
 
 #include "tensor_fwd_kernel.cuh"
@@ -715,8 +718,8 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
 }
 
 // CTA pairs: for groups of kQPairRows and more, where an item has enough stages to pay for handing it over between two
-// CTAs, and, where rows start on 128-byte lines (a 128-byte box row is then one L2 request, else two, and a single CTA's
-// loads hold it up), not so many that the exposed epilogue a pair saves on is small beside them.
+// CTAs, and, where rows start on 128-byte lines (a box row of 128 bytes is then one line of L2, else two, and a single
+// CTA's loads hold it up more), not so many that the exposed epilogue a pair saves on is small beside them.
 // Single CTAs / pairs in us, 32 experts, N = 4096, 512 and 1024 rows each:
 //   K = 736    55 / 56, 100 / 107    K = 1312   83 / 74, 154 / 134   (rows do not start on 128 bytes)
 //   K = 2880  135 / 123, 243 / 215   K = 4128  268 / 219, 440 / 372
