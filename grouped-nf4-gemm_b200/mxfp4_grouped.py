@@ -165,15 +165,19 @@ def quantize_mxfp4(x):
     K = shape[-1] if shape else 0
     if K == 0 or K % MX_BLOCK:
         raise ValueError(f"the last dimension must be a positive multiple of {MX_BLOCK}, got shape {tuple(shape)}")
-    if len(shape) != 2:
-        x = x.reshape(x.numel() // K, K)
-    rows = x.shape[0]
+    dev = x.device
+    if len(shape) == 2:
+        rows = shape[0]
+        blocks = torch.empty((rows, K // 2), dtype=torch.uint8, device=dev)
+        scales = torch.empty((rows, K // MX_BLOCK), dtype=torch.uint8, device=dev)
+    else:
+        rows = x.numel() // K
+        x = x.reshape(rows, K)
+        blocks = torch.empty((*shape[:-1], K // 2), dtype=torch.uint8, device=dev)
+        scales = torch.empty((*shape[:-1], K // MX_BLOCK), dtype=torch.uint8, device=dev)
     pitch, unit = x.stride()
     if unit != 1:
         x, pitch = x.contiguous(), K
-    dev = x.device
-    blocks = torch.empty((*shape[:-1], K // 2), dtype=torch.uint8, device=dev)
-    scales = torch.empty((*shape[:-1], K // MX_BLOCK), dtype=torch.uint8, device=dev)
     rc = _call_on(dev, _gnf4b.load().gnf4b_quantize_mxfp4, x.data_ptr(), dtype, rows, K, pitch if rows > 1 else K,
                   blocks.data_ptr(), scales.data_ptr())
     if rc:
@@ -183,8 +187,9 @@ def quantize_mxfp4(x):
 
 def _check_packed(blocks, scales, what: str):
     bs, ss = blocks.shape, scales.shape
-    if blocks.dtype is torch.uint8 and scales.dtype is torch.uint8 and len(bs) == len(ss) > 0 and bs[:-1] == ss[:-1] \
-            and bs[-1] == 16 * ss[-1] > 0 and scales.device == blocks.device:
+    n = len(bs)
+    if blocks.dtype is torch.uint8 and scales.dtype is torch.uint8 and n == len(ss) and n and bs[-1] == 16 * ss[-1] > 0 \
+            and (bs[0] == ss[0] if n == 2 else bs[:-1] == ss[:-1]) and scales.device == blocks.device:
         return
     if blocks.dtype != torch.uint8 or scales.dtype != torch.uint8:
         raise TypeError(f"{what}: blocks and scales must be uint8, got {blocks.dtype} and {scales.dtype}")

@@ -119,6 +119,23 @@ def test_routing_excluded_experts_and_dead_tokens(T):
     assert int(r.counts.sum()) == (T - 2) * k
 
 
+@pytest.mark.parametrize("E,k", [(3, 3), (16, 4), (32, 9), (33, 20), (200, 18)])
+def test_routing_rows_with_little_to_choose_from(E, k):
+    """Fewer finite logits than choices, one, none; ties of everything; also where a lane holds one expert."""
+    logits = torch.randn(64, E, generator=gen(70 + E))
+    for t in range(32):
+        logits[t, torch.randperm(E, generator=gen(t))[t % (E + 1):]] = float("-inf")
+    logits[32:40] = 1.25
+    logits[40:44] = 0.0
+    logits[41, ::2] = -0.0
+    for mode in (0, 1):
+        r = ep_moe.route_topk_train(logits.to(DEV), k, mode)
+        c = ep_moe.route_topk_train(logits, k, mode)
+        assert torch.equal(r.idx.cpu(), c.idx) and torch.equal(r.counts.cpu(), c.counts)
+        # sums of at most E terms, two more roundings and the exponentials' few units, on both sides
+        assert ((r.weights.cpu() - c.weights).abs() <= 2 * (E + 16) * 2 * U32 * c.weights + 1e-30).all()
+
+
 def test_routing_nothing_counts_and_no_tokens():
     x = torch.randn(5, 16, generator=gen(8)).to(DEV).requires_grad_()
     r = ep_moe.route_topk_train(x, 2, token_mask=torch.zeros(5, dtype=torch.bool, device=DEV))
