@@ -138,7 +138,7 @@ class _RouteTopkTrain(torch.autograd.Function):
         lse = torch.empty(M + 1, dtype=torch.float32, device=dev)          # and the number of tokens that count
         counts = torch.empty(E, dtype=torch.int32, device=dev)
         balance = torch.empty((), dtype=torch.float32, device=dev)
-        z = torch.empty((), dtype=torch.float32, device=dev)
+        z = torch.empty_like(balance)
         need = _route_scratch(lib, dev, M, E)
         scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         stride = logits.stride(0) if M > 1 else E
@@ -167,7 +167,7 @@ def _route_backward(ctx, g_w, g_balance, g_z):
     logits, token_mask, idx, w, lse, counts = ctx.saved_tensors
     k, mode, norm = ctx.rule
     M, E = logits.shape
-    grad = torch.empty((M, E), dtype=logits.dtype, device=logits.device)
+    grad = torch.empty(M, E, dtype=logits.dtype, device=logits.device)
     n_tokens = lse.data_ptr() + 4 * M
     if g_w is not None:
         g_w = g_w.contiguous()

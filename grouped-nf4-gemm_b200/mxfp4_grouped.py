@@ -168,13 +168,13 @@ def quantize_mxfp4(x):
     dev = x.device
     if len(shape) == 2:
         rows = shape[0]
-        blocks = torch.empty((rows, K // 2), dtype=torch.uint8, device=dev)
-        scales = torch.empty((rows, K // MX_BLOCK), dtype=torch.uint8, device=dev)
+        blocks = torch.empty(rows, K // 2, dtype=torch.uint8, device=dev)
+        scales = torch.empty(rows, K // MX_BLOCK, dtype=torch.uint8, device=dev)
     else:
         rows = x.numel() // K
         x = x.reshape(rows, K)
-        blocks = torch.empty((*shape[:-1], K // 2), dtype=torch.uint8, device=dev)
-        scales = torch.empty((*shape[:-1], K // MX_BLOCK), dtype=torch.uint8, device=dev)
+        blocks = torch.empty(*shape[:-1], K // 2, dtype=torch.uint8, device=dev)
+        scales = torch.empty(*shape[:-1], K // MX_BLOCK, dtype=torch.uint8, device=dev)
     pitch, unit = x.stride()
     if unit != 1:
         x, pitch = x.contiguous(), K
@@ -213,7 +213,7 @@ def dequantize_mxfp4(blocks, scales, dtype=torch.bfloat16):
         raise TypeError(f"dequantize_mxfp4 returns bfloat16, float16 or float32, not {dtype}")
     _check_packed(blocks, scales, "dequantize_mxfp4")
     blocks, scales = _packed_rows(blocks, 4), scales.contiguous()
-    out = torch.empty((*blocks.shape[:-1], 2 * blocks.shape[-1]), dtype=dtype, device=blocks.device)
+    out = torch.empty(*blocks.shape[:-1], 2 * blocks.shape[-1], dtype=dtype, device=blocks.device)
     rc = _call_on(blocks.device, _gnf4b.load().gnf4b_dequantize_mxfp4, blocks.data_ptr(), scales.data_ptr(), scales.numel(),
                   _X_DTYPES[dtype], out.data_ptr())
     if rc:
@@ -257,15 +257,6 @@ def glu_quantize_mxfp4(gate_up, act: str = "silu", bias=None, row_expert=None):
     return blocks, scales
 
 
-def _tma_ready(blocks):
-    """A weight stack as the product's TMA loads take it: 16-byte aligned, positive strides in multiples of 16 bytes."""
-    E, N, _ = blocks.shape
-    se, sn, unit = blocks.stride()
-    if unit == 1 and blocks.data_ptr() % 16 == 0 and (E == 1 or (se > 0 and se % 16 == 0)) and (N == 1 or (sn > 0 and sn % 16 == 0)):
-        return blocks
-    return _packed_rows(blocks, 16)
-
-
 def gemm_mxfp4_grouped_w4a4(a_blocks, a_scales, blocks, scales, sizes, expert_ids, *, group_offsets=None, max_rows=None):
     """Grouped product of MXFP4 rows with MXFP4 expert stacks: ``out[t] = dequant(a)[t] @ dequant(W[e(t)]).T``, both
     operands multiplied as they are packed, on the block-scaled tensor cores (fp32 accumulation, one rounding to bf16).
@@ -277,29 +268,39 @@ def gemm_mxfp4_grouped_w4a4(a_blocks, a_scales, blocks, scales, sizes, expert_id
     if not a_blocks.is_cuda:
         _require_cuda(a_blocks, "gemm_mxfp4_grouped_w4a4",
                       "The CPU-checkable equivalent multiplies mxfp4_pack_ref.dequant_mxfp4 of both operands per group.")
-    if a_blocks.dim() != 2 or blocks.dim() != 3:
-        raise ValueError(f"a_blocks must be [T, K//2] and blocks [E, N, K//2], got {tuple(a_blocks.shape)} and {tuple(blocks.shape)}")
+    bs, ws = a_blocks.shape, blocks.shape
+    if len(bs) != 2 or len(ws) != 3:
+        raise ValueError(f"a_blocks must be [T, K//2] and blocks [E, N, K//2], got {tuple(bs)} and {tuple(ws)}")
     _check_packed(a_blocks, a_scales, "gemm_mxfp4_grouped_w4a4 (rows)")
     _check_packed(blocks, scales, "gemm_mxfp4_grouped_w4a4 (stack)")
     dev = a_blocks.device
-    T, half = a_blocks.shape
-    E, N, half_w = blocks.shape
+    T, half = bs
+    E, N, half_w = ws
     if blocks.device != dev:
         raise ValueError("rows and stack must live on the same device")
     if half_w != half:
         raise ValueError(f"the rows have K={2 * half} but the stack packs K={2 * half_w}")
     for table in (group_offsets, expert_ids, sizes):
-        if torch.is_tensor(table) and table.is_cuda and table.device != dev:
+        if isinstance(table, torch.Tensor) and table.is_cuda and table.device != dev:
             raise ValueError(f"a group table lives on {table.device}, the rows on {dev}")
-    out = torch.empty((T, N), dtype=torch.bfloat16, device=dev)
+    out = torch.empty(T, N, dtype=torch.bfloat16, device=dev)
     if T == 0 or N == 0 or E == 0:
         return out
-    a_blocks, a_scales, blocks = _packed_rows(a_blocks, 16), a_scales.contiguous(), _tma_ready(blocks)
+    x_p, w_p = a_blocks.data_ptr(), blocks.data_ptr()
+    if x_p % 16 or not a_blocks.is_contiguous():
+        a_blocks = _packed_rows(a_blocks, 16)
+        x_p = a_blocks.data_ptr()
+    a_scales = a_scales.contiguous()
+    # the stack as TMA takes it: 16-byte aligned, positive strides in multiples of 16 bytes
+    w_e, w_n, unit = blocks.stride()
+    if unit != 1 or w_p % 16 or (E > 1 and (w_e <= 0 or w_e % 16)) or (N > 1 and (w_n <= 0 or w_n % 16)):
+        blocks = _packed_rows(blocks, 16)
+        w_p = blocks.data_ptr()
+        w_e, w_n, _ = blocks.stride()
     s_e, s_n, unit = scales.stride()
     if unit != 1:
         scales = scales.contiguous()
         s_e, s_n, _ = scales.stride()
-    w_e, w_n, _ = blocks.stride()
     prev = torch.cuda.current_device()
     if dev.index != prev:
         torch.cuda.set_device(dev)                      # the C library launches on the current device
@@ -309,7 +310,7 @@ def gemm_mxfp4_grouped_w4a4(a_blocks, a_scales, blocks, scales, sizes, expert_id
         if G == 0:
             return out
         rc = _gnf4b.load().gnf4b_gemm_grouped_w4a4(
-            a_blocks.data_ptr(), a_scales.data_ptr(), T, blocks.data_ptr(), w_e, w_n, scales.data_ptr(), s_e, s_n,
+            x_p, a_scales.data_ptr(), T, w_p, w_e, w_n, scales.data_ptr(), s_e, s_n,
             off_t if isinstance(off_t, int) else off_t.data_ptr(), ids_t if isinstance(ids_t, int) else ids_t.data_ptr(), G, E, N,
             2 * half, max_rows, out.data_ptr(), _status_ptr(dev), stream_ptr)
     finally:

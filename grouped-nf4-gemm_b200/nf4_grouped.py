@@ -421,8 +421,10 @@ def _group_tables(sizes, expert_ids, T: int, E: int, dev, group_offsets=None, ma
         if not (torch.is_tensor(group_offsets) and group_offsets.is_cuda and group_offsets.dtype == torch.int32):
             raise TypeError("group_offsets must be a CUDA int32 tensor of G+1 entries")
         G = int(group_offsets.numel()) - 1
-        ids_t = (expert_ids.to(torch.int32).contiguous() if ids_dev
-                 else to_device_i32(([int(v) for v in expert_ids],), dev)[0])
+        if ids_dev:
+            ids_t = (expert_ids if expert_ids.dtype is torch.int32 else expert_ids.to(torch.int32)).contiguous()
+        else:
+            ids_t = to_device_i32(([int(v) for v in expert_ids],), dev)[0]
         if ids_t.numel() != G:
             raise ValueError(f"group_offsets has {G} groups but expert_ids has {ids_t.numel()}")
         return group_offsets.contiguous(), ids_t, G, int(max_rows) if max_rows else -1

@@ -237,7 +237,7 @@ def _glu_backward(ctx, grad_out):
     codes, steps = ctx.saved_tensors
     grad_out = grad_out.contiguous()
     rows = codes.shape[0]
-    grad = torch.empty((rows, 2 * ctx.h), dtype=torch.bfloat16, device=codes.device)
+    grad = torch.empty(rows, 2 * ctx.h, dtype=torch.bfloat16, device=codes.device)
     rc = _call_on(codes.device, _gnf4b.load().gnf4b_glu_ckpt8_bwd, grad_out.data_ptr(), codes.data_ptr(), steps.data_ptr(), rows,
                   ctx.h, ctx.act, grad.data_ptr())
     if rc:

@@ -133,6 +133,22 @@ def test_quantize_views(dtype):
         assert torch.equal(s.cpu(), rs) and torch.equal(b.cpu(), rb), view.shape
 
 
+@pytest.mark.parametrize("shape", [(64,), (0, 32), (2, 0, 96), (1, 1, 1, 32), (3, 2, 2, 64)])
+def test_quantize_and_back_any_rank(shape):
+    x = torch.randn(*shape, generator=gen(31)).to(torch.bfloat16)
+    b, s = M.quantize_mxfp4(x.to(DEV))
+    assert b.shape == (*shape[:-1], shape[-1] // 2) and s.shape == (*shape[:-1], shape[-1] // 32)
+    back = M.dequantize_mxfp4(b, s)
+    assert back.shape == x.shape
+    if x.numel():
+        rb, rs = M.quantize_mxfp4(x.reshape(-1, shape[-1]).to(DEV))
+        assert torch.equal(b.reshape(rb.shape), rb) and torch.equal(back.reshape(-1, shape[-1]), M.dequantize_mxfp4(rb, rs))
+    with pytest.raises(ValueError):
+        M.dequantize_mxfp4(b, s[..., :-1])
+    with pytest.raises(ValueError):
+        M.dequantize_mxfp4(b[None], s)
+
+
 def test_dequantize_every_byte_and_exponent():
     b = torch.arange(256, dtype=torch.uint8).reshape(16, 16).repeat(256, 1)          # every byte under every exponent
     s = torch.arange(256, dtype=torch.uint8).repeat_interleave(16)[:, None]
