@@ -257,6 +257,16 @@ def glu_quantize_mxfp4(gate_up, act: str = "silu", bias=None, row_expert=None):
     return blocks, scales
 
 
+def _refuse_w4a4(a_blocks, a_scales, blocks, scales):
+    if a_blocks.dim() != 2 or blocks.dim() != 3:
+        raise ValueError(f"a_blocks must be [T, K//2] and blocks [E, N, K//2], got {tuple(a_blocks.shape)} and {tuple(blocks.shape)}")
+    _check_packed(a_blocks, a_scales, "gemm_mxfp4_grouped_w4a4 (rows)")
+    _check_packed(blocks, scales, "gemm_mxfp4_grouped_w4a4 (stack)")
+    if blocks.device != a_blocks.device:
+        raise ValueError("rows and stack must live on the same device")
+    raise ValueError(f"the rows have K={2 * a_blocks.shape[1]} but the stack packs K={2 * blocks.shape[2]}")
+
+
 def gemm_mxfp4_grouped_w4a4(a_blocks, a_scales, blocks, scales, sizes, expert_ids, *, group_offsets=None, max_rows=None):
     """Grouped product of MXFP4 rows with MXFP4 expert stacks: ``out[t] = dequant(a)[t] @ dequant(W[e(t)]).T``, both
     operands multiplied as they are packed, on the block-scaled tensor cores (fp32 accumulation, one rounding to bf16).
@@ -268,21 +278,19 @@ def gemm_mxfp4_grouped_w4a4(a_blocks, a_scales, blocks, scales, sizes, expert_id
     if not a_blocks.is_cuda:
         _require_cuda(a_blocks, "gemm_mxfp4_grouped_w4a4",
                       "The CPU-checkable equivalent multiplies mxfp4_pack_ref.dequant_mxfp4 of both operands per group.")
-    bs, ws = a_blocks.shape, blocks.shape
-    if len(bs) != 2 or len(ws) != 3:
-        raise ValueError(f"a_blocks must be [T, K//2] and blocks [E, N, K//2], got {tuple(bs)} and {tuple(ws)}")
-    _check_packed(a_blocks, a_scales, "gemm_mxfp4_grouped_w4a4 (rows)")
-    _check_packed(blocks, scales, "gemm_mxfp4_grouped_w4a4 (stack)")
-    dev = a_blocks.device
-    T, half = bs
-    E, N, half_w = ws
-    if blocks.device != dev:
-        raise ValueError("rows and stack must live on the same device")
-    if half_w != half:
-        raise ValueError(f"the rows have K={2 * half} but the stack packs K={2 * half_w}")
+    u8, index = torch.uint8, a_blocks.get_device()
+    xb, xs, wb, ws = a_blocks.shape, a_scales.shape, blocks.shape, scales.shape
+    if not (a_blocks.dtype is u8 and a_scales.dtype is u8 and blocks.dtype is u8 and scales.dtype is u8
+            and len(xb) == len(xs) == 2 and len(wb) == len(ws) == 3 and xb[0] == xs[0] and wb[0] == ws[0] and wb[1] == ws[1]
+            and wb[2] == xb[1] == 16 * xs[1] > 0 and ws[2] == xs[1]
+            and a_scales.get_device() == blocks.get_device() == scales.get_device() == index):
+        _refuse_w4a4(a_blocks, a_scales, blocks, scales)
     for table in (group_offsets, expert_ids, sizes):
-        if isinstance(table, torch.Tensor) and table.is_cuda and table.device != dev:
-            raise ValueError(f"a group table lives on {table.device}, the rows on {dev}")
+        if isinstance(table, torch.Tensor) and table.is_cuda and table.get_device() != index:
+            raise ValueError(f"a group table lives on {table.device}, the rows on {a_blocks.device}")
+    T, half = xb
+    E, N, _ = wb
+    dev = a_blocks.device
     out = torch.empty(T, N, dtype=torch.bfloat16, device=dev)
     if T == 0 or N == 0 or E == 0:
         return out
@@ -302,7 +310,7 @@ def gemm_mxfp4_grouped_w4a4(a_blocks, a_scales, blocks, scales, sizes, expert_id
         scales = scales.contiguous()
         s_e, s_n, _ = scales.stride()
     prev = torch.cuda.current_device()
-    if dev.index != prev:
+    if index != prev:
         torch.cuda.set_device(dev)                      # the C library launches on the current device
     try:
         stream_ptr = _raw_stream(dev)
@@ -314,7 +322,7 @@ def gemm_mxfp4_grouped_w4a4(a_blocks, a_scales, blocks, scales, sizes, expert_id
             off_t if isinstance(off_t, int) else off_t.data_ptr(), ids_t if isinstance(ids_t, int) else ids_t.data_ptr(), G, E, N,
             2 * half, max_rows, out.data_ptr(), _status_ptr(dev), stream_ptr)
     finally:
-        if dev.index != prev:
+        if index != prev:
             torch.cuda.set_device(prev)
     if rc:
         _gnf4b.check(rc, "gnf4b_gemm_grouped_w4a4")
