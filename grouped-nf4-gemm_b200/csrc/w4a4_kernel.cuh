@@ -496,8 +496,9 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
         const int64_t kb = a.K / 32;
         const uint8_t* w_hi = a.ws + (int64_t)(a.E - 1) * a.ws_se + (a.N - 1) * a.ws_sn + kb;
         const uint8_t* x_hi = a.xs + a.T * kb;
-        const bool aligned = ((reinterpret_cast<uintptr_t>(a.ws) | reinterpret_cast<uintptr_t>(a.xs) | (uintptr_t)kb | (uintptr_t)a.ws_sn |
-                               (uintptr_t)a.ws_se) & 15) == 0;     // every row starts on 16 bytes
+        const uintptr_t places = reinterpret_cast<uintptr_t>(a.ws) | reinterpret_cast<uintptr_t>(a.xs) | (uintptr_t)kb | (uintptr_t)a.ws_sn |
+                                 (uintptr_t)a.ws_se;
+        const bool aligned = (places & 15) == 0, aligned8 = (places & 7) == 0;       // every row starts on 16 / on 8 bytes
         const int spans = (a.k_stages + 3) >> 2;
         int32_t g = 0;
         QItem it;
@@ -557,7 +558,9 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
                     const uint4* q = reinterpret_cast<const uint4*>(p - at[o]);
                     uint4 v0, v1, v2;
                     if (sp < inside[o]) {
-                        v0 = __ldg(q); v1 = __ldg(q + 1); v2 = __ldg(q + 2);
+                        v0 = __ldg(q); v1 = __ldg(q + 1);
+                        v2 = make_uint4(0, 0, 0, 0);          // (not v1, which would have to arrive first)
+                        if (valid + (aligned8 ? 8 : 15) > 32) v2 = __ldg(q + 2);
                     } else {
                         const bool w = sw + o * kQScaleWarps < 4;
                         const uint8_t* lo = w ? a.ws : a.xs;
@@ -591,6 +594,9 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
                 if (aligned && valid >= 32) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) out[o][j] = raw[o][j];
+                } else if (aligned8) {                      // 120 cycles instead of 270 a block
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) out[o][j] = 4 * j < valid ? ((raw_at[o] & 8) ? raw[o][j + 2] : raw[o][j]) : 0u;
                 } else {
                     align_scale_row(raw[o], raw_at[o], valid, out[o]);
                 }
