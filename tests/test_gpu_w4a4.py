@@ -331,6 +331,23 @@ def test_product_extreme_scales_and_nan():
     assert torch.isnan(nan[1]).all() and torch.isfinite(nan[[0, 2, 3, 4]]).all()
 
 
+@pytest.mark.parametrize("max_rows,K,N,G", [(3, 64, 20480, 256), (3, 1344, 20480, 256), (400, 1344, 40960, 130)])
+def test_product_hundreds_of_items_per_sm(max_rows, K, N, G):
+    """More than 256 items for every SM (and SM pair, the last case)."""
+    wb, ws = packed((2, N), K, 60)
+    xb, xs = packed((2 * G,), K, 61)
+    sizes = [(1, 3, 2)[i % 3] for i in range(G)]
+    ids = [i % 2 for i in range(G)]
+    T = sum(sizes)
+    xb, xs = xb[:T].contiguous(), xs[:T].contiguous()
+    off = torch.tensor([0, *torch.tensor(sizes).cumsum(0).tolist()], dtype=torch.int32, device=DEV)
+    out = M.gemm_mxfp4_grouped_w4a4(xb, xs, wb, ws, None, torch.tensor(ids, device=DEV), group_offsets=off, max_rows=max_rows)
+    expert = torch.tensor(ids).repeat_interleave(torch.tensor(sizes)).to(DEV)
+    for e in range(2):                                     # all of an expert's rows as one group: the same sums
+        rows = torch.nonzero(expert == e).reshape(-1)
+        assert torch.equal(out[rows], M.gemm_mxfp4_grouped_w4a4(xb[rows], xs[rows], wb, ws, [len(rows)], [e]))
+
+
 def test_product_beyond_32_bit_offsets():
     """A stack of more than 4 GiB: the last expert against its own copy."""
     E, N, K = 300, 4096, 7168
