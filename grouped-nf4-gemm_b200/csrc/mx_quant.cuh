@@ -186,7 +186,7 @@ mx_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restri
 #pragma unroll
     for (int k = 0; k < U; ++k) {
         const int64_t i = first + k * kMxThreads;
-        if (i >= items) break;
+        if (OT != 2 && i >= items) break;
         float f[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -195,9 +195,17 @@ mx_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restri
             f[2 * j + 1] = __fmul_rn(p.y + p.y, sc[k]);
         }
         if (OT == 2) {
-            float4* o = static_cast<float4*>(out) + 2 * i;
-            __stcs(o, make_float4(f[0], f[1], f[2], f[3]));
-            __stcs(o + 1, make_float4(f[4], f[5], f[6], f[7]));
+            // two lanes hold 16 numbers and store one lane's eight after the other's, so that a store writes whole
+            // 32-byte sectors (1237 x 7168: 11.8 us with half sectors)
+            const bool odd = threadIdx.x & 1;
+            float g[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) g[j] = __shfl_xor_sync(0xffffffffu, odd ? f[j] : f[4 + j], 1);
+            if (i < items) {                          // items come in fours: both lanes or none
+                float4* o = static_cast<float4*>(out) + 2 * (i - odd) + odd;
+                __stcs(o, odd ? make_float4(g[0], g[1], g[2], g[3]) : make_float4(f[0], f[1], f[2], f[3]));
+                __stcs(o + 2, odd ? make_float4(f[4], f[5], f[6], f[7]) : make_float4(g[0], g[1], g[2], g[3]));
+            }
         } else {
             uint32_t w[4];
 #pragma unroll
