@@ -24,12 +24,10 @@ CKPT_BLOCK = 64                     # values per scale of the 8-bit checkpoint
 CKPT_TINY = 2.0 ** -100             # a block whose largest magnitude is below this is held as zeros
 
 
-PACKAGE = str(Path(__file__).resolve().parents[1] / "grouped-nf4-gemm_b200")
-
-
 def _package():
-    if PACKAGE not in sys.path:
-        sys.path.insert(0, PACKAGE)
+    root = str(Path(__file__).resolve().parents[1] / "grouped-nf4-gemm_b200")
+    if root not in sys.path:
+        sys.path.insert(0, root)
 
 
 # ------------------------------------------------------------------------------------------------ cases
