@@ -292,8 +292,10 @@ def gemm_mxfp4_grouped_w4a4(a_blocks, a_scales, blocks, scales, sizes, expert_id
     E, N, _ = wb
     dev = a_blocks.device
     out = torch.empty(T, N, dtype=torch.bfloat16, device=dev)
-    if T == 0 or N == 0 or E == 0:
+    if T == 0 or N == 0:
         return out
+    if E == 0:
+        raise ValueError(f"the stack holds no experts, but there are {T} rows")
     x_p, w_p = a_blocks.data_ptr(), blocks.data_ptr()
     if x_p % 16 or not a_blocks.is_contiguous():
         a_blocks = _packed_rows(a_blocks, 16)
