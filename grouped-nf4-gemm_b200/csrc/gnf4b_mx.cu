@@ -104,9 +104,10 @@ int gnf4b_gemm_grouped_w4a4(const uint8_t* x_blocks, const uint8_t* x_scales, in
     if (!x_blocks || !x_scales || !W || !S || !group_offsets || !expert_ids || !out) return GNF4B_EINVAL;
     if (s_stride_e < 0 || s_stride_n < 0) return GNF4B_EINVAL;
     if (!aligned(out, 4)) return GNF4B_EINVAL;
-    // TMA: 16-byte aligned bases and positive strides in multiples of 16 bytes (K / 2 is one: K is a multiple of 32)
-    if (!aligned(x_blocks, 16) || !aligned(W, 16) || w_stride_n % 16 || w_stride_e % 16 || (N > 1 && w_stride_n <= 0) ||
-        (E > 1 && w_stride_e <= 0))
+    // TMA: 16-byte aligned bases and positive strides in multiples of 16 bytes (K / 2 is one: K is a multiple of 32); the
+    // stride of a dimension of one is not used
+    if (!aligned(x_blocks, 16) || !aligned(W, 16) || (N > 1 && (w_stride_n <= 0 || w_stride_n % 16)) ||
+        (E > 1 && (w_stride_e <= 0 || w_stride_e % 16)))
         return GNF4B_EUNSUPPORTED;
     DevInfo di;
     const int rc = device_info(&di);

@@ -459,8 +459,8 @@ int gnf4b_glu_quantize_mxfp4(const void* gate_up, int64_t rows, int64_t h, int a
  * on the block-scaled tensor cores, nothing decoded.  x_blocks [T, K/2] and x_scales [T, K/32] contiguous, rows sorted
  * by group; W / S, group_offsets, expert_ids, max_rows, status_word as in gnf4b_gemm_grouped with GNF4B_FMT_MXFP4
  * (max_rows only shapes the tiles here: understating it costs speed, not rows).  x_blocks and W start on 16 bytes and
- * W's strides are positive multiples of 16 bytes (GNF4B_EUNSUPPORTED otherwise); the scales may have any alignment and
- * any non-negative strides; T and N up to 2^31 - 257.  A scale byte of 255 is NaN here, as the OCP format defines it.
+ * W's strides are positive multiples of 16 bytes (GNF4B_EUNSUPPORTED otherwise; the stride of a dimension of one is not
+ * used); the scales may have any alignment and any non-negative strides; T and N up to 2^31 - 257.  A scale byte of 255 is NaN here, as the OCP format defines it.
  * Rows that belong to no group, or to a padding group, are left as they were. */
 int gnf4b_gemm_grouped_w4a4(const uint8_t* x_blocks, const uint8_t* x_scales, int64_t T,
                             const uint8_t* W, int64_t w_stride_e, int64_t w_stride_n,
