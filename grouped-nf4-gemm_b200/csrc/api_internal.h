@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <mutex>
+
 namespace gnf4b {
 
 struct DevInfo {
@@ -21,13 +23,19 @@ static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 
 // cudaFuncSetAttribute is per device and not free; raise a kernel's dynamic shared-memory
-// limit only when a launch needs more than was already granted on this device.
+// limit only when a launch needs more than was already granted on this device.  One thread at a time: a smaller limit
+// set between another thread's larger one and its record would leave a record of more than the kernel has.
+inline std::mutex& smem_limit_mutex() {
+    static std::mutex mu;
+    return mu;
+}
 template <typename F>
 static cudaError_t ensure_smem(F kfn, size_t smem, int* granted /*[64], zero-initialised*/) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     dev &= 63;
+    std::lock_guard<std::mutex> lock(smem_limit_mutex());
     if ((int)smem > granted[dev]) {
         e = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
