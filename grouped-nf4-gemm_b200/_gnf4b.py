@@ -157,6 +157,8 @@ def _declare(lib):
     lib.gnf4b_glu_quantize_mxfp4.argtypes = [vp, i64, i64, C.c_int, vp, vp, i32, vp, vp, vp, vp]
     lib.gnf4b_gemm_grouped_w4a4.restype = C.c_int
     lib.gnf4b_gemm_grouped_w4a4.argtypes = [vp, vp, i64, vp, i64, i64, vp, i64, i64, vp, vp, i32, i32, i64, i64, i32, vp, vp, vp]
+    lib.gnf4b_w4a4_plan.restype = C.c_int
+    lib.gnf4b_w4a4_plan.argtypes = [i64, i32, i64, i64, i32, i32, i32, vp]
     lib.gnf4b_route_train_scratch_bytes.restype = sz
     lib.gnf4b_route_train_scratch_bytes.argtypes = [i64, i32]
     lib.gnf4b_route_train_fwd.restype = C.c_int
@@ -191,6 +193,7 @@ EXPORTS = ("gnf4b_abi_version", "gnf4b_strerror", "gnf4b_last_cuda_error", "gnf4
            "gnf4b_gather_rows_by_id", "gnf4b_gather_rows_addr", "gnf4b_ep_plan_large", "gnf4b_ep_plan_large_scratch_bytes",
            "gnf4b_ep_push_blocks", "gnf4b_ep_wait_flags",
            "gnf4b_quantize_mxfp4", "gnf4b_dequantize_mxfp4", "gnf4b_glu_quantize_mxfp4", "gnf4b_gemm_grouped_w4a4",
+           "gnf4b_w4a4_plan",
            "gnf4b_route_train_scratch_bytes", "gnf4b_route_train_fwd", "gnf4b_route_train_bwd", "gnf4b_glu_ckpt8_fwd",
            "gnf4b_glu_ckpt8_bwd",
            "gnf4b_device_info")

@@ -92,6 +92,19 @@ int gnf4b_glu_quantize_mxfp4(const void* gate_up, int64_t rows, int64_t h, int a
     return e == cudaSuccess ? GNF4B_OK : cuda_fail(e, "glu_quantize_mxfp4 launch");
 }
 
+int gnf4b_w4a4_plan(int64_t T, int32_t G, int64_t N, int64_t K, int32_t max_rows, int32_t sm_count, int32_t smem_optin,
+                    int32_t* plan) {
+    if (T <= 0 || G <= 0 || sm_count <= 0 || smem_optin <= 0 || !plan) return GNF4B_EINVAL;
+    if (N <= 0 || K <= 0 || K % 32) return GNF4B_ESHAPE;
+    if (T > INT32_MAX - 256 || N > INT32_MAX - 256 || K > INT32_MAX) return GNF4B_ETOOBIG;
+    const W4A4Plan p = w4a4_plan(T, G, N, K, max_rows, sm_count, smem_optin);
+    if (p.stages < 2) return GNF4B_EUNSUPPORTED;
+    const int32_t fields[GNF4B_W4A4_PLAN_FIELDS] = {p.pair, p.rows_w, p.tok_cap, p.xbox, p.x_bytes, p.x_blocks, p.stages, p.acc_bufs,
+                                                    (int32_t)p.smem};
+    std::copy(fields, fields + GNF4B_W4A4_PLAN_FIELDS, plan);
+    return GNF4B_OK;
+}
+
 int gnf4b_gemm_grouped_w4a4(const uint8_t* x_blocks, const uint8_t* x_scales, int64_t T, const uint8_t* W, int64_t w_stride_e,
                             int64_t w_stride_n, const uint8_t* S, int64_t s_stride_e, int64_t s_stride_n, const int32_t* group_offsets,
                             const int32_t* expert_ids, int32_t G, int32_t E, int64_t N, int64_t K, int32_t max_rows, void* out,
@@ -116,6 +129,7 @@ int gnf4b_gemm_grouped_w4a4(const uint8_t* x_blocks, const uint8_t* x_scales, in
     if (!enc) return GNF4B_EUNSUPPORTED;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
     const W4A4Plan p = w4a4_plan(T, G, N, K, max_rows, di.sm_count, di.smem_optin);
+    if (p.stages < 2) return GNF4B_EUNSUPPORTED;
     // items are numbered in 31 bits (a group adds at most one chunk beyond its share)
     if ((ceil_div(T, 16) + G) * ceil_div(N, p.rows_w) > INT32_MAX) return GNF4B_ETOOBIG;
     W4A4Args a;

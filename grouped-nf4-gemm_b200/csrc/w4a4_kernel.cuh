@@ -742,7 +742,8 @@ struct W4A4Plan {
     size_t smem;
 };
 
-// Tile shape from the row counts alone.  max_rows <= 0: unknown, any group may be long.
+// Tile shape from the row counts alone.  max_rows <= 0: unknown, any group may be long.  Fewer than two stages: the device
+// has too little shared memory.
 static inline W4A4Plan w4a4_plan(int64_t T, int32_t G, int64_t N, int64_t K, int32_t max_rows, int sm_count, int smem_optin) {
     W4A4Plan p;
     const int64_t longest = max_rows > 0 ? (max_rows < T ? max_rows : T) : T;
@@ -768,11 +769,11 @@ static inline W4A4Plan w4a4_plan(int64_t T, int32_t G, int64_t N, int64_t K, int
         p.xbox = 64;
         p.x_bytes = (int)round_up(p.tok_cap / 2, p.xbox) * kQRowBytes;
     }
-    const size_t room = (size_t)smem_optin - w4a4_fixed_bytes(p.x_blocks);
+    const size_t fixed = w4a4_fixed_bytes(p.x_blocks), room = (size_t)smem_optin > fixed ? (size_t)smem_optin - fixed : 0;
     p.stages = (int)(room / (size_t)(kQWTile + p.x_bytes));
     if (p.stages > kQMaxStages) p.stages = kQMaxStages;
     p.acc_bufs = 2 * p.tok_cap + p.stages * 8 * (1 + p.x_blocks) <= kQTmemCols ? 2 : 1;
-    p.smem = w4a4_fixed_bytes(p.x_blocks) + (size_t)p.stages * (kQWTile + p.x_bytes);
+    p.smem = fixed + (size_t)p.stages * (kQWTile + p.x_bytes);
     return p;
 }
 

@@ -467,6 +467,13 @@ int gnf4b_gemm_grouped_w4a4(const uint8_t* x_blocks, const uint8_t* x_scales, in
                             const uint8_t* S, int64_t s_stride_e, int64_t s_stride_n,
                             const int32_t* group_offsets, const int32_t* expert_ids, int32_t G, int32_t E,
                             int64_t N, int64_t K, int32_t max_rows, void* out, int32_t* status_word, void* cuda_stream);
+/* The tiles that call would use on a GPU of sm_count SMs with smem_optin bytes of opt-in shared memory (no device needed):
+ * [0] 1 = CTA pairs, [1] weight rows per item and CTA, [2] activation rows per item, at most, [3] activation rows per load,
+ * [4] bytes of a stage's activations in a CTA, [5] 128-row blocks of activation scales, [6] stages, [7] accumulators,
+ * [8] bytes of shared memory of a CTA. */
+#define GNF4B_W4A4_PLAN_FIELDS 9
+int gnf4b_w4a4_plan(int64_t T, int32_t G, int64_t N, int64_t K, int32_t max_rows, int32_t sm_count, int32_t smem_optin,
+                    int32_t* plan);
 
 /* Routing for training.  Selection and weights as gnf4b_route_topk, on logits [T, E] of bf16, fp16 or fp32 (rows `stride`
  * elements apart; E <= 1024, k <= 32), with what a training step needs beside them.  Over the n tokens that count (all,
