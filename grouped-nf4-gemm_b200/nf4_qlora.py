@@ -78,6 +78,17 @@ def gemm_4bit_grouped_train(a_cat, packed, absmax, sizes, expert_ids, weights_fn
     return FusedGroupedNf4.apply(a_cat, packed, absmax, sizes, expert_ids, weights_fn, dgrad_kernel)
 
 
+def _dgrad_mxfp4(grad_out, blocks, scales, sizes, expert_ids):
+    """``dgrad_mxfp4_grouped`` for any N: its kernel takes multiples of 8 (16-byte rows of ``grad_out``), other widths are
+    filled up with columns of zeros against rows of zeros."""
+    from mxfp4_grouped import dgrad_mxfp4_grouped
+    fill = -blocks.shape[1] % 8
+    if fill:
+        grad_out = torch.nn.functional.pad(grad_out, (0, fill))
+        blocks, scales = (torch.nn.functional.pad(t, (0, 0, 0, fill)) for t in (blocks, scales))
+    return dgrad_mxfp4_grouped(grad_out.contiguous(), blocks, scales, sizes, expert_ids)
+
+
 class FusedGroupedMxfp4(torch.autograd.Function):
     """The MXFP4 counterpart: forward ``gemm_mxfp4_grouped``, backward ``dgrad_mxfp4_grouped``."""
 
@@ -92,9 +103,7 @@ class FusedGroupedMxfp4(torch.autograd.Function):
     def backward(ctx, grad_out):
         if not ctx.needs_input_grad[0]:
             return (None,) * 5
-        from mxfp4_grouped import dgrad_mxfp4_grouped
-        blocks, scales = ctx.stack
-        return (dgrad_mxfp4_grouped(grad_out.contiguous(), blocks, scales, ctx.sizes, ctx.expert_ids),) + (None,) * 4
+        return (_dgrad_mxfp4(grad_out, *ctx.stack, ctx.sizes, ctx.expert_ids),) + (None,) * 4
 
 
 def gemm_mxfp4_grouped_train(a_cat, blocks, scales, sizes, expert_ids):
@@ -183,10 +192,7 @@ class FusedGroupedMxfp4W4A4(torch.autograd.Function):
     def backward(ctx, grad_out):
         if not ctx.needs_input_grad[0]:
             return (None,) * 5
-        from mxfp4_grouped import dgrad_mxfp4_grouped
-        blocks, scales = ctx.stack
-        grad = dgrad_mxfp4_grouped(grad_out.contiguous(), blocks, scales, ctx.sizes, ctx.expert_ids)
-        return (grad.to(ctx.a_dtype),) + (None,) * 4
+        return (_dgrad_mxfp4(grad_out, *ctx.stack, ctx.sizes, ctx.expert_ids).to(ctx.a_dtype),) + (None,) * 4
 
 
 def gemm_mxfp4_grouped_w4a4_train(a_cat, blocks, scales, sizes, expert_ids):
