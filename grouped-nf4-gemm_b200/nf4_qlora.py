@@ -31,6 +31,31 @@ def _host_ints(v):
     return [int(x) for x in (v.tolist() if torch.is_tensor(v) else v)]
 
 
+class _FirstOnly(torch.autograd.Function):
+    """Identity behind a kernel's gradient: a second derivative through it is refused when it is asked for, instead of coming
+    back without this term."""
+
+    @staticmethod
+    def forward(ctx, grad, what):
+        ctx.what = what
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, _grad):
+        raise RuntimeError(f"the gradient of {ctx.what} is a kernel's result: it cannot be differentiated a second time")
+
+
+def first_derivative_only(grad, what: str):
+    """``grad`` as a backward pass under ``create_graph=True`` returns it, see ``_FirstOnly``."""
+    return _FirstOnly.apply(grad.detach().requires_grad_(), what)
+
+
+def _product_gradient(dgrad, what, grad_out, *stack_and_groups):
+    """``dgrad(grad_out, ...)``.  The product is linear in its rows: its gradient depends on ``grad_out`` alone."""
+    grad = dgrad(grad_out, *stack_and_groups)
+    return first_derivative_only(grad, what) if torch.is_grad_enabled() and grad_out.requires_grad else grad
+
+
 class FusedGroupedNf4(torch.autograd.Function):
     """``out = gemm_4bit_grouped(a_cat, packed, absmax, sizes, expert_ids)`` with
     ``grad_a = dgrad_4bit_grouped(grad_out, ...)``.
@@ -61,7 +86,8 @@ class FusedGroupedNf4(torch.autograd.Function):
         packed, absmax = ctx.stack if ctx.weights_fn is None else ctx.weights_fn()
         grad_out = grad_out.contiguous()
         if ctx.use_kernel and packed.device == grad_out.device and dgrad_eligible(grad_out, packed, absmax) is None:
-            return (dgrad_4bit_grouped(grad_out, packed, absmax, ctx.sizes, ctx.expert_ids),) + (None,) * 6
+            return (_product_gradient(dgrad_4bit_grouped, "gemm_4bit_grouped_train", grad_out, packed, absmax, ctx.sizes, ctx.expert_ids),
+                    *(None,) * 6)
         n_out, k_in = packed.shape[1], packed.shape[2] * 2
         grad_a = torch.zeros(grad_out.shape[0], k_in, dtype=grad_out.dtype, device=grad_out.device)
         first = 0
@@ -103,7 +129,8 @@ class FusedGroupedMxfp4(torch.autograd.Function):
     def backward(ctx, grad_out):
         if not ctx.needs_input_grad[0]:
             return (None,) * 5
-        return (_dgrad_mxfp4(grad_out, *ctx.stack, ctx.sizes, ctx.expert_ids),) + (None,) * 4
+        return (_product_gradient(_dgrad_mxfp4, "gemm_mxfp4_grouped_train", grad_out, *ctx.stack, ctx.sizes, ctx.expert_ids),
+                *(None,) * 4)
 
 
 def gemm_mxfp4_grouped_train(a_cat, blocks, scales, sizes, expert_ids):
@@ -192,7 +219,8 @@ class FusedGroupedMxfp4W4A4(torch.autograd.Function):
     def backward(ctx, grad_out):
         if not ctx.needs_input_grad[0]:
             return (None,) * 5
-        return (_dgrad_mxfp4(grad_out, *ctx.stack, ctx.sizes, ctx.expert_ids).to(ctx.a_dtype),) + (None,) * 4
+        grad = _product_gradient(_dgrad_mxfp4, "gemm_mxfp4_grouped_w4a4_train", grad_out, *ctx.stack, ctx.sizes, ctx.expert_ids)
+        return (grad.to(ctx.a_dtype),) + (None,) * 4
 
 
 def gemm_mxfp4_grouped_w4a4_train(a_cat, blocks, scales, sizes, expert_ids):

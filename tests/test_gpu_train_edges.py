@@ -53,3 +53,36 @@ def test_ffn_gradient_with_an_odd_result_width():
         y = Q.ffn_mxfp4_grouped_train(x, *gu, *dn, sizes, ids, rows=rows)
         y.float().square().sum().backward()
         assert y.shape == (9, N) and torch.isfinite(x.grad).all() and x.grad.abs().amax(1).all()
+
+
+PRODUCTS = ["gemm_4bit_grouped_train", "gemm_mxfp4_grouped_train", "gemm_mxfp4_grouped_w4a4_train"]
+
+
+@pytest.mark.parametrize("product", PRODUCTS)
+def test_second_derivatives_of_products_are_refused_where_they_exist(product):
+    g = gen(3)
+    stack = (synth.nf4_stack if "4bit" in product else synth.mxfp4_stack)(2, 64, 128, g, device=DEV)
+    x = torch.randn(6, 128, generator=g).to(torch.bfloat16).to(DEV).requires_grad_()
+    y = getattr(Q, product)(x, *stack, [2, 4], [1, 0])
+    want, = torch.autograd.grad(y.float().square().sum(), x, retain_graph=True)
+    grad, = torch.autograd.grad(y.float().square().sum(), x, create_graph=True)
+    assert torch.equal(grad, want)
+    with pytest.raises(RuntimeError, match=product):          # a penalty beside a term that has a gradient of its own
+        (grad.float().square().sum() + x.float().sum()).backward()
+    # an incoming gradient that is a constant: the product's own gradient is one too
+    x.grad = None                                             # the sum's part got there before the refusal
+    y = getattr(Q, product)(x, *stack, [2, 4], [1, 0])
+    grad, = torch.autograd.grad(y, x, torch.ones_like(y), create_graph=True)
+    (grad.float().square().sum() + x.float().sum()).backward()
+    assert torch.equal(x.grad, torch.ones_like(x))
+
+
+def test_the_loop_of_the_nf4_gradient_stays_differentiable():
+    g = gen(4)
+    stack = synth.nf4_stack(2, 64, 128, g, device=DEV)
+    x = torch.randn(6, 128, generator=g).to(torch.bfloat16).to(DEV).requires_grad_()
+    y = Q.gemm_4bit_grouped_train(x, *stack, [2, 4], [1, 0], dgrad_kernel=False)
+    go = torch.randn(6, 64, generator=g).to(torch.bfloat16).to(DEV).requires_grad_()
+    grad, = torch.autograd.grad(y, x, go, create_graph=True)
+    grad.float().sum().backward()
+    assert go.grad is not None and go.grad.abs().sum() > 0
