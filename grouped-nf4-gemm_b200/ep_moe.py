@@ -156,9 +156,11 @@ class _RouteTopkTrain(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, _g_idx, g_w, _g_counts, g_balance, g_z):
-        if torch.is_grad_enabled():                 # create_graph=True: the gradient is no graph
-            return _route_backward_once(ctx, g_w, g_balance, g_z)
-        return _route_backward(ctx, g_w, g_balance, g_z)
+        grad = _route_backward(ctx, g_w, g_balance, g_z)
+        if torch.is_grad_enabled():                 # create_graph=True: the gradient depends on the logits, whatever comes in
+            from nf4_qlora import first_derivative_only
+            grad = first_derivative_only(grad, "route_topk_train")
+        return grad, None, None, None, None
 
 
 def _route_backward(ctx, g_w, g_balance, g_z):
@@ -178,10 +180,9 @@ def _route_backward(ctx, g_w, g_balance, g_z):
                   None if g_z is None else g_z.data_ptr(), grad.data_ptr())
     if rc:
         _gnf4b.check(rc, "gnf4b_route_train_bwd")
-    return grad, None, None, None, None
+    return grad
 
 
-_route_backward_once = torch.autograd.function.once_differentiable(_route_backward)
 _ROUTE_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}        # GNF4B_X_*
 ROUTE_TRAIN_MAX_EXPERTS, ROUTE_TRAIN_MAX_K = 1024, 32
 

@@ -260,9 +260,9 @@ class _GluTrain(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_out):
-        if torch.is_grad_enabled():                 # create_graph=True: the gradient is no graph
-            return _glu_backward_once(ctx, grad_out)
-        return _glu_backward(ctx, grad_out)
+        grad = _glu_backward(ctx, grad_out)
+        # create_graph=True: the gradient depends on gate_up, whatever comes in
+        return (first_derivative_only(grad, "glu_train") if torch.is_grad_enabled() else grad), None, None, None
 
 
 def _glu_backward(ctx, grad_out):
@@ -276,10 +276,7 @@ def _glu_backward(ctx, grad_out):
                   ctx.h, ctx.act, grad.data_ptr())
     if rc:
         _gnf4b.check(rc, "gnf4b_glu_ckpt8_bwd")
-    return grad, None, None, None
-
-
-_glu_backward_once = torch.autograd.function.once_differentiable(_glu_backward)
+    return grad
 
 
 def glu_train(gate_up, act: str = "silu", *, bias=None, row_expert=None):

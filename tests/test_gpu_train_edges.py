@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-import mxfp4_grouped as M
+import ep_moe
 import nf4_qlora as Q
 import synth
 from mxfp4_pack_ref import dequant_mxfp4
@@ -86,3 +86,23 @@ def test_the_loop_of_the_nf4_gradient_stays_differentiable():
     grad, = torch.autograd.grad(y, x, go, create_graph=True)
     grad.float().sum().backward()
     assert go.grad is not None and go.grad.abs().sum() > 0
+
+
+# ------------------------------------------------------------------------------------------------ second derivatives
+def test_second_derivatives_are_refused_beside_other_terms():
+    """A penalty on a gradient, beside a term whose gradient is a graph: the part through the kernel must not go missing."""
+    x = torch.randn(8, 16, generator=gen(5)).to(DEV).requires_grad_()
+    r = ep_moe.route_topk_train(x, 2)
+    for out in (r.balance_loss, r.z_loss, r.weights):
+        want, = torch.autograd.grad(out, x, torch.ones_like(out), retain_graph=True)
+        grad, = torch.autograd.grad(out, x, torch.ones_like(out), create_graph=True)
+        assert torch.equal(grad, want)
+        with pytest.raises(RuntimeError, match="route_topk_train"):
+            (grad.square().sum() + x.sum()).backward()
+    gu = torch.randn(4, 64, generator=gen(6)).to(torch.bfloat16).to(DEV).requires_grad_()
+    out = Q.glu_train(gu)
+    want, = torch.autograd.grad(out, gu, torch.ones_like(out), retain_graph=True)
+    grad, = torch.autograd.grad(out, gu, torch.ones_like(out), create_graph=True)
+    assert torch.equal(grad, want)
+    with pytest.raises(RuntimeError, match="glu_train"):
+        (grad.float().square().sum() + gu.float().sum()).backward()
