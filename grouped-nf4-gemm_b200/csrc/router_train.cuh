@@ -29,8 +29,8 @@
 //
 // Measured at 65536 tokens x 256 experts, top 8, fp32 (67 MB of logits, 10 us of reading): forward 50 us, about 500
 // instructions a token at 71 % of the issue slots and 10 us of launches and joining (115 us with k scans, and 27 to 66 us more for
-// a second kernel over the CTAs' sums); backward 34 us, 300 instructions at 53 % (42 us with 24 instead of 32 warps per SM;
-// 20 us would be the bytes).  65536 x 32 bf16, top 4: 27 and 12 us.
+// a second kernel over the CTAs' sums); backward 35 us, about 320 instructions at 53 % (42 us with 24 instead of 32 warps per
+// SM; 20 us would be the bytes; 34 without the sum that corrects lse).  65536 x 32 bf16, top 4: 28.7 and 13.4 us (12.3 without).
 #pragma once
 
 #include "common.cuh"
@@ -524,10 +524,13 @@ route_train_bwd_kernel(const __grid_constant__ RouteTrainBwdArgs a) {
         const bool dead = lse == -INFINITY;
         const bool counted = !dead && keep_n;
         const bool has = e_sel >= 0 && e_sel < a.E;
-        float p[NE], ap = 0.f;
+        // lse in one fp32 number is off by up to half its last place, 5e-4 where the logits are around 10000, and by the same
+        // for every expert of the token: dividing by the sum of what it gives, which lies near 1, takes that factor out
+        float p[NE], ap = 0.f, z = 0.f;
 #pragma unroll
         for (int i = 0; i < NE; ++i) {
             p[i] = dead ? 0.f : rt_exp(v[i] - lse);
+            z += p[i];
             ap = fmaf(p[i], push[i], ap);
         }
         if (t + step < a.T) load(t + step);
@@ -539,7 +542,12 @@ route_train_bwd_kernel(const __grid_constant__ RouteTrainBwdArgs a) {
         for (int o = 16; o > 0; o >>= 1) {
             gw += __shfl_xor_sync(0xffffffffu, gw, o);
             ap += __shfl_xor_sync(0xffffffffu, ap, o);
+            z += __shfl_xor_sync(0xffffffffu, z, o);
         }
+        const float rz = dead ? 0.f : rt_rcp(z);
+        ap *= rz;
+#pragma unroll
+        for (int i = 0; i < NE; ++i) p[i] *= rz;
         if (through_w && has) mine[e_sel] = renorm ? w * (g - gw) : g;
         __syncwarp();
         const float zc = gz * lse - ap;

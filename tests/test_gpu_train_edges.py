@@ -6,6 +6,7 @@ import ep_moe
 import nf4_qlora as Q
 import synth
 from mxfp4_pack_ref import dequant_mxfp4
+from test_gpu_train_ops import check_routing
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -86,6 +87,37 @@ def test_the_loop_of_the_nf4_gradient_stays_differentiable():
     grad, = torch.autograd.grad(y, x, go, create_graph=True)
     grad.float().sum().backward()
     assert go.grad is not None and go.grad.abs().sum() > 0
+
+
+# ------------------------------------------------------------------------------------------------ routing
+@pytest.mark.parametrize("mode,norm", [(0, False), (1, False)])
+@pytest.mark.parametrize("offset", [100.0, -3000.0, 1e4, -1e5, 1e6])
+def test_routing_far_from_zero(offset, mode, norm):
+    """Logits with a common offset: probabilities and gradients depend on their differences, and so does the error."""
+    for T, E, k in ((40, 32, 4), (300, 256, 8), (70, 1000, 20)):
+        logits = 2 * torch.randn(T, E, generator=gen(T)) + offset
+        logits[3] = float("-inf")
+        logits[5, 1:] = float("-inf")
+        check_routing(logits.to(DEV), k, mode, norm, None)
+
+
+def test_routing_logits_of_the_largest_size():
+    """Differences beyond the exponential's range, sizes up to the type's largest: one expert takes all, without a NaN."""
+    big = torch.finfo(torch.float32).max
+    logits = torch.randn(6, 64, generator=gen(7))
+    logits[0, 9], logits[1, 9], logits[2] = big, 1e30, -big
+    logits[3, :32], logits[4] = 3e38, -1e30
+    logits[4, 11] = -1e29
+    x = logits.to(DEV).requires_grad_()
+    r = ep_moe.route_topk_train(x, 4)
+    r.weights.backward(torch.ones_like(r.weights))
+    want = logits.double().requires_grad_()
+    p = torch.softmax(want, 1)
+    p.gather(1, r.idx.cpu()).sum().backward()
+    # d = p_e ([e chosen] - sum of the chosen p): two factors up to 1, each off by the rounding of a sum of 64 exponentials and
+    # of its parts (half a step of 2^-23 a term, a handful of units for exponential and reciprocal), well within 72 steps
+    assert ((x.grad.cpu().double() - want.grad).abs() <= 2 * 72 * 2.0 ** -23).all()
+    assert torch.isfinite(torch.autograd.grad(ep_moe.route_topk_train(x, 4).balance_loss, x)[0]).all()
 
 
 # ------------------------------------------------------------------------------------------------ second derivatives
