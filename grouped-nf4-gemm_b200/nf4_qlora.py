@@ -308,6 +308,8 @@ def glu_train(gate_up, act: str = "silu", *, bias=None, row_expert=None):
         if tuple(row_expert.shape) != (rows,) or row_expert.device != dev or row_expert.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"row_expert must be an integer tensor of {rows} expert ids on {dev}")
         bias, row_expert = bias.detach().contiguous(), row_expert.to(torch.int32).contiguous()
+    if not torch.is_grad_enabled():
+        gate_up = gate_up.detach()        # autograd asks a function for its inputs' gradients under no_grad all the same
     return _GluTrain.apply(gate_up.contiguous(), _GLU_ACTS[act], bias, row_expert)
 
 

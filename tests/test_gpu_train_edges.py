@@ -138,3 +138,19 @@ def test_second_derivatives_are_refused_beside_other_terms():
     assert torch.equal(grad, want)
     with pytest.raises(RuntimeError, match="glu_train"):
         (grad.float().square().sum() + gu.float().sum()).backward()
+
+
+# ------------------------------------------------------------------------------------------------ GLU
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+@pytest.mark.parametrize("act", ["silu", "gpt_oss"])
+def test_glu_without_gradients_makes_no_checkpoint(mode, act):
+    rows, h = 4096, 1024
+    x = torch.randn(rows, 2 * h, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    want = Q.glu_train(x, act).detach()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    with mode():
+        out = Q.glu_train(x, act)
+    assert torch.cuda.max_memory_allocated() - before <= 2 * rows * h + 4096          # the result and nothing beside it
+    assert torch.equal(out, want) and not out.requires_grad
