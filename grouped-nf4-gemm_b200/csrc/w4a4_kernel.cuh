@@ -723,18 +723,34 @@ w4a4_kernel(const __grid_constant__ W4A4Args a, const __grid_constant__ CUtensor
     if (threadIdx.x == 0 && *abort_flag && a.status) atomicOr(a.status, GNF4B_ST_TIMEOUT);
 }
 
-// CTA pairs: for groups of kQPairRows and more, where an item has enough stages to pay for handing it over between two
-// CTAs, and, where rows start on 128-byte lines (a box row of 128 bytes is then one line of L2, else two, and a single
-// CTA's loads hold it up more), not so many that the exposed epilogue a pair saves on is small beside them.
-// Single CTAs / pairs in us, 32 experts, N = 4096, 512 and 1024 rows each:
-//   K = 736    55 / 56, 100 / 107    K = 1312   83 / 74, 154 / 134   (rows do not start on 128 bytes)
-//   K = 2880  135 / 123, 243 / 215   K = 4128  268 / 219, 440 / 372
-//   K = 2048   83 / 82, 150 / 141    K = 2816  115 / 114, 210 / 205  (rows do)
-// and with rows on 128 bytes, 64 experts, N = 2048: K = 1024 51 / 52, 95 / 99; K = 1280 67 / 73, 121 / 129; K = 1536 69 / 70,
-// 129 / 127; 16 experts, N = 4096: K = 4096 78 / 80, 142 / 143; K = 7168 117 / 125, 216 / 228.  300 rows (32 experts): K = 2048
-// 66 / 71, K = 2880 106 / 111; 400 rows, N = 5760, K = 2880: 150 / 144.
-constexpr int kQPairRows = 384;
-constexpr int kQPairStages = 6, kQPairStagesAligned = 20;      // K > 1280; K <= 5120 where rows start on 128 bytes
+// CTA pairs: where a group is long and an item has enough stages to pay for handing it over between two CTAs.  A box row of
+// 128 bytes is one line of L2 where rows start on 128-byte lines (K a multiple of 256) and two where they do not; single CTAs
+// are held up by the second line, and there pairs win on every long group.  On the lines the two are about even, and
+// pairs fall behind where the last span of scales holds one or two stages (K = 1280, 1536, 2304).
+// Microseconds of pairs / of single CTAs, 32 experts, N = 4096, equal groups:
+//                  300 rows    384         448         512         1024
+//   off:  K = 736   49 / 45    51 / 48     54 / 53     57 / 55    105 / 100
+//             1056  64 / 60    67 / 64     70 / 72     72 / 75    122 / 135
+//             1312  67 / 66    71 / 70     73 / 80     76 / 83    132 / 153
+//             2080  94 / 86    94 / 92     97 / 106   100 / 111   183 / 210
+//             2880  95 / 90   100 / 101   105 / 113   111 / 119   205 / 227
+//             2912 100 / 119  108 / 119   115 / 139   122 / 142   232 / 275
+//             4128 148 / 156  156 / 167   166 / 192   180 / 204   351 / 391
+//             7200 248 / 249  256 / 267   273 / 311   298 / 326   592 / 627
+//   on:   K = 1024  42 / 39    44 / 42     48 / 46     50 / 49     93 / 93
+//             1536  61 / 52    64 / 58     66 / 63     69 / 68    124 / 125
+//             1792  64 / 58    68 / 66     72 / 72     76 / 77    137 / 144
+//             2048  65 / 62    70 / 69     75 / 75     79 / 81    143 / 150
+//             2304  89 / 73    93 / 81     95 / 89    100 / 95    181 / 174
+//             2816  93 / 82    96 / 91    101 / 100   107 / 106   196 / 198
+//             4096 125 / 109  127 / 120   130 / 131   137 / 137   256 / 261
+//             7168 220 / 177  207 / 192   213 / 208   223 / 221   415 / 432
+// Off the lines at 416 rows: N = 5760, K = 2880 144 / 152 (384 rows: 137 / 140); 64 experts, N = 2048, K = 1312 74 / 91 (72 / 80);
+// 16 experts, N = 4096, K = 2080 66 / 64 (59 / 58); 8 experts, N = 14336, K = 4128 185 / 173 (193 / 154).  K = 1056 with 576
+// rows 98 / 89.  On them: 128 experts, N = 1536, K = 2048, 1024 rows 219 / 234; 16 experts, N = 4096, K = 7168 213 / 207.
+constexpr int kQPairRows = 400, kQPairRowsAligned = 448;
+constexpr int kQPairStages = 6;                                        // off the lines: K > 1280
+constexpr int kQPairStagesAlignedLo = 7, kQPairStagesAlignedHi = 8;    // on them: 1536 < K <= 2048
 
 struct W4A4Plan {
     int rows_w, tok_cap, xbox, x_bytes, x_blocks, stages, acc_bufs;
@@ -763,7 +779,9 @@ static inline W4A4Plan w4a4_plan(int64_t T, int32_t G, int64_t N, int64_t K, int
         }
     }
     const int64_t k_stages = ceil_div(K, kQStageK);
-    p.pair = longest >= kQPairRows && k_stages >= kQPairStages && (k_stages <= kQPairStagesAligned || (K / 2) % 128 != 0);
+    const bool on_lines = (K / 2) % 128 == 0;
+    p.pair = on_lines ? longest >= kQPairRowsAligned && k_stages >= kQPairStagesAlignedLo && k_stages <= kQPairStagesAlignedHi
+                      : longest >= kQPairRows && k_stages >= kQPairStages;
     if (p.pair) {
         p.tok_cap = (int)round_up(p.tok_cap, 32);
         p.xbox = 64;

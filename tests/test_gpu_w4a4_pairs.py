@@ -52,7 +52,7 @@ def check(out, xb, xs, wb, ws, sizes, ids):
         first += n
 
 
-SIZES = [[384], [400, 1, 0, 17], [511], [513], [1000, 16, 33], [1, 385, 0, 64, 770]]
+SIZES = [[400], [401, 1, 0, 17], [511], [513], [1000, 16, 33], [1, 385, 0, 64, 770]]
 
 
 @pytest.mark.parametrize("sizes", SIZES)
@@ -68,7 +68,7 @@ def test_shapes(N, sizes):
     assert nf4_grouped.last_status(DEV) == 0
 
 
-@pytest.mark.parametrize("K", [1344, 1536, 2048, 2080, 2816, 2880, 2912, 4128, 5152])
+@pytest.mark.parametrize("K", [1344, 1568, 1792, 2048, 2080, 2880, 2912, 4128, 5152])
 def test_lengths(K):
     """Whole and broken last stages and spans of scales; scale rows on 16 bytes, on 8, on none; rows on and off 128 bytes."""
     E, N, sizes, ids = 2, 300, [450, 0, 5, 384], [1, 0, 0, 1]
