@@ -114,10 +114,14 @@ def route_topk(logits: torch.Tensor, k: int, mode: int = 0, norm: bool = False):
 
 
 class RoutingTrain(NamedTuple):
-    """What ``route_topk_train`` returns; ``weights``, ``balance_loss`` and ``z_loss`` carry gradients to the logits."""
-    idx: torch.Tensor             # [M, k] int64
-    weights: torch.Tensor         # [M, k] fp32
-    counts: torch.Tensor          # [E] int32, tokens that chose each expert
+    """What ``route_topk_train`` returns; ``weights``, ``balance_loss`` and ``z_loss`` carry gradients to the logits.
+
+    ``counts`` are the losses' counts: of the tokens that count.  ``idx`` routes every token, so with a mask or an empty
+    token they are not the sizes of the groups that ``idx`` makes; those are ``torch.bincount(idx.reshape(-1),
+    minlength=E)``."""
+    idx: torch.Tensor             # [M, k] int64, of every token
+    weights: torch.Tensor         # [M, k] fp32, of every token
+    counts: torch.Tensor          # [E] int32, tokens that count and chose each expert
     balance_loss: torch.Tensor    # fp32 scalar
     z_loss: torch.Tensor          # fp32 scalar
 
@@ -211,7 +215,7 @@ def route_topk_train(logits: torch.Tensor, k: int, mode: int = 0, norm: bool = F
         z_loss       = mean_t logsumexp(logits_t)^2
 
     and both are 0 when no token counts.  A masked token is routed and weighted all the same (a batch's padding; mask
-    its result, not its route).  A token whose logits are all -inf gets weights 0 and no gradient.  On a GPU one kernel
+    its result, not its route): group sizes come from ``idx``, not from ``counts``.  A token whose logits are all -inf gets weights 0 and no gradient.  On a GPU one kernel
     each way (E <= 1024, k <= 32); on the CPU the same in tensor operations."""
     if logits.dim() != 2:
         raise ValueError(f"logits must be [tokens, experts], got shape {tuple(logits.shape)}")

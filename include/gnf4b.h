@@ -478,7 +478,8 @@ int gnf4b_w4a4_plan(int64_t T, int32_t G, int64_t N, int64_t K, int32_t max_rows
 /* Routing for training.  Selection and weights as gnf4b_route_topk, on logits [T, E] of bf16, fp16 or fp32 (rows `stride`
  * elements apart; E <= 1024, k <= 32), with what a training step needs beside them.  Over the n tokens that count (all,
  * or those with token_mask[t] != 0; never a token whose logits are all -inf):
- *   counts[E] tokens that chose the expert;   balance_loss = E sum_e (counts_e / (n k)) mean_t p[t, e]   (1 when even)
+ *   counts[E] of these, the tokens that chose the expert (not the group sizes of idx, which routes every token)
+ *   balance_loss = E sum_e (counts_e / (n k)) mean_t p[t, e]   (1 when even)
  *   z_loss = mean_t (log sum_e exp logits[t, e])^2;   n_tokens = n as a float;   n = 0: both losses 0
  * Masked tokens are routed all the same.  A token whose logits are all -inf gets weights 0.  A NaN logit is chosen after
  * every other one; the token's weights and, if it counts, the losses are NaN.  lse [T] is kept for the backward pass.

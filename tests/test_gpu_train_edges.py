@@ -101,6 +101,28 @@ def test_routing_far_from_zero(offset, mode, norm):
         check_routing(logits.to(DEV), k, mode, norm, None)
 
 
+def test_a_masked_batch_through_a_layer():
+    """The groups of a padded batch are made from the ids of all tokens; the losses' counts leave the padding out."""
+    T, E, k, K, h = 60, 5, 2, 128, 64
+    g = gen(8)
+    gu, dn = synth.nf4_stack(E, 2 * h, K, g, scale=0.08, device=DEV), synth.nf4_stack(E, K, h, g, scale=0.08, device=DEV)
+    x = torch.randn(T, K, generator=g).to(torch.bfloat16).to(DEV)
+    logits = torch.randn(T, E, generator=g)
+    logits[7] = float("-inf")
+    mask = torch.rand(T, generator=g) < 0.7
+    r = ep_moe.route_topk_train(logits.to(DEV), k, token_mask=mask.to(DEV))
+    c = ep_moe.route_topk_train(logits, k, token_mask=mask)
+    assert torch.equal(r.counts.cpu(), c.counts) and int(r.counts.sum()) == k * int((mask & (torch.arange(T) != 7)).sum())
+    order = torch.argsort(r.idx.reshape(-1), stable=True)
+    sizes = torch.bincount(r.idx.reshape(-1), minlength=E)
+    assert int(sizes.sum()) == T * k and not torch.equal(sizes.int(), r.counts)
+    y = Q.ffn_4bit_grouped_train(x[order // k], *gu, *dn, sizes, torch.arange(E, device=DEV))
+    for p in range(0, T * k, 7):
+        one = Q.ffn_4bit_grouped_train(x[order[p] // k][None], *gu, *dn, [1], [int(r.idx.reshape(-1)[order[p]])])
+        # the same sums in another order and a rounding to bf16 after each of three steps, at either side
+        assert float((y[p].double() - one[0].double()).norm() / one[0].double().norm()) <= 6 * 2.0 ** -8
+
+
 def test_routing_logits_of_the_largest_size():
     """Differences beyond the exponential's range, sizes up to the type's largest: one expert takes all, without a NaN."""
     big = torch.finfo(torch.float32).max
