@@ -382,7 +382,8 @@ route_train_fwd_kernel(const __grid_constant__ RouteTrainArgs a) {
         }
         const bool chosen = place < a.k;
         const float ej = (chosen && !dead) ? rt_exp(sel - top) : 0.f;
-        if (renorm) z = warp_sum(ej);
+        // renormalised probabilities of a row with a NaN are NaN like the probabilities; mode 1 has only the chosen logits
+        if (renorm) z = warp_sum(ej) + (a.mode == 0 && !plain && !dead ? z : 0.f);
         if (chosen) {
             a.idx[t * a.k + place] = sel_e;
             a.w[t * a.k + place] = dead ? 0.f : ej * rt_rcp(z);

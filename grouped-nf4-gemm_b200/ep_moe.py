@@ -249,6 +249,8 @@ def _route_train_ops(logits, k, mode, norm, token_mask):
     safe = lg.masked_fill(dead[:, None], 0.0)
     logp = torch.log_softmax(safe, dim=-1)
     w = torch.softmax(torch.gather(safe, 1, idx), dim=-1) if mode == 1 or norm else torch.exp(torch.gather(logp, 1, idx))
+    if mode == 0:                                       # a NaN (or two infinities) leaves no probability to renormalise
+        w = w.masked_fill(torch.isnan(logp.detach()).any(1, keepdim=True), float("nan"))
     w = w.masked_fill(dead[:, None], 0.0)
     n = keep.sum().clamp_min(1).float()
     chosen = torch.zeros_like(lg).scatter_(1, idx, 1.0)

@@ -482,7 +482,7 @@ int gnf4b_w4a4_plan(int64_t T, int32_t G, int64_t N, int64_t K, int32_t max_rows
  *   balance_loss = E sum_e (counts_e / (n k)) mean_t p[t, e]   (1 when even)
  *   z_loss = mean_t (log sum_e exp logits[t, e])^2;   n_tokens = n as a float;   n = 0: both losses 0
  * Masked tokens are routed all the same.  A token whose logits are all -inf gets weights 0.  A NaN logit is chosen after
- * every other one; the token's weights and, if it counts, the losses are NaN.  lse [T] is kept for the backward pass.
+ * every other one; the token's weights (in mode 1 only if it was chosen) and, if it counts, the losses are NaN.  lse [T] is kept for the backward pass.
  * scratch: gnf4b_route_train_scratch_bytes(T, E) bytes (8-byte aligned, any content; 0 for small batches), not shared by
  * calls that overlap.  Deterministic (no floating-point atomics).
  * gnf4b_route_train_bwd: grad [T, E] (contiguous, the logits' type) from g_weights [T, k] (fp32), g_balance and g_z

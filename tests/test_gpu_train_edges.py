@@ -101,6 +101,22 @@ def test_routing_far_from_zero(offset, mode, norm):
         check_routing(logits.to(DEV), k, mode, norm, None)
 
 
+@pytest.mark.parametrize("T", [10, 300])
+@pytest.mark.parametrize("mode,norm", [(0, False), (0, True), (1, False)])
+def test_routing_rows_with_a_nan_as_route_topk_weighs_them(T, mode, norm):
+    x = torch.randn(T, 24, generator=gen(9))
+    x[4, 5], x[6, 3], x[7, [1, 2]] = float("nan"), float("inf"), float("inf")
+    x[8, 5] = float("-inf")
+    r = ep_moe.route_topk_train(x.to(DEV), 3, mode, norm)
+    c = ep_moe.route_topk_train(x, 3, mode, norm)
+    idx, w = ep_moe.route_topk(x.to(DEV), 3, mode, norm)
+    assert torch.equal(r.idx, idx) and torch.equal(r.idx.cpu(), c.idx)
+    for other in (w, c.weights.to(DEV)):
+        # a sum of 24 exponentials (1 + |x| <= 16 units of 2^-24 each), a division, at either side
+        torch.testing.assert_close(r.weights, other, rtol=2 * (24 + 16 + 8) * 2.0 ** -23, atol=0, equal_nan=True)
+    assert torch.isnan(r.weights[4]).all() == (mode == 0)
+
+
 def test_a_masked_batch_through_a_layer():
     """The groups of a padded batch are made from the ids of all tokens; the losses' counts leave the padding out."""
     T, E, k, K, h = 60, 5, 2, 128, 64
