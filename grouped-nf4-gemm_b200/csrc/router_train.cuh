@@ -494,6 +494,7 @@ route_train_bwd_kernel(const __grid_constant__ RouteTrainBwdArgs a) {
     const float n = __ldg(a.n_tokens);
     const float gb = (a.g_balance && n > 0.f) ? __ldg(a.g_balance) * (float)a.E / (n * n * (float)a.k) : 0.f;
     const float gz = (a.g_z && n > 0.f) ? 2.f * __ldg(a.g_z) / n : 0.f;
+    const bool losses = gb != 0.f || gz != 0.f;      // else no term of theirs: a NaN logit times nothing is not NaN
     float push[NE];                                  // d balance / d p_e of one token
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
@@ -523,7 +524,7 @@ route_train_bwd_kernel(const __grid_constant__ RouteTrainBwdArgs a) {
         const float lse = lse_n, w = w_n, g = g_n;
         const int64_t e_sel = e_n;
         const bool dead = lse == -INFINITY;
-        const bool counted = !dead && keep_n;
+        const bool counted = losses && !dead && keep_n;
         const bool has = e_sel >= 0 && e_sel < a.E;
         // lse in one fp32 number is off by up to half its last place, 5e-4 where the logits are around 10000, and by the same
         // for every expert of the token: dividing by the sum of what it gives, which lies near 1, takes that factor out

@@ -117,6 +117,25 @@ def test_routing_rows_with_a_nan_as_route_topk_weighs_them(T, mode, norm):
     assert torch.isnan(r.weights[4]).all() == (mode == 0)
 
 
+@pytest.mark.parametrize("T", [10, 300])
+def test_routing_gradient_of_chosen_weights_beside_a_nan(T):
+    """Mode 1 weighs the chosen logits alone: without a gradient of the losses a NaN that was not chosen has no part in it."""
+    x = torch.randn(T, 24, generator=gen(10))
+    x[4, 5] = float("nan")
+    g_w = torch.randn(T, 3, generator=gen(11))
+    grads = []
+    for dev in (DEV, "cpu"):
+        v = x.to(dev).requires_grad_()
+        grads.append(torch.autograd.grad(ep_moe.route_topk_train(v, 3, 1).weights, v, g_w.to(dev))[0].cpu())
+    assert torch.isfinite(grads[0]).all()
+    # w (g - sum w g): three products and their sum, each half a step of 2^-23, weights good to (3 + 16) steps
+    assert ((grads[0] - grads[1]).abs() <= 2 * (19 + 4) * 2.0 ** -23 * 4 * g_w.abs().amax()).all()
+    v = x.to(DEV).requires_grad_()
+    r = ep_moe.route_topk_train(v, 3, 1)
+    grad, = torch.autograd.grad((r.weights, r.z_loss), v, (g_w.to(DEV), torch.ones((), device=DEV)))
+    assert torch.isnan(grad[4]).all() and torch.isfinite(grad[torch.arange(T) != 4]).all()
+
+
 def test_a_masked_batch_through_a_layer():
     """The groups of a padded batch are made from the ids of all tokens; the losses' counts leave the padding out."""
     T, E, k, K, h = 60, 5, 2, 128, 64
