@@ -668,8 +668,9 @@ def gemm_4bit_grouped(a_cat, B, absmax, sizes, expert_ids, block_m: int | None =
     ``max_rows`` -- the largest group size if the caller knows it (a path hint only).
     ``path`` -- 0 planner, 1 streaming kernel, 2 tensor-core kernel (ablation).
     ``tables_ready`` -- True promises that device-side ``group_offsets`` / ``expert_ids`` / ``sizes`` were NOT
-    written by the kernel launched just before this call on the stream; the decode kernel then starts
-    streaming weights while that kernel still runs.  Default: true for host lists (they are uploaded by a
+    written by the kernel launched just before this call on the stream, and neither was the stack (by
+    ``mxfp4_grouped.quantize_mxfp4``, for one); the decode kernel then starts streaming weights while that kernel
+    still runs.  Default: true for host lists (they are uploaded by a
     stream-ordered copy), false for device tensors.
     """
     E, N, _ = B.shape

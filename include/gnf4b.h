@@ -50,10 +50,11 @@ extern "C" {
 #define GNF4B_FLAG_SMEM_OPERANDS 0x10000u /* ablation: forward on the first tensor kernel (both MMA
                                             operands in shared memory) instead of weights in TMEM */
 
-#define GNF4B_FLAG_TABLES_READY   0x40000u /* group_offsets / expert_ids were not written by the kernel launched
-                                            just before this call on the stream (they were uploaded, or made
-                                            earlier): the decode kernel then streams its first weights while
-                                            that previous kernel is still running */
+#define GNF4B_FLAG_TABLES_READY   0x40000u /* neither group_offsets / expert_ids nor the stack were written by the
+                                            kernel launched just before this call on the stream (they were
+                                            uploaded, or made earlier): the decode kernel then streams its first
+                                            weights while that previous kernel is still running -- so not for a
+                                            stack that gnf4b_quantize_mxfp4 has just packed */
 #define GNF4B_FLAG_DECODE_ONE_ROW 0x80000u /* ablation: decode kernel with one weight row per warp in flight where it
                                             would keep two */
 
