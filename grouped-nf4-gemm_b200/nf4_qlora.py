@@ -283,7 +283,9 @@ def glu_train(gate_up, act: str = "silu", *, bias=None, row_expert=None):
     """The activation between an expert's two products, differentiable: ``gate_up [rows, 2h]`` bf16 -> ``[rows, h]`` bf16.
     ``act="silu"``: SiLU(gate) * up over column halves; ``act="gpt_oss"``: gate and up interleaved, clamped at 7,
     (up + 1) * gate * sigmoid(1.702 gate), with an optional frozen ``bias`` bf16 ``[E, 2h]`` added by ``row_expert [rows]``.
-    fp32 inside, one rounding.
+    fp32 inside, one rounding: not the bits of ``mxfp4_grouped.glu_gpt_oss`` and what is built on it (``ffn_mxfp4_grouped``,
+    ``glu_quantize_mxfp4``), which round the bias sum and four intermediate results to bf16 as a chain of tensor operations
+    does.
 
     What stays until the backward pass is gate and up in 8 bits (per 64 values of a row one fp32 step, their largest
     magnitude / 127): 2.1 bytes per pair where autograd through tensor operations keeps 10 and more, and neither
@@ -326,7 +328,8 @@ def ffn_4bit_grouped_train(a_cat, packed_gu, absmax_gu, packed_dn, absmax_dn, si
 
 def ffn_mxfp4_grouped_train(a_cat, blocks_gu, scales_gu, blocks_dn, scales_dn, sizes, expert_ids, *, act: str = "gpt_oss",
                             bias_gu=None, row_expert=None, rows: str = "bf16"):
-    """The MXFP4 counterpart on frozen stacks.  ``rows="mxfp4"`` multiplies MXFP4 rows forward
+    """The MXFP4 counterpart on frozen stacks; ``bias_gu`` (bf16 ``[E, N_gu]``, ``act="gpt_oss"``) by ``row_expert [T]``.  The
+    activation is ``glu_train``: the result is not the bits of ``ffn_mxfp4_grouped``.  ``rows="mxfp4"`` multiplies MXFP4 rows forward
     (``gemm_mxfp4_grouped_w4a4_train``), ``"bf16"`` the rows as they are."""
     if rows not in ("bf16", "mxfp4"):
         raise ValueError("rows is 'bf16' or 'mxfp4'")
