@@ -109,10 +109,12 @@ def dgrad_mxfp4_grouped_host(grad_host, blocks, scales, sizes, expert_ids, out=N
                         blocks.shape[2] * 2, out, return_status=return_status)
 
 
-def dgrad_mxfp4_grouped(grad_out, blocks, scales, sizes, expert_ids, *, group_offsets=None, max_rows=None):
+def dgrad_mxfp4_grouped(grad_out, blocks, scales, sizes, expert_ids, *, group_offsets=None, max_rows=None,
+                        zero_rest: bool = False):
     """``grad_a[t,:] = grad_out[t,:] @ dequant_mxfp4(blocks[e(t)])`` in one launch, ``[T,K]``
     bf16.  The reference has this only as a per-expert Python loop on the GPU
-    (kernel/mxfp4_qlora.py:105-122) and as a CPU kernel (gnf4_native/cpu_kernels.c:1386-1397)."""
+    (kernel/mxfp4_qlora.py:105-122) and as a CPU kernel (gnf4_native/cpu_kernels.c:1386-1397).  Rows of no group or
+    of a padding group (expert id -1) are not written, or zeros with ``zero_rest``."""
     E, N, half = blocks.shape
     _require_cuda(grad_out, "dgrad_mxfp4_grouped",
                   "The CPU-checkable equivalent is grad_out @ dequant_mxfp4(blocks, scales) per group.")
@@ -121,7 +123,7 @@ def dgrad_mxfp4_grouped(grad_out, blocks, scales, sizes, expert_ids, *, group_of
     if grad_out.shape[1] != N:
         raise ValueError(f"grad_out has {grad_out.shape[1]} columns but the stack has N={N}")
     return _launch(_gnf4b.FMT_MXFP4, _gnf4b.OP_DGRAD, grad_out, blocks, scales, sizes, expert_ids, half * 2,
-                   group_offsets=group_offsets, max_rows=max_rows)
+                   group_offsets=group_offsets, max_rows=max_rows, zero_rest=zero_rest)
 
 
 def dequant_stack_cuda(blocks, scales):

@@ -476,8 +476,9 @@ def _group_tables(sizes, expert_ids, T: int, E: int, dev, group_offsets=None, ma
 
 
 def _launch(fmt, op, x, W, S, sizes, expert_ids, n_out, *, split_k=None, path=_gnf4b.PATH_AUTO,
-            group_offsets=None, max_rows=None, tables_ready=None, x_glu: int = 0):
-    """One grouped launch.  x [T, C] bf16/fp16, W [E, N, K/2] u8, S scales -> bf16 [T, n_out].
+            group_offsets=None, max_rows=None, tables_ready=None, x_glu: int = 0, zero_rest: bool = False):
+    """One grouped launch.  x [T, C] bf16/fp16, W [E, N, K/2] u8, S scales -> bf16 [T, n_out].  Rows of no group or of a
+    padding group are not written, or zeros (``zero_rest``).
     ``x_glu`` (FLAG_X_SILU_GLU / FLAG_X_GPT_OSS_GLU): x is the gate_up output [T, 2K]; returns None when the
     library has no kernel that applies the activation on load for this problem."""
     dev = x.device
@@ -511,7 +512,7 @@ def _launch(fmt, op, x, W, S, sizes, expert_ids, n_out, *, split_k=None, path=_g
         sdt = _gnf4b.S_E8M0
     if S.stride(2) != 1:
         S = S.contiguous()
-    out = torch.empty(T, n_out, dtype=torch.bfloat16, device=dev)
+    out = (torch.zeros if zero_rest else torch.empty)(T, n_out, dtype=torch.bfloat16, device=dev)
     if T == 0:
         return out
     lib = _gnf4b.load()
@@ -708,12 +709,13 @@ def dgrad_eligible(grad_out, B, absmax, block_k: int = 64):
 
 
 def dgrad_4bit_grouped(grad_out, B, absmax, sizes, expert_ids, config=None, *, group_offsets=None,
-                       max_rows=None):
+                       max_rows=None, zero_rest: bool = False):
     """``grad_a[t,:] = grad_out[t,:] @ dequant_nf4(B[e(t)])`` in one launch (ref :1056-1121).
 
     ``grad_out [T,N]`` bf16, same stack and grouping as the forward; returns ``[T,K]`` bf16.
     ``config`` (a Triton tile tuple in the reference) only takes part in the eligibility
-    check; the result does not depend on it."""
+    check; the result does not depend on it.  Rows of no group or of a padding group (expert id -1) are not
+    written, or zeros with ``zero_rest``."""
     E, N, half = B.shape
     K = half * 2
     T = grad_out.shape[0]
@@ -727,6 +729,9 @@ def dgrad_4bit_grouped(grad_out, B, absmax, sizes, expert_ids, config=None, *, g
             "check dgrad_eligible() first rather than catching this.")
     if grad_out.shape[1] != N:
         raise ValueError(f"grad_out has {grad_out.shape[1]} columns but the stack has N={N}")
+    if zero_rest:
+        return _launch(_gnf4b.FMT_NF4, _gnf4b.OP_DGRAD, grad_out, B, absmax, sizes, expert_ids, K,
+                       group_offsets=group_offsets, max_rows=max_rows, zero_rest=True)
     return _dispatch(_gnf4b.FMT_NF4, _gnf4b.OP_DGRAD, grad_out, B, absmax, sizes, expert_ids, K,
                      group_offsets=group_offsets, max_rows=max_rows)
 

@@ -50,9 +50,11 @@ def first_derivative_only(grad, what: str):
     return _FirstOnly.apply(grad.detach().requires_grad_(), what)
 
 
-def _product_gradient(dgrad, what, grad_out, *stack_and_groups):
-    """``dgrad(grad_out, ...)``.  The product is linear in its rows: its gradient depends on ``grad_out`` alone."""
-    grad = dgrad(grad_out, *stack_and_groups)
+def _product_gradient(dgrad, what, grad_out, packed, scales, sizes, expert_ids):
+    """``dgrad(grad_out, ...)``.  The product is linear in its rows: its gradient depends on ``grad_out`` alone.  Rows that no
+    expert takes have the gradient zero; with group tables in host memory and no padding group there are none."""
+    on_host = not any(torch.is_tensor(t) and t.is_cuda for t in (sizes, expert_ids))
+    grad = dgrad(grad_out, packed, scales, sizes, expert_ids, zero_rest=not on_host or min(_host_ints(expert_ids), default=0) < 0)
     return first_derivative_only(grad, what) if torch.is_grad_enabled() and grad_out.requires_grad else grad
 
 
@@ -92,7 +94,7 @@ class FusedGroupedNf4(torch.autograd.Function):
         grad_a = torch.zeros(grad_out.shape[0], k_in, dtype=grad_out.dtype, device=grad_out.device)
         first = 0
         for rows, e in zip(_host_ints(ctx.sizes), _host_ints(ctx.expert_ids)):
-            if rows:
+            if rows and e >= 0:                              # a padding group has no gradient
                 w = dequant_ref(packed[e].to(grad_out.device), absmax[e].to(grad_out.device), n_out, k_in)
                 grad_a[first:first + rows] = grad_out[first:first + rows] @ w.to(grad_out.dtype)
             first += rows
@@ -104,7 +106,7 @@ def gemm_4bit_grouped_train(a_cat, packed, absmax, sizes, expert_ids, weights_fn
     return FusedGroupedNf4.apply(a_cat, packed, absmax, sizes, expert_ids, weights_fn, dgrad_kernel)
 
 
-def _dgrad_mxfp4(grad_out, blocks, scales, sizes, expert_ids):
+def _dgrad_mxfp4(grad_out, blocks, scales, sizes, expert_ids, zero_rest):
     """``dgrad_mxfp4_grouped`` for any N: its kernel takes multiples of 8 (16-byte rows of ``grad_out``), other widths are
     filled up with columns of zeros against rows of zeros."""
     from mxfp4_grouped import dgrad_mxfp4_grouped
@@ -112,7 +114,7 @@ def _dgrad_mxfp4(grad_out, blocks, scales, sizes, expert_ids):
     if fill:
         grad_out = torch.nn.functional.pad(grad_out, (0, fill))
         blocks, scales = (torch.nn.functional.pad(t, (0, 0, 0, fill)) for t in (blocks, scales))
-    return dgrad_mxfp4_grouped(grad_out.contiguous(), blocks, scales, sizes, expert_ids)
+    return dgrad_mxfp4_grouped(grad_out.contiguous(), blocks, scales, sizes, expert_ids, zero_rest=zero_rest)
 
 
 class FusedGroupedMxfp4(torch.autograd.Function):

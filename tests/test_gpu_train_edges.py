@@ -44,6 +44,44 @@ def test_gradient_of_any_width(product, N):
             first += n
 
 
+@pytest.mark.parametrize("kernel", [True, False])
+@pytest.mark.parametrize("product", ["gemm_4bit_grouped_train", "gemm_mxfp4_grouped_train", "gemm_mxfp4_grouped_w4a4_train"])
+def test_rows_without_an_expert_have_no_gradient(product, kernel):
+    """A padding group and rows behind the last one: zeros, whatever the gradient's memory held before."""
+    nf4 = "4bit" in product
+    if not kernel and not nf4:
+        pytest.skip("only the NF4 gradient has the loop")
+    g = gen(12)
+    stack = (synth.nf4_stack if nf4 else synth.mxfp4_stack)(2, 64, 128, g, device=DEV)
+    more = dict(dgrad_kernel=kernel) if nf4 else {}
+    x = torch.randn(300, 128, generator=g).to(torch.bfloat16).to(DEV).requires_grad_()
+    go = torch.randn(300, 64, generator=g).to(torch.bfloat16).to(DEV)
+    want = torch.zeros_like(x)
+    first = 0
+    for n, e in ((100, 1), (50, -1), (90, 0)):
+        if e >= 0:
+            part = x.detach()[first:first + n].clone().requires_grad_()
+            want[first:first + n] = torch.autograd.grad(getattr(Q, product)(part, *stack, [n], [e], **more), part, go[first:first + n])[0]
+        first += n
+    sizes, ids = [100, 50, 90], [1, -1, 0]
+    for tables in ((torch.tensor(sizes, device=DEV), torch.tensor(ids, device=DEV)), (sizes + [60], ids + [-1]),
+                   (torch.tensor(sizes, device=DEV), torch.tensor(ids))):
+        y = getattr(Q, product)(x, *stack, *tables, **more)
+        stale = [torch.full((300, 128), float("nan"), dtype=torch.bfloat16, device=DEV) for _ in range(4)]
+        del stale
+        assert torch.equal(torch.autograd.grad(y, x, go)[0], want)
+
+
+@pytest.mark.parametrize("product", ["gemm_4bit_grouped_train", "gemm_mxfp4_grouped_train", "gemm_mxfp4_grouped_w4a4_train"])
+def test_products_of_no_rows(product):
+    stack = (synth.nf4_stack if "4bit" in product else synth.mxfp4_stack)(2, 20, 128, gen(13), device=DEV)
+    for sizes, ids in (([], []), ([0, 0], [1, 0]), (torch.zeros(2, dtype=torch.int64, device=DEV), torch.tensor([0, 1], device=DEV))):
+        x = torch.empty(0, 128, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+        y = getattr(Q, product)(x, *stack, sizes, ids)
+        y.sum().backward()
+        assert y.shape == (0, 20) and x.grad.shape == (0, 128)
+
+
 def test_ffn_gradient_with_an_odd_result_width():
     E, K, h, N, sizes, ids = 2, 64, 32, 61, [3, 6], [1, 0]
     g = gen(2)
