@@ -848,6 +848,11 @@ def main():
     if args.impl == "reference":
         if rank != 0:
             return 0
+        from oracle import oracle as O
+        if O.load_ref() is None:
+            print(json.dumps({"impl": "reference", "unavailable": "oracle/_ref is not built: it is made from the reference checkout, "
+                                                                  "which is not here"}))
+            return 0
         # the whole job of the other arm: tokens per GPU x GPUs (weak scaling), on the host cores
         n = max(1, args.gpus)
         job_tokens = args.tokens * n
