@@ -249,3 +249,28 @@ def test_glu_without_gradients_makes_no_checkpoint(mode, act):
         out = Q.glu_train(x, act)
     assert torch.cuda.max_memory_allocated() - before <= 2 * rows * h + 4096          # the result and nothing beside it
     assert torch.equal(out, want) and not out.requires_grad
+
+
+@pytest.mark.parametrize("act", ["silu", "gpt_oss"])
+def test_glu_codes_are_nearest(act):
+    """Every value is held by a code that no other code is nearer than: off by at most half a step of the block's maximum / 127.
+    127 / max is rounded once (2^-24), so a value may pass half way by 127 * 2^-24 steps; many lie there exactly."""
+    import _gnf4b
+    rows, h = 257, 200
+    nb = -(-h // 64)
+    gu = torch.randn(rows, 2 * h, generator=gen(14)).to(torch.bfloat16)
+    gu[:40, ::3] = gu[:40].float().abs().amax(1, keepdim=True).to(torch.bfloat16) / 2                  # 63.5 steps
+    gu[40] = torch.linspace(-4, 4, 2 * h).to(torch.bfloat16)
+    x = gu.to(DEV)
+    out = torch.empty(rows, h, dtype=torch.bfloat16, device=DEV)
+    codes = torch.empty(rows, nb, 2, 64, dtype=torch.int8, device=DEV)
+    steps = torch.empty(rows, nb, 2, dtype=torch.float32, device=DEV)
+    assert _gnf4b.load().gnf4b_glu_ckpt8_fwd(x.data_ptr(), rows, h, 0 if act == "silu" else 1, None, None, 0, out.data_ptr(), codes.data_ptr(),
+                                             steps.data_ptr(), None, torch.cuda.current_stream().cuda_stream) == 0
+    gate, up = (gu[:, :h], gu[:, h:]) if act == "silu" else (gu[:, 0::2], gu[:, 1::2])
+    v = torch.nn.functional.pad(torch.stack((gate, up), 1).double(), (0, nb * 64 - h)).reshape(rows, 2, nb, 64).transpose(1, 2)
+    top = v.abs().amax(-1, keepdim=True)
+    assert torch.equal(steps.cpu(), (top[..., 0].float() / 127.0))
+    code = codes.cpu().double()
+    assert code.abs().max() == 127 and ((v * 127 - code * top).abs() <= top * (0.5 + 127 * 2.0 ** -24)).all()
+    assert ((v * 254 / top) % 2 == 1).sum() > 500                     # of the inputs: values half way between two codes
