@@ -27,9 +27,9 @@
 // sums as 64-bit fixed-point numbers in steps of 2^-32 (a sum is at most 2^31; a step is far below the fp32 sums' own
 // rounding), so that the order in which CTAs arrive cannot change a bit.  The last CTA to arrive computes the losses.
 //
-// Measured at 65536 tokens x 256 experts, top 8, fp32 (67 MB of logits, 10 us of reading): forward 50 us, about 500
+// Measured at 65536 tokens x 256 experts, top 8, fp32 (67 MB of logits, 10 us of reading): forward 51 us, about 500
 // instructions a token at 71 % of the issue slots and 10 us of launches and joining (115 us with k scans, and 27 to 66 us more for
-// a second kernel over the CTAs' sums); backward 35 us, about 320 instructions at 53 % (42 us with 24 instead of 32 warps per
+// a second kernel over the CTAs' sums); backward 35 us, about 320 instructions a token (42 us with 24 instead of 32 warps per
 // SM; 20 us would be the bytes; 34 without the sum that corrects lse).  65536 x 32 bf16, top 4: 28.7 and 13.4 us (12.3 without).
 #pragma once
 

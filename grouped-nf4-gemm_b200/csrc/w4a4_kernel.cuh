@@ -36,11 +36,11 @@
 // Measured (kernel alone, graphs of 20 launches): gpt-oss gate_up (N = 5760, K = 2880, 32 experts) 4 rows each 55 us, 5.1 TB/s;
 // 1024 rows each 281-308 us, 3.9-3.5 PFLOP/s; Qwen3 gate_up (N = 1536, K = 2048, 128 experts) 256 rows each 70-79 us, 2.9-2.6
 // PFLOP/s (the lower figures at 1.65 GHz, where the power limit then holds the clock); one gpt-oss token through 4 experts
-// 13 us.  (The W4A16 kernels here: 288, 979, 218 us for the first three.)
+// 13 us.  (The W4A16 kernels here: 252, 1115, 218 us for the first three, 12 for the last.)
 // What bounds it: with few rows the issuer, 635 cycles per stage at about 31 per tcgen05 instruction and 130 per completed
 // barrier (without the MMAs and copies 47 us of the 55, the rate of a plain copy); with 256 rows the tiles' way from L2 into
-// shared memory, 45 to 49 bytes per cycle and SM (without MMAs and copies 58 us of 70, in a pair 170 of 203 for 8 x 2048 rows,
-// K = 7168), and the power limit; scales take 3 to 9 % (rows on 16 bytes the less).  A launch reaches its first MMA after
+// shared memory, 45 to 49 bytes per cycle and SM (without MMAs and copies 58 us of 70; in pairs, measured on 8 x 2048 rows, K = 7168,
+// which the rule gives to single CTAs, 170 of 203), and the power limit; scales take 3 to 9 % (rows on 16 bytes the less).  A launch reaches its first MMA after
 // 3.5 us with few rows (1.6 of them launch and group table) and after 6 with many, when every SM loads at once.
 #pragma once
 
