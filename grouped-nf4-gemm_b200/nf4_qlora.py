@@ -144,7 +144,7 @@ def _lora_delta_grouped_loop(a_cat, lora_A, lora_B, sizes, expert_ids, scaling=1
     path is tested against.  ``None`` when there are no rows."""
     out, first = None, 0
     for rows, e in zip(_host_ints(sizes), _host_ints(expert_ids)):
-        if rows:
+        if rows and e >= 0:                                  # a padding group has no delta
             x = a_cat[first:first + rows].to(lora_A.dtype)
             d = scaling * ((x @ lora_A[e].t()) @ lora_B[e].t())
             if out is None:
@@ -162,6 +162,8 @@ def lora_delta_grouped(a_cat, lora_A, lora_B, sizes, expert_ids, scaling=1.0):
     graph has two nodes per projection instead of two per expert; when padding would multiply the rows by
     more than ``_PAD_WASTE_LIMIT`` the per-expert loop is used."""
     size_list = _host_ints(sizes)
+    on_device = torch.is_tensor(expert_ids) and expert_ids.device.type != "cpu"
+    ids = None if on_device else _host_ints(expert_ids)
     live = [g for g, n in enumerate(size_list) if n > 0]
     if not live:
         return None
@@ -170,10 +172,9 @@ def lora_delta_grouped(a_cat, lora_A, lora_B, sizes, expert_ids, scaling=1.0):
     if len(live) * widest > _PAD_WASTE_LIMIT * total:
         return _lora_delta_grouped_loop(a_cat, lora_A, lora_B, sizes, expert_ids, scaling)
     dev = a_cat.device
-    if torch.is_tensor(expert_ids) and expert_ids.device.type != "cpu":
+    if on_device:
         experts = expert_ids.to(torch.int64)[torch.tensor(live, dtype=torch.int64, device=expert_ids.device)]
     else:
-        ids = _host_ints(expert_ids)
         experts = torch.tensor([ids[g] for g in live], dtype=torch.int64, device=dev)
     # row t of the live rows belongs to live group grp[t], at position pos[t] inside it
     counts = torch.tensor(rows, dtype=torch.int64, device=dev)
@@ -181,12 +182,19 @@ def lora_delta_grouped(a_cat, lora_A, lora_B, sizes, expert_ids, scaling=1.0):
     grp = torch.repeat_interleave(torch.arange(len(live), device=dev), counts, output_size=total)
     pos = torch.arange(total, device=dev) - starts[grp]
     # live rows in a_cat: the groups are contiguous, empty groups take no rows, so they are rows [0, total)
+    a_rows, none = a_cat[:total].to(lora_A.dtype), None
+    if on_device or min(ids) < 0:
+        # rows of a padding group (expert -1) have no delta: what they hold, and what comes back through them, stays out of
+        # the factors' gradients whatever it is
+        none = (experts < 0)[grp][:, None]
+        experts = experts.clamp_min(0)
+        a_rows = a_rows.masked_fill(none, 0)
     x = torch.zeros(len(live), widest, a_cat.shape[1], dtype=lora_A.dtype, device=dev)
-    x[grp, pos] = a_cat[:total].to(lora_A.dtype)
+    x[grp, pos] = a_rows
     low = torch.bmm(x, lora_A[experts].transpose(1, 2))                        # [G, widest, r]
     d = scaling * torch.bmm(low, lora_B[experts].transpose(1, 2))              # [G, widest, N]
     out = torch.zeros(a_cat.shape[0], lora_B.shape[1], dtype=d.dtype, device=dev)
-    out[:total] = d[grp, pos]
+    out[:total] = d[grp, pos] if none is None else d[grp, pos].masked_fill(none, 0)
     return out
 
 

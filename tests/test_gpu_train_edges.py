@@ -72,6 +72,32 @@ def test_rows_without_an_expert_have_no_gradient(product, kernel):
         assert torch.equal(torch.autograd.grad(y, x, go)[0], want)
 
 
+@pytest.mark.parametrize("on_device", [False, True])
+def test_ffn_with_factors_and_padding_groups(on_device):
+    """Rows of padding groups hold unwritten memory between the products: none of it reaches a gradient."""
+    E, K, h, N, r = 3, 128, 64, 128, 4
+    g = gen(15)
+    gu, dn = synth.nf4_stack(E, 2 * h, K, g, scale=0.08, device=DEV), synth.nf4_stack(E, N, h, g, scale=0.08, device=DEV)
+    factors = [0.1 * torch.randn(*s, generator=g) for s in ((E, r, K), (E, 2 * h, r), (E, r, h), (E, N, r))]
+    x, go = (torch.randn(n, d, generator=g).to(torch.bfloat16) for n, d in ((40, K), (40, N)))
+    sizes, ids = [10, 14, 16], [1, -1, 2]
+    keep = torch.cat((torch.arange(10), torch.arange(24, 40)))
+
+    def grads(x, go, sizes, ids):
+        leaves = [t.to(DEV).requires_grad_() for t in (x, *factors)]
+        stale = [torch.full((40, n), float("nan"), dtype=torch.bfloat16, device=DEV) for n in (h, 2 * h, N, K) for _ in range(3)]
+        del stale
+        y = Q.ffn_4bit_grouped_train(leaves[0], *gu, *dn, sizes, ids, lora_gu=leaves[1:3], lora_dn=leaves[3:])
+        return torch.autograd.grad(y, leaves, go.to(DEV))
+
+    go[10:24] = 0                                             # the caller leaves the padding's result alone
+    tables = (torch.tensor(sizes, device=DEV), torch.tensor(ids, device=DEV)) if on_device else (sizes, ids)
+    got, want = grads(x, go, *tables), grads(x[keep], go[keep], [10, 16], [1, 2])
+    assert not got[0][10:24].any()
+    for a, b in zip((got[0][keep.to(DEV)], *got[1:]), want):
+        assert torch.isfinite(a).all() and float((a.double() - b.double()).norm()) <= 1e-5 * float(b.double().norm())
+
+
 @pytest.mark.parametrize("product", ["gemm_4bit_grouped_train", "gemm_mxfp4_grouped_train", "gemm_mxfp4_grouped_w4a4_train"])
 def test_products_of_no_rows(product):
     stack = (synth.nf4_stack if "4bit" in product else synth.mxfp4_stack)(2, 20, 128, gen(13), device=DEV)
