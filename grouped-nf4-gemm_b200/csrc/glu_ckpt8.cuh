@@ -8,9 +8,9 @@
 //     silu:     act = gate s(gate) up,                      s the logistic function
 //     gpt-oss:  act = (up~ + 1) gate~ s(1.702 gate~), gate~ = min(gate, 7), up~ = clamp(up, -7, 7); no gradient beyond
 //
-// The product v * (127 / max|v|) is taken exactly before it is rounded to a whole number.  Where a value lies half way between two
-// codes (half of the block's maximum is 63.5 steps) the rounding of 127 / max decides, so that another way to write the
-// same formula may take the other of the two, which is as near.
+// The product v * (127 / max|v|) is taken exactly before it is rounded to a whole number.  Where a value lies half way
+// between two codes (half of the block's maximum is 63.5 steps) the rounding of 127 / max decides, so that another way to
+// write the same formula may take the other of the two, which is as near.
 //
 // A step of the block's maximum / 127 costs at most half a step, 0.4 % of the block's largest magnitude, and halves what
 // a layer keeps between the passes (2 bytes + 1/8 instead of 4 per pair).  A block whose maximum is below 2^-100 is kept

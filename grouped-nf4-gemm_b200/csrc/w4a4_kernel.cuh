@@ -39,9 +39,10 @@
 // 13 us.  (The W4A16 kernels here: 252, 1115, 218 us for the first three, 12 for the last.)
 // What bounds it: with few rows the issuer, 635 cycles per stage at about 31 per tcgen05 instruction and 130 per completed
 // barrier (without the MMAs and copies 47 us of the 55, the rate of a plain copy); with 256 rows the tiles' way from L2 into
-// shared memory, 45 to 49 bytes per cycle and SM (without MMAs and copies 58 us of 70; in pairs, measured on 8 x 2048 rows, K = 7168,
-// which the rule gives to single CTAs, 170 of 203), and the power limit; scales take 3 to 9 % (rows on 16 bytes the less).  A launch reaches its first MMA after
-// 3.5 us with few rows (1.6 of them launch and group table) and after 6 with many, when every SM loads at once.
+// shared memory, 45 to 49 bytes per cycle and SM (without MMAs and copies 58 us of 70; in pairs, measured on 8 x 2048 rows,
+// K = 7168, which the rule gives to single CTAs, 170 of 203), and the power limit; scales take 3 to 9 % (rows on 16 bytes the
+// less).  A launch reaches its first MMA after 3.5 us with few rows (1.6 of them launch and group table) and after 6 with
+// many, when every SM loads at once.
 #pragma once
 
 #include "tensor_fwd_kernel.cuh"

@@ -215,8 +215,8 @@ def route_topk_train(logits: torch.Tensor, k: int, mode: int = 0, norm: bool = F
         z_loss       = mean_t logsumexp(logits_t)^2
 
     and both are 0 when no token counts.  A masked token is routed and weighted all the same (a batch's padding; mask
-    its result, not its route): group sizes come from ``idx``, not from ``counts``.  A token whose logits are all -inf gets weights 0 and no gradient.  On a GPU one kernel
-    each way (E <= 1024, k <= 32); on the CPU the same in tensor operations."""
+    its result, not its route): group sizes come from ``idx``, not from ``counts``.  A token whose logits are all -inf gets
+    weights 0 and no gradient.  On a GPU one kernel each way (E <= 1024, k <= 32); on the CPU the same in tensor operations."""
     if logits.dim() != 2:
         raise ValueError(f"logits must be [tokens, experts], got shape {tuple(logits.shape)}")
     if logits.dtype not in _ROUTE_DTYPES:

@@ -339,8 +339,8 @@ def ffn_4bit_grouped_train(a_cat, packed_gu, absmax_gu, packed_dn, absmax_dn, si
 def ffn_mxfp4_grouped_train(a_cat, blocks_gu, scales_gu, blocks_dn, scales_dn, sizes, expert_ids, *, act: str = "gpt_oss",
                             bias_gu=None, row_expert=None, rows: str = "bf16"):
     """The MXFP4 counterpart on frozen stacks; ``bias_gu`` (bf16 ``[E, N_gu]``, ``act="gpt_oss"``) by ``row_expert [T]``.  The
-    activation is ``glu_train``: the result is not the bits of ``ffn_mxfp4_grouped``.  ``rows="mxfp4"`` multiplies MXFP4 rows forward
-    (``gemm_mxfp4_grouped_w4a4_train``), ``"bf16"`` the rows as they are."""
+    activation is ``glu_train``: the result is not the bits of ``ffn_mxfp4_grouped``.  ``rows="mxfp4"`` multiplies MXFP4 rows
+    forward (``gemm_mxfp4_grouped_w4a4_train``), ``"bf16"`` the rows as they are."""
     if rows not in ("bf16", "mxfp4"):
         raise ValueError("rows is 'bf16' or 'mxfp4'")
     product = gemm_mxfp4_grouped_train if rows == "bf16" else gemm_mxfp4_grouped_w4a4_train

@@ -461,7 +461,8 @@ int gnf4b_glu_quantize_mxfp4(const void* gate_up, int64_t rows, int64_t h, int a
  * by group; W / S, group_offsets, expert_ids, max_rows, status_word as in gnf4b_gemm_grouped with GNF4B_FMT_MXFP4
  * (max_rows only shapes the tiles here: understating it costs speed, not rows).  x_blocks and W start on 16 bytes and
  * W's strides are positive multiples of 16 bytes (GNF4B_EUNSUPPORTED otherwise; the stride of a dimension of one is not
- * used); the scales may have any alignment and any non-negative strides; T and N up to 2^31 - 257.  A scale byte of 255 is NaN here, as the OCP format defines it.
+ * used); the scales may have any alignment and any non-negative strides; T and N up to 2^31 - 257.  A scale byte of 255 is
+ * NaN here, as the OCP format defines it.
  * Rows that belong to no group, or to a padding group, are left as they were. */
 int gnf4b_gemm_grouped_w4a4(const uint8_t* x_blocks, const uint8_t* x_scales, int64_t T,
                             const uint8_t* W, int64_t w_stride_e, int64_t w_stride_n,
@@ -483,7 +484,8 @@ int gnf4b_w4a4_plan(int64_t T, int32_t G, int64_t N, int64_t K, int32_t max_rows
  *   balance_loss = E sum_e (counts_e / (n k)) mean_t p[t, e]   (1 when even)
  *   z_loss = mean_t (log sum_e exp logits[t, e])^2;   n_tokens = n as a float;   n = 0: both losses 0
  * Masked tokens are routed all the same.  A token whose logits are all -inf gets weights 0.  A NaN logit is chosen after
- * every other one; the token's weights (in mode 1 only if it was chosen) and, if it counts, the losses are NaN.  lse [T] is kept for the backward pass.
+ * every other one; the token's weights (in mode 1 only if it was chosen) and, if it counts, the losses are NaN.  lse [T]
+ * is kept for the backward pass.
  * scratch: gnf4b_route_train_scratch_bytes(T, E) bytes (8-byte aligned, any content; 0 for small batches), not shared by
  * calls that overlap.  Deterministic (no floating-point atomics).
  * gnf4b_route_train_bwd: grad [T, E] (contiguous, the logits' type) from g_weights [T, k] (fp32), g_balance and g_z
