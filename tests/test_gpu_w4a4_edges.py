@@ -46,3 +46,51 @@ def test_odd_strides_of_dimensions_of_one():
                                          ws.clone(memory_format=torch.contiguous_format), sizes, ids)
         assert torch.equal(M.gemm_mxfp4_grouped_w4a4(xb, xs, wb, ws, sizes, ids), want)
     assert nf4_grouped.last_status(DEV) == 0
+
+
+def test_two_host_threads_at_once():
+    """Each thread on its own stream, over products of very different tiles, the quantiser, the router and the GLU."""
+    import threading
+
+    import ep_moe
+    import nf4_qlora
+
+    K, E, N = 1312, 3, 300
+    wb, ws = packed((E, N), K, 5)
+    batches = []
+    for i, sizes in enumerate(([1, 1], [400, 3], [17, 0, 60], [130], [1, 300])):
+        x = torch.randn(sum(sizes), K, generator=gen(20 + i)).to(torch.bfloat16).to(DEV)
+        batches.append((x, sizes, [(i + j) % E for j in range(len(sizes))]))
+
+    def one(x, sizes, ids):
+        y = M.gemm_mxfp4_grouped_w4a4(*M.quantize_mxfp4(x), wb, ws, sizes, ids)
+        logits = y.float().clamp(-4, 4).requires_grad_()
+        r = ep_moe.route_topk_train(logits, 5)
+        grad, = torch.autograd.grad((r.weights, r.z_loss), logits, (torch.ones_like(r.weights), torch.ones_like(r.z_loss)))
+        gu = y.clamp(-4, 4).requires_grad_()
+        out = nf4_qlora.glu_train(gu, "silu")
+        return y, r.idx, r.balance_loss.detach(), grad, out.detach(), torch.autograd.grad(out, gu, torch.ones_like(out))[0]
+
+    want = [one(*b) for b in batches]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(first):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for i in range(60):
+                    b = (first + i * (1 + first)) % len(batches)
+                    got = one(*batches[b])
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(p, q) for p, q in zip(got, want[b])):
+                        wrong.append((first, i, b))
+        except Exception as e:                          # a thread's exception would be lost
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(t,)) for t in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong and nf4_grouped.last_status(DEV) == 0
